@@ -39,6 +39,12 @@ SIGNATURES = {
     "haste_b200_layer_norm_gru_backward": [_i] * 6 + [_p] * 26,
     "haste_b200_layer_norm_indrnn_forward": [_i] * 6 + [_p] * 9 + [_f, _p, _p],
     "haste_b200_layer_norm_indrnn_backward": [_i] * 6 + [_p] * 18,
+    "haste_b200_causal_conv1d_forward": [_p, _p],
+    "haste_b200_causal_conv1d_backward": [_p, _p],
+    "haste_b200_selective_scan_forward": [_p, _p],
+    "haste_b200_selective_scan_backward": [_p, _p],
+    "haste_b200_fused_norm_forward": [_p, _p],
+    "haste_b200_fused_norm_backward": [_p, _p],
     "haste_b200_gemm": [_i] * 4 + [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _i, _p],
     "haste_b200_set_recurrence_path": [_i],
     "haste_b200_set_gemm_path": [_i],
@@ -51,7 +57,9 @@ SIGNATURES = {
     "haste_b200_profile_read": [_p, _i],
 }
 OTHER_SYMBOLS = ["haste_b200_last_error", "haste_b200_version", "haste_b200_launch_count",
-                 "haste_b200_sm_budget"]
+                 "haste_b200_sm_budget", "haste_b200_causal_conv1d_scratch",
+                 "haste_b200_selective_scan_checkpoints", "haste_b200_selective_scan_scratch",
+                 "haste_b200_fused_norm_scratch"]
 
 _lib = None
 

@@ -81,9 +81,10 @@ def _build_pybind(target, link, force):
     import torch
     from torch.utils import cpp_extension as ce
     src = target[:-3] + ".cc"
-    header = os.path.join(HERE, "..", "include", "haste_b200.h")
+    headers = [os.path.join(HERE, "..", "include", "haste_b200.h")]
+    headers += [os.path.join(TORCH_EXT_DIR, f) for f in os.listdir(TORCH_EXT_DIR) if f.endswith(".h")]
     if (not force and os.path.exists(target) and os.path.exists(LIB)
-            and os.path.getmtime(target) > max(os.path.getmtime(src), os.path.getmtime(header))):
+            and os.path.getmtime(target) > max(map(os.path.getmtime, [src, *headers]))):
         return target
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     incs = ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(HERE, "..", "include"),

@@ -7,6 +7,18 @@
 #include "cells.cuh"
 
 namespace hb {
+// The state space operators take the header's argument blocks as they are.
+int causal_conv1d_forward(const haste_b200_causal_conv1d& a, cudaStream_t s);
+int causal_conv1d_backward(const haste_b200_causal_conv1d& a, cudaStream_t s);
+long long causal_conv1d_scratch(const haste_b200_causal_conv1d& a);
+int selective_scan_forward(const haste_b200_selective_scan& a, cudaStream_t s);
+int selective_scan_backward(const haste_b200_selective_scan& a, cudaStream_t s);
+long long selective_scan_checkpoints(const haste_b200_selective_scan& a);
+long long selective_scan_scratch(const haste_b200_selective_scan& a, bool backward);
+int fused_norm_forward(const haste_b200_fused_norm& a, cudaStream_t s);
+int fused_norm_backward(const haste_b200_fused_norm& a, cudaStream_t s);
+long long fused_norm_scratch(const haste_b200_fused_norm& a);
+
 const char* last_error();
 long long launch_count();
 static std::atomic<int> g_rec_path{HASTE_B200_PATH_AUTO};
@@ -325,6 +337,36 @@ int haste_b200_layer_norm_indrnn_backward(
   IndrnnBwd a{dtype, transposed_inputs, T, N, C, H, W, u, b, x, h, dh_new, dx, dW, du, db, dh,
               workspace, zoneout_mask, gamma, dgamma, act_Wx, cache_Wx};
   return indrnn_backward(a, (cudaStream_t)stream);
+}
+
+// The state space operators work on the caller's scratch alone, so they need no lock.
+#define HB_STATE_SPACE(op)                                                                        \
+  int haste_b200_##op##_forward(const haste_b200_##op* args, void* stream) {                      \
+    HB_TRY(report_timeout());                                                                     \
+    HB_REQUIRE(args, "null pointer");                                                             \
+    return op##_forward(*args, (cudaStream_t)stream);                                             \
+  }                                                                                               \
+  int haste_b200_##op##_backward(const haste_b200_##op* args, void* stream) {                     \
+    HB_TRY(report_timeout());                                                                     \
+    HB_REQUIRE(args, "null pointer");                                                             \
+    return op##_backward(*args, (cudaStream_t)stream);                                            \
+  }
+HB_STATE_SPACE(causal_conv1d)
+HB_STATE_SPACE(selective_scan)
+HB_STATE_SPACE(fused_norm)
+#undef HB_STATE_SPACE
+
+long long haste_b200_causal_conv1d_scratch(const haste_b200_causal_conv1d* args) {
+  return args ? causal_conv1d_scratch(*args) : 0;
+}
+long long haste_b200_selective_scan_checkpoints(const haste_b200_selective_scan* args) {
+  return args ? selective_scan_checkpoints(*args) : 0;
+}
+long long haste_b200_selective_scan_scratch(const haste_b200_selective_scan* args, int backward) {
+  return args ? selective_scan_scratch(*args, backward != 0) : 0;
+}
+long long haste_b200_fused_norm_scratch(const haste_b200_fused_norm* args) {
+  return args ? fused_norm_scratch(*args) : 0;
 }
 
 int haste_b200_gemm(int dtype, int M, int N, int K, const void* a, long long a_rs, long long a_cs,

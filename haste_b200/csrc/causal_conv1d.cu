@@ -1,0 +1,322 @@
+// Short causal depthwise convolution along time with bias and SiLU, forward and backward.
+//
+//   p_t = bias + sum_k w_k x_{t-(W-1)+k},  y_t = silu(p_t)
+//
+// A stream over x and y (backward: x and dy in, dx out): 2 W + 5 operations a value against 4 to 8
+// bytes, so HBM bounds it.  A thread owns V neighbouring channels and walks a chunk of steps with
+// the last W - 1 inputs in registers; a group of steps is loaded ahead of its arithmetic.
+#include <algorithm>
+
+#include "state_space.cuh"
+
+namespace hb {
+namespace {
+
+using namespace ss;
+
+constexpr int GROUP = 4;  // steps whose loads go out together
+
+template <typename T>
+struct ConvArgs {
+  int T_, N, D, chunk, dtiles;
+  bool param_f32, silu;
+  Seq<const T> x, dy;
+  Seq<T> y, dx;
+  const void *w, *b;
+  const T* state;
+  T* final_state;
+  const long long* lengths;
+  const T* dfinal;
+  T* dstate;
+  float* part;
+  int items, parts;
+};
+
+// The input at a step of the row, the initial state's rows before it (step >= -(W-1)).
+template <typename T, int V, int W>
+__device__ __forceinline__ void input_at(const ConvArgs<T>& a, int t, int len, int n, int d, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  if (t >= 0) {
+    if (t < len) load<T, V>(a.x.at(t, n) + d, v);
+  } else if (a.state) {
+    load<T, V>(a.state + ((long long)n * (W - 1) + t + W - 1) * a.D + d, v);
+  }
+}
+
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
+  const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
+  const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
+  if (d >= a.D) return;
+  const int len = row_length(a.lengths, n, a.T_);
+  const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk);
+  float w[W][V], b[V], xs[W][V];  // xs: the window, its last row the step at hand
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    b[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k][i] = ldp<T>(a.w, a.param_f32, (long long)(d + i) * W + k);
+  }
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
+  for (int t = t0; t < t1; t += GROUP) {
+    Pack<T, V> in[GROUP];
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u)
+      if (t + u < t1 && t + u < len) in[u] = *reinterpret_cast<const Pack<T, V>*>(a.x.at(t + u, n) + d);
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u) {
+      if (t + u >= t1) break;
+      const bool live = t + u < len;
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) xs[k][i] = xs[k + 1][i];
+        xs[W - 1][i] = live ? ld(&in[u].v[i]) : 0.f;
+        float p = b[i];
+#pragma unroll
+        for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
+        y[i] = !live ? 0.f : a.silu ? silu(p) : p;
+      }
+      store<T, V>(a.y.at(t + u, n) + d, y);
+    }
+  }
+  // The last W - 1 inputs of the row.  Row k comes from row k + len of the state at the earliest, so
+  // in ascending order the two may be one buffer; what this thread has read above is in registers,
+  // and no other thread reads these channels' state (a chunk is longer than W - 1 steps).
+  if (c == 0 && a.final_state) {
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      float v[V];
+      input_at<T, V, W>(a, len - (W - 1) + k, len, n, d, v);
+      store<T, V>(a.final_state + ((long long)n * (W - 1) + k) * a.D + d, v);
+    }
+  }
+}
+
+// dx_t = sum_k w_k dp_{t+(W-1)-k} with dp = dy silu'(p): a thread walks its chunk and W - 1 steps
+// beyond it, recomputes p, and emits dx W - 1 steps behind.  dw and db are summed in registers over
+// the chunks that a block takes in turn; its partial rows are added in a fixed order afterwards.
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
+  const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
+  const int part = blockIdx.x / a.dtiles;
+  if (d >= a.D) return;
+  float w[W][V], b[V], dw[W][V], db[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    b[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
+    db[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      w[k][i] = ldp<T>(a.w, a.param_f32, (long long)(d + i) * W + k);
+      dw[k][i] = 0.f;
+    }
+  }
+  for (int item = part; item < a.items; item += a.parts) {
+    const int n = item % a.N, c = item / a.N;
+    const int len = row_length(a.lengths, n, a.T_);
+    const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk);
+    float xs[W][V], dp[W][V];
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) dp[k][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
+    for (int t = t0; t < t1 + W - 1; t += GROUP) {
+      Pack<T, V> in[GROUP], gr[GROUP];
+#pragma unroll
+      for (int u = 0; u < GROUP; ++u)
+        if (t + u < t1 + W - 1 && t + u < len) {
+          in[u] = *reinterpret_cast<const Pack<T, V>*>(a.x.at(t + u, n) + d);
+          gr[u] = *reinterpret_cast<const Pack<T, V>*>(a.dy.at(t + u, n) + d);
+        }
+#pragma unroll
+      for (int u = 0; u < GROUP; ++u) {
+        if (t + u >= t1 + W - 1) break;
+        const bool live = t + u < len, mine = live && t + u < t1;
+        const int te = t + u - (W - 1);  // the step whose dx is complete now
+        float dx[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k) {
+            xs[k][i] = xs[k + 1][i];
+            dp[k][i] = dp[k + 1][i];
+          }
+          xs[W - 1][i] = live ? ld(&in[u].v[i]) : 0.f;
+          float g = live ? ld(&gr[u].v[i]) : 0.f;
+          if (a.silu) {
+            float p = b[i];
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
+            // a step behind the row's end has g = 0, and p there comes from the row's own values
+            g = live ? g * silu_slope(p, sigmoid(p)) : 0.f;
+          }
+          dp[W - 1][i] = g;
+          if (mine) {
+            db[i] += g;
+#pragma unroll
+            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, xs[k][i], dw[k][i]);
+          }
+          dx[i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < W; ++k) dx[i] = fmaf(w[k][i], dp[W - 1 - k][i], dx[i]);
+        }
+        const bool before = te < 0;  // a row of the initial state
+        if (before ? c != 0 : te < t0) continue;
+        if (a.dfinal && te >= len - (W - 1) && te < len) {
+          float f[V];
+          load<T, V>(a.dfinal + ((long long)n * (W - 1) + te - len + W - 1) * a.D + d, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) dx[i] += f[i];
+        }
+        if (!before) {
+          if (a.dx.p) store<T, V>(a.dx.at(te, n) + d, dx);
+        } else if (a.dstate) {
+          store<T, V>(a.dstate + ((long long)n * (W - 1) + te + W - 1) * a.D + d, dx);
+        }
+      }
+    }
+  }
+  // partial row of this block: [D][W] of dw, then [D] of db
+  float* row = a.part + (long long)part * a.D * (W + 1);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) row[(long long)(d + i) * W + k] = dw[k][i];
+    row[(long long)a.D * W + d + i] = db[i];
+  }
+}
+
+int check(const haste_b200_causal_conv1d& a, bool backward) {
+  HB_REQUIRE(storage_dtype(a.dtype), "dtype");
+  HB_REQUIRE(a.param_dtype == HASTE_B200_F32 || a.param_dtype == a.dtype, "param_dtype");
+  HB_REQUIRE(a.T >= 0 && a.N >= 0 && a.D >= 0, "T,N,D");
+  HB_REQUIRE(a.W >= 2 && a.W <= 4, "W must be 2, 3 or 4");
+  HB_REQUIRE((long long)a.D * (a.W + 1) < (1LL << 31), "D");
+  if (a.N == 0 || a.D == 0) return HASTE_B200_OK;
+  HB_REQUIRE(a.weight, "null pointer");
+  HB_REQUIRE(a.T == 0 || (a.x.data && (backward ? a.dy.data != nullptr : a.y.data != nullptr)), "null pointer");
+  HB_REQUIRE(!backward || (a.dweight && a.scratch), "null pointer");
+  return HASTE_B200_OK;
+}
+
+// Channels per thread: as many as 16 bytes hold, less where a width, a stride or a start forbids it.
+// Half as many in the backward pass, whose windows and sums take twice the registers.
+int width(const haste_b200_causal_conv1d& a, bool backward) {
+  const int e = (int)dtype_size(a.dtype);
+  for (int v = backward ? 4 : 16 / e; v > 1; v /= 2) {
+    bool ok = a.D % v == 0 && aligned(a.x, e, v * e) && aligned(a.state, v * e) && aligned(a.final_state, v * e);
+    ok &= backward ? aligned(a.dy, e, v * e) && aligned(a.dx, e, v * e) && aligned(a.dfinal_state, v * e) &&
+                         aligned(a.dstate, v * e)
+                   : aligned(a.y, e, v * e);
+    if (ok) return v;
+  }
+  return 1;
+}
+
+struct Shape {
+  int threads, dtiles, chunk, chunks;
+  Shape(const haste_b200_causal_conv1d& a, int v) {
+    const int lanes = ceil_div(a.D, v);
+    threads = std::min(128, ceil_div(lanes, 32) * 32);
+    dtiles = ceil_div(lanes, threads);
+    // A chunk reads W - 1 steps twice, so long chunks while there are threads to fill the GPU.
+    chunk = 64;
+    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < 1024LL * sm_count()) chunk /= 2;
+    chunks = std::max(1, ceil_div(a.T, chunk));
+  }
+  long long items(int N) const { return (long long)chunks * N; }
+};
+
+// Blocks of the backward pass that share a row of partial sums: about eight per SM.
+int parts(const haste_b200_causal_conv1d& a, const Shape& s) {
+  return (int)std::max(1LL, std::min(s.items(a.N), (long long)ceil_div(8LL * sm_count(), s.dtiles)));
+}
+
+template <typename T>
+ConvArgs<T> pack(const haste_b200_causal_conv1d& a, const Shape& s) {
+  ConvArgs<T> k;
+  k.T_ = a.T; k.N = a.N; k.D = a.D; k.chunk = s.chunk; k.dtiles = s.dtiles;
+  k.param_f32 = a.param_dtype == HASTE_B200_F32;
+  k.silu = a.silu != 0;
+  k.x = Seq<const T>(a.x); k.y = Seq<T>(a.y); k.dy = Seq<const T>(a.dy); k.dx = Seq<T>(a.dx);
+  k.w = a.weight; k.b = a.bias;
+  k.state = static_cast<const T*>(a.state);
+  k.final_state = static_cast<T*>(a.final_state);
+  k.lengths = a.lengths;
+  k.dfinal = static_cast<const T*>(a.dfinal_state);
+  k.dstate = static_cast<T*>(a.dstate);
+  k.part = a.scratch;
+  k.items = (int)s.items(a.N);
+  k.parts = parts(a, s);
+  return k;
+}
+
+template <typename T, int V, int W>
+int launch(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t st) {
+  const Shape s(a, V);
+  HB_REQUIRE(s.items(a.N) * s.dtiles < (1LL << 31), "T*N too large");
+  const ConvArgs<T> k = pack<T>(a, s);
+  if (backward) {
+    if constexpr (V <= 4) conv_bwd<T, V, W><<<k.parts * s.dtiles, s.threads, 0, st>>>(k);
+  } else {
+    conv_fwd<T, V, W><<<k.items * s.dtiles, s.threads, 0, st>>>(k);
+  }
+  HB_LAUNCH_OK();
+  count_launch(1);
+  if (!backward) return HASTE_B200_OK;
+  SumJobs jobs;
+  jobs.add(a.dweight, 0, 1, a.D * W, a.param_dtype);
+  jobs.add(a.dbias, (long long)a.D * W, 1, a.D, a.param_dtype);
+  return sum_parts(a.scratch, k.parts, (long long)a.D * (W + 1), jobs, st);
+}
+
+template <typename T, int V>
+int by_taps(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t s) {
+  if (a.W == 4) return launch<T, V, 4>(a, backward, s);
+  if (a.W == 3) return launch<T, V, 3>(a, backward, s);
+  return launch<T, V, 2>(a, backward, s);
+}
+
+template <typename T>
+int by_width(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t s) {
+  switch (width(a, backward)) {
+    case 8: if constexpr (sizeof(T) == 2) return by_taps<T, 8>(a, backward, s);
+    case 4: return by_taps<T, 4>(a, backward, s);
+    case 2: return by_taps<T, 2>(a, backward, s);
+    default: return by_taps<T, 1>(a, backward, s);
+  }
+}
+
+int run(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t s) {
+  HB_TRY(check(a, backward));
+  if (a.N == 0 || a.D == 0) return HASTE_B200_OK;
+  if (a.dtype == HASTE_B200_F32) return by_width<float>(a, backward, s);
+  if (a.dtype == HASTE_B200_BF16) return by_width<__nv_bfloat16>(a, backward, s);
+  return by_width<__half>(a, backward, s);
+}
+
+}  // namespace
+
+int causal_conv1d_forward(const haste_b200_causal_conv1d& a, cudaStream_t s) {
+  ProfScope p(PH_OTHER, s);
+  return run(a, false, s);
+}
+int causal_conv1d_backward(const haste_b200_causal_conv1d& a, cudaStream_t s) {
+  ProfScope p(PH_OTHER, s);
+  return run(a, true, s);
+}
+long long causal_conv1d_scratch(const haste_b200_causal_conv1d& a) {
+  // (enough for every width: the pointers that decide on it may not be there yet)
+  if (a.N <= 0 || a.D <= 0 || a.T < 0) return 0;
+  long long rows = 0;
+  for (int v = 1; v <= 4; v *= 2) rows = std::max(rows, (long long)parts(a, Shape(a, v)));
+  return rows * a.D * (a.W + 1);
+}
+
+}  // namespace hb

@@ -534,6 +534,47 @@ def layer_norm_indrnn_backward(x, kernel, recurrent_scale, bias, gamma, zoneout_
     return [dx, dh, dW, du, db, dgamma]
 
 
+# ---------------------------------------------------------------- state space operators
+# Without a counterpart in the reference: the tensor-level forms of `haste_b200.ssm`, which says what
+# they compute.  Sequences are [T,N,...] views with any strides but 1 along the last axis; an output
+# lies in memory like the sequence that it belongs to.  Optional tensors are None.
+def causal_conv1d_forward(x, weight, bias=None, state=None, lengths=None, silu=True):
+    """[y, final_state]: x [T,N,D], weight [D,W], bias [D], state [N,W-1,D]."""
+    return list(_C.native().causal_conv1d_forward(x, weight, bias, state, lengths, silu, None))
+
+
+def causal_conv1d_backward(x, weight, bias, state, lengths, silu, dy, dfinal_state=None):
+    """[dx, dweight, dbias, dstate]; the last two are None where the tensor is."""
+    return list(_C.native().causal_conv1d_backward(x, weight, bias, state, lengths, silu, dy, dfinal_state))
+
+
+def selective_scan_forward(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, lengths=None,
+                           softplus=True, training=False):
+    """[y, final_state, checkpoints]: x, dt, z [T,N,D], A [D,S], B, C [T,N,G,S], D, dt_bias [D],
+    state [N,D,S]; `checkpoints` (None unless training) is for the backward pass."""
+    return list(_C.native().selective_scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus,
+                                                   training, None))
+
+
+def selective_scan_backward(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, checkpoints, dy,
+                            dfinal_state=None):
+    """[dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dstate]; None where the tensor is."""
+    return _C.native().selective_scan_backward(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus,
+                                               checkpoints, dy, dfinal_state)
+
+
+def fused_norm_forward(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1e-5,
+                       layer_norm=False, training=False):
+    """[y, r, statistics]: x, gate, residual [T,N,H]; r is None without a residual, `statistics`
+    (None unless training) is for the backward pass."""
+    return list(_C.native().fused_norm_forward(x, weight, bias, gate, residual, scale, eps, layer_norm, training))
+
+
+def fused_norm_backward(x, weight, bias, gate, residual, scale, eps, layer_norm, statistics, dy, dr=None):
+    """[dx, dweight, dbias, dgate, dresidual, dscale]; None where the tensor is."""
+    return _C.native().fused_norm_backward(x, weight, bias, gate, residual, scale, eps, layer_norm, statistics, dy, dr)
+
+
 # ---------------------------------------------------------------- helpers for tests/bench
 def gemm(a, b, out=None, accumulate=False):
     """out (+)= a @ b for 2-D CUDA tensors with arbitrary strides (views allowed)."""

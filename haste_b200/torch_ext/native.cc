@@ -40,7 +40,9 @@ bool has_c(int cell) { return cell == LSTM || cell == LN_LSTM; }
   X(gru_forward) X(gru_backward) X(indrnn_forward) X(indrnn_backward) X(layer_norm_lstm_forward)     \
   X(layer_norm_lstm_backward) X(layer_norm_gru_forward) X(layer_norm_gru_backward)                   \
   X(layer_norm_indrnn_forward) X(layer_norm_indrnn_backward) X(lstm_forward_iterate)                 \
-  X(gru_forward_iterate)
+  X(gru_forward_iterate) X(causal_conv1d_forward) X(causal_conv1d_backward) X(causal_conv1d_scratch)   \
+  X(selective_scan_forward) X(selective_scan_backward) X(selective_scan_checkpoints)                 \
+  X(selective_scan_scratch) X(fused_norm_forward) X(fused_norm_backward) X(fused_norm_scratch)
 struct Library {
 #define HB_FIELD(f) decltype(&haste_b200_##f) f = nullptr;
   HB_FUNCTIONS(HB_FIELD)
@@ -490,6 +492,8 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> forward(
   return {batch_first ? y.transpose(0, 1) : y, final_state(y), cf};
 }
 
+#include "native_state_space.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -502,4 +506,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("load", &load);
   m.def("forward", &forward, py::call_guard<py::gil_scoped_release>());
+  state_space::bind(m);
 }

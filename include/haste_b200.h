@@ -303,6 +303,101 @@ int haste_b200_layer_norm_indrnn_backward(
     void* dx, void* dW, void* du, void* db, void* dgamma, void* dh, void* workspace,
     const void* act_Wx, const void* cache_Wx, const void* zoneout_mask, void* stream);
 
+/* ---- Selective state space operators ------------------------------------ */
+/* No counterpart in the reference.  The parts of a state space block, next to the recurrences
+ * above: a short causal convolution along time, a scan whose decay and input depend on the data,
+ * and a norm fused with the block's gate and residual.
+ *
+ * Their arguments come in one block each, zeroed by the caller before it is filled; a pointer that
+ * is NULL means that the tensor is absent.  A sequence is a view: element (t,n,j) lies at
+ * data[t * t_stride + n * n_stride + j] (strides in elements, j unit-strided), so halves of a
+ * projection and batch-first tensors are taken as they lie.  Outputs must not overlap inputs,
+ * except where said.  dtype is the storage of all sequences (HASTE_B200_F32, BF16 or F16),
+ * arithmetic and sums are fp32.  `lengths` [N] (device, 64-bit) ends each row early: from step
+ * lengths[n] on (values are clamped to 0..T) inputs are not read, outputs are zero, and the final
+ * state is the one after lengths[n] steps.
+ * These entry points allocate nothing and keep no state: scratch comes from the caller, so calls
+ * may be captured into graphs and issued on any number of streams at once. */
+typedef struct {
+  void* data;
+  long long t_stride, n_stride;
+} haste_b200_sequence;
+
+/* y_t[d] = act(bias[d] + sum_k weight[d,k] x_{t-(W-1)+k}[d]), act = SiLU if `silu`, else identity.
+ * The steps before the first are `state` (zeros if NULL).  W is 2, 3 or 4.
+ *   x, y [T,N,D]  weight [D,W]  bias [D]  state, final_state [N,W-1,D] dense, dtype
+ *   final_state may be the same buffer as state.
+ * backward: dy, dx [T,N,D], dfinal_state, dstate [N,W-1,D], dweight, dbias like their parameters;
+ * dx, dstate and dbias may be NULL.  scratch: haste_b200_causal_conv1d_scratch() floats. */
+typedef struct {
+  int dtype, param_dtype; /* param_dtype: of weight, bias and their gradients; F32 or dtype */
+  int T, N, D, W, silu;
+  haste_b200_sequence x, y, dy, dx;
+  const void *weight, *bias, *state;
+  void* final_state;
+  const long long* lengths;
+  const void* dfinal_state;
+  void *dstate, *dweight, *dbias;
+  float* scratch;
+} haste_b200_causal_conv1d;
+int haste_b200_causal_conv1d_forward(const haste_b200_causal_conv1d* args, void* stream);
+int haste_b200_causal_conv1d_backward(const haste_b200_causal_conv1d* args, void* stream);
+long long haste_b200_causal_conv1d_scratch(const haste_b200_causal_conv1d* args);
+
+/* delta = softplus(dt + dt_bias) (without softplus if `softplus` is 0),
+ * h_t[d,s] = exp(delta_t[d] A[d,s]) h_{t-1}[d,s] + delta_t[d] x_t[d] B_t[g,s],  g = d / (D/G),
+ * y_t[d] = (sum_s C_t[g,s] h_t[d,s] + skip[d] x_t[d]) * silu(z_t[d]).
+ *   x, dt, z, y [T,N,D]   B, C [T,N,G,S]: element (t,n,g,s) at t_stride, n_stride and B_g, C_g
+ *   A [D,S], skip [D], dt_bias [D]: float   state, final_state [N,D,S]: float, dense; may be the
+ *   same buffer.  S is 1..128, G divides D.
+ * checkpoints: what the backward pass starts its pieces from, haste_b200_selective_scan_checkpoints()
+ * floats; NULL if there will be none.
+ * backward: reads checkpoints, dy and dfinal_state; writes dx, ddt, dz (if z), dB, dC (sequences
+ * like B and C with dB_g, dC_g), dA, dskip, ddt_bias (float, like their parameters) and dstate
+ * (may be NULL).  scratch: haste_b200_selective_scan_scratch() floats. */
+typedef struct {
+  int dtype, T, N, D, G, S, softplus;
+  haste_b200_sequence x, dt, z, y, B, C;
+  long long B_g, C_g;
+  const float *A, *skip, *dt_bias, *state;
+  float* final_state;
+  const long long* lengths;
+  float* checkpoints;
+  haste_b200_sequence dy, dx, ddt, dz, dB, dC;
+  long long dB_g, dC_g;
+  const float* dfinal_state;
+  float *dA, *dskip, *ddt_bias, *dstate;
+  float* scratch;
+} haste_b200_selective_scan;
+int haste_b200_selective_scan_forward(const haste_b200_selective_scan* args, void* stream);
+int haste_b200_selective_scan_backward(const haste_b200_selective_scan* args, void* stream);
+long long haste_b200_selective_scan_checkpoints(const haste_b200_selective_scan* args);
+/* floats of scratch that the forward (backward != 0: backward) call needs */
+long long haste_b200_selective_scan_scratch(const haste_b200_selective_scan* args, int backward);
+
+/* u = x * silu(gate);  r = residual + scale * u;  y = norm(r) * weight + bias
+ * (norm: root mean square, or mean and variance if `layer_norm`; eps inside the root).
+ *   x, gate, y [T,N,H] dtype   residual, r [T,N,H] residual_dtype (F32 or dtype; without a residual
+ *   pass dtype)   scale, weight, bias [H] param_dtype (F32 or dtype); scale needs a residual
+ *   stats [T,N,2] float: mean (0 without layer_norm) and 1 / deviation; NULL if there will be no
+ *   backward pass.  r may be NULL, or the same buffer as residual.  H is 1..8192.
+ * backward: reads dy and dr (may be NULL: no gradient of r); writes dx, dgate, dresidual, dscale,
+ * dweight, dbias like their tensors.  Any of dx, dgate, dresidual may be NULL.
+ * scratch: haste_b200_fused_norm_scratch() floats. */
+typedef struct {
+  int dtype, residual_dtype, param_dtype, T, N, H, layer_norm;
+  float eps;
+  haste_b200_sequence x, gate, residual, y, r;
+  const void *scale, *weight, *bias;
+  float* stats;
+  haste_b200_sequence dy, dr, dx, dgate, dresidual;
+  void *dscale, *dweight, *dbias;
+  float* scratch;
+} haste_b200_fused_norm;
+int haste_b200_fused_norm_forward(const haste_b200_fused_norm* args, void* stream);
+int haste_b200_fused_norm_backward(const haste_b200_fused_norm* args, void* stream);
+long long haste_b200_fused_norm_scratch(const haste_b200_fused_norm* args);
+
 /* ---- Dense contraction (exposed for tests and benchmarks) --------------- */
 /* C[m,n] (+)= sum_k A(m,k) B(k,n);  A(m,k) at a[m*a_rs + k*a_cs],
  * B(k,n) at b[k*b_rs + n*b_cs], C row-major with leading dimension ldc.
