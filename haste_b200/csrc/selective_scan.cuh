@@ -14,62 +14,144 @@ constexpr int CKPT = 8;  // steps between the states that the forward pass leave
 template <typename T>
 struct Args {
   int T_, N, D, G, S, per, ctiles;  // per: channels of a group, ctiles: blocks that share them out
+  int chunks, chunk;                // pieces of the sequence that blocks work on side by side, steps of one
   bool softplus;
   Seq<const T> x, dt, z, B, C, dy;
   Seq<T> y, dx, ddt, dz, dB, dC;
   long long B_g, C_g, dB_g, dC_g;
   const float *A, *skip, *dt_bias, *state, *dfinal;
   float *final_state, *checkpoints, *dstate, *part;
+  float *ends, *sums;  // [chunks][N][D][S], [chunks][N][D]: what a piece adds to the state, and its sum of delta
   const long long* lengths;
 };
 
-// Where a block works: channels d0 .. d0 + CB - 1 of group g in row n.
+// Where a block works: channels d0 .. d0 + count - 1 of group g in row n, steps first .. last - 1.
 struct Place {
-  int n, g, d0, count;  // count: channels that exist
+  int ct, n, g, d0, count, piece, first, last;
   template <typename A>
   __device__ __forceinline__ Place(const A& a, int CB) {
-    const int ct = blockIdx.x % a.ctiles, r = blockIdx.x / a.ctiles;
+    int r = blockIdx.x / a.ctiles;
+    ct = blockIdx.x % a.ctiles;
     g = r % a.G;
-    n = r / a.G;
-    const int first = ct * CB;
-    d0 = g * a.per + first;
-    count = min(CB, a.per - first);
+    r /= a.G;
+    n = r % a.N;
+    piece = r / a.N;
+    d0 = g * a.per + ct * CB;
+    count = min(CB, a.per - ct * CB);
+    first = piece * a.chunk;
+    last = min(a.T_, first + a.chunk);
   }
 };
 
-// 2^v on the special function unit; a = exp(delta A) is exp2(delta (A log2 e)).
+// 2^v on the special function unit, whose results are low by 2.4e-8 of their value on average for v in
+// [-1/64, 0] and by 5.4e-8 below (measured).  A state that decays slowly adds that bias up over
+// 1 / (1 - a) steps, so decay() shifts the argument by half of it, in the same instruction.
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float EXP2_LOW = 3e-8f;
+// exp(delta A) for two states, A in units of log2(e).
+__device__ __forceinline__ float2 decay(float2 delta, float2 A) {
+  const float2 v = __ffma2_rn(delta, A, make_float2(EXP2_LOW, EXP2_LOW));
+  return make_float2(exp2_fast(v.x), exp2_fast(v.y));
+}
 
-// log(1 + exp(v)), from the side where the exponential is small.
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(__expf(-fabsf(v))); }
+// delta = log(1 + exp(v)) = max(v, 0) + log(1 + e) and its slope, with e = exp(-|v|).  The product
+// -|v| log2(e) is taken in two parts, so that e keeps its bits for large |v|; log(1 + e) / e on [0, 1] is a
+// polynomial of degree 8, fitted for the least relative error (3e-8).
+struct Softplus {
+  float value, slope;
+  __device__ __forceinline__ explicit Softplus(float v) {
+    float m = fabsf(v);
+    m = m > 128.f ? 128.f : m;  // (a NaN stays)
+    const float hi = -m * LOG2E, lo = fmaf(m, -1.925963033500e-8f, fmaf(-m, LOG2E, -hi));
+    const float r = exp2_fast(hi), e = fmaf(r, lo * 0.69314718f, r);
+    float p = 0.00523269070233413f;
+    p = fmaf(p, e, -0.02950522894050519f);
+    p = fmaf(p, e, 0.0782259443637453f);
+    p = fmaf(p, e, -0.13663246046340774f);
+    p = fmaf(p, e, 0.191060074281249f);
+    p = fmaf(p, e, -0.2484298258665141f);
+    p = fmaf(p, e, 0.33319096896971945f);
+    p = fmaf(p, e, -0.4999949314926837f);
+    p = fmaf(p, e, 0.9999999698819679f);
+    value = fmaf(p, e, fmaxf(v, 0.f));
+    slope = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
+  }
+};
 
 // A thread's NS neighbouring values of a row of S, zero beyond its end.
-__device__ __forceinline__ void load_states(const float* p, int s0, int S, float (&v)[NS]) {
+__device__ __forceinline__ void load_states(const float* p, int s0, int S, float2 (&v)[NS / 2]) {
   if (S % NS == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    if (s0 < S) {
-      const float4 w = *reinterpret_cast<const float4*>(p + s0);
-      v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-    } else {
-      v[0] = v[1] = v[2] = v[3] = 0.f;
-    }
+    const float4 w = s0 < S ? *reinterpret_cast<const float4*>(p + s0) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[0] = make_float2(w.x, w.y);
+    v[1] = make_float2(w.z, w.w);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < NS; ++i) v[i] = s0 + i < S ? p[s0 + i] : 0.f;
+  for (int i = 0; i < NS / 2; ++i) {
+    v[i].x = s0 + 2 * i < S ? p[s0 + 2 * i] : 0.f;
+    v[i].y = s0 + 2 * i + 1 < S ? p[s0 + 2 * i + 1] : 0.f;
+  }
 }
-__device__ __forceinline__ void store_states(float* p, int s0, int S, const float (&v)[NS]) {
+__device__ __forceinline__ void store_states(float* p, int s0, int S, const float2 (&v)[NS / 2]) {
   if (S % NS == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    if (s0 < S) *reinterpret_cast<float4*>(p + s0) = make_float4(v[0], v[1], v[2], v[3]);
+    if (s0 < S) *reinterpret_cast<float4*>(p + s0) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < NS; ++i)
-    if (s0 + i < S) p[s0 + i] = v[i];
+  for (int i = 0; i < NS / 2; ++i) {
+    if (s0 + 2 * i < S) p[s0 + 2 * i] = v[i].x;
+    if (s0 + 2 * i + 1 < S) p[s0 + 2 * i + 1] = v[i].y;
+  }
+}
+// Four floats of shared memory as two pairs.
+__device__ __forceinline__ void load_pairs(const float* p, float2 (&v)[2]) {
+  const float4 w = *reinterpret_cast<const float4*>(p);
+  v[0] = make_float2(w.x, w.y);
+  v[1] = make_float2(w.z, w.w);
+}
+// B bytes of global to shared memory behind the thread's back, zeros unless `ok`.
+template <int B>
+__device__ __forceinline__ void copy_async(float* to, const float* from, bool ok) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  const int bytes = ok ? B : 0;
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// How a block is laid out: Q lanes of NS states a channel, CH channels a thread, tiles of TT staged steps.
+constexpr int THREADS = 128;
+template <int Q, int CH, int TT>
+struct Tile {
+  static constexpr int CB = THREADS / Q, CT = CB * CH, SP = Q * NS;
+  static constexpr int PER = TT * CT >= THREADS ? TT * CT / THREADS : 1;  // staged (step, channel) pairs of a thread
+  static constexpr int V = PER < 4 ? PER : 4;                            // neighbouring channels among them, at most
+  // A row of the lanes' partial sums, one per lane of a channel: shifted so that a warp's stores fall into 32 banks.
+  static constexpr int YC = CT + (Q == 1 ? 0 : 32 / Q);
+  // rows of B or C that the block loads together, and how often
+  static constexpr int BR = THREADS / SP, PB = (TT + BR - 1) / BR;
+};
+constexpr int fwd_steps(int Q) { return Q <= 2 ? 8 : 16; }
+
+// The sums of the Q lanes' parts for V neighbouring channels; p: the first lane's.
+template <int Q, int V, int YC>
+__device__ __forceinline__ void sum_parts_of(const float* p, float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    float w[V];
+    load<float, V>(p + i * YC, w);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = i ? s[v] + w[v] : w[v];
+  }
 }
 
 // Sums COUNT values over the LANES lanes that differ in the bits of LANES / 2 * STRIDE .. STRIDE.  While
@@ -102,6 +184,14 @@ __device__ __forceinline__ int lane_sums(float (&v)[COUNT], int lane, bool& owne
   return base;
 }
 
+// Whether a group's width, the strides and the starts allow accesses of V channels.
+inline bool wide(const haste_b200_selective_scan& a, int V, bool backward) {
+  const int e = (int)dtype_size(a.dtype), b = V * e;
+  bool ok = (a.D / a.G) % V == 0 && aligned(a.x, e, b) && aligned(a.dt, e, b) && aligned(a.z, e, b);
+  if (!backward) return ok && aligned(a.y, e, b);
+  return ok && aligned(a.dy, e, b) && aligned(a.dx, e, b) && aligned(a.ddt, e, b) && aligned(a.dz, e, b);
+}
+
 // Lanes per channel: states in fours, a power of two.
 inline int lanes(int S) {
   int q = 1;
@@ -111,12 +201,53 @@ inline int lanes(int S) {
 
 int check(const haste_b200_selective_scan& a, bool backward);
 
+// One definition per storage type, each in a file of its own.
+template <typename T>
+int forward(const haste_b200_selective_scan& a, cudaStream_t s);
+template <typename T>
+int backward(const haste_b200_selective_scan& a, cudaStream_t s);
+int forward_pieces(const haste_b200_selective_scan& a);
+
+// How a backward call is cut: channels per thread, and pieces of the sequence.
+struct BwdShape {
+  int Q, CH, ctiles, chunks, chunk;
+  long long blocks;  // of a piece
+  explicit BwdShape(const haste_b200_selective_scan& a) {
+    Q = lanes(a.S);
+    const int per = a.D / a.G, CB = THREADS / Q;
+    const long long rows = (long long)a.N * a.G;
+    CH = rows * ceil_div(per, 2 * CB) >= 3LL * sm_count() ? 2 : 1;
+#ifdef FORCECH
+    CH = FORCECH;
+#endif
+    ctiles = ceil_div(per, CB * CH);
+    blocks = rows * ctiles;
+    chunks = 1;
+    chunk = a.T > 0 ? a.T : 1;
+    if (blocks < 2LL * sm_count()) {
+      const long long most = ceil_div(a.T, 64), want = (3LL * sm_count() + blocks - 1) / blocks;
+      if (want >= 2 && most >= 2) {
+        chunk = ceil_div(ceil_div(a.T, want < most ? want : most), 32) * 32;
+        chunks = ceil_div(a.T, chunk);
+      }
+    }
+  }
+  // scratch: partial rows of dB and dC, sums of dA, dskip and ddt_bias, the pieces' ends
+  long long bc_floats(const haste_b200_selective_scan& a) const { return (long long)ctiles * a.T * a.N * a.G * 2 * Q * NS; }
+  long long sum_floats(const haste_b200_selective_scan& a) const { return (long long)chunks * a.N * a.D * (a.S + 2); }
+  long long floats(const haste_b200_selective_scan& a) const {
+    return bc_floats(a) + sum_floats(a) + (chunks > 1 ? (long long)chunks * a.N * a.D * (a.S + 1) : 0);
+  }
+};
+
 template <typename T>
 Args<T> pack(const haste_b200_selective_scan& a, int CB) {
   Args<T> k;
   k.T_ = a.T; k.N = a.N; k.D = a.D; k.G = a.G; k.S = a.S;
   k.per = a.D / a.G;
   k.ctiles = ceil_div(k.per, CB);
+  k.chunks = 1;
+  k.chunk = a.T;
   k.softplus = a.softplus != 0;
   k.x = Seq<const T>(a.x); k.dt = Seq<const T>(a.dt); k.z = Seq<const T>(a.z);
   k.B = Seq<const T>(a.B); k.C = Seq<const T>(a.C); k.dy = Seq<const T>(a.dy);
@@ -125,6 +256,7 @@ Args<T> pack(const haste_b200_selective_scan& a, int CB) {
   k.B_g = a.B_g; k.C_g = a.C_g; k.dB_g = a.dB_g; k.dC_g = a.dC_g;
   k.A = a.A; k.skip = a.skip; k.dt_bias = a.dt_bias; k.state = a.state; k.dfinal = a.dfinal_state;
   k.final_state = a.final_state; k.checkpoints = a.checkpoints; k.dstate = a.dstate; k.part = a.scratch;
+  k.ends = k.sums = nullptr;
   k.lengths = a.lengths;
   return k;
 }

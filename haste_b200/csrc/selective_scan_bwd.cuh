@@ -1,0 +1,541 @@
+// Selective scan, backward.  With dy already multiplied by silu(z), from the last step to the first:
+//
+//   lam_t = C_t dy_t + a_{t+1} lam_{t+1}          a_t = exp(delta_t A)
+//   dC_t = sum_d dy_t h_t,   dB_t = sum_d lam_t delta_t x_t
+//   dx_t = delta_t (lam_t . B_t) + skip dy_t
+//   ddelta_t = x_t (lam_t . B_t) + lam_t . (A a_t h_{t-1}),   dA = sum_t lam_t delta_t a_t h_{t-1}
+//
+// The forward pass left the state in front of every CKPT steps; a thread computes those steps' states
+// and decays again, keeps them in registers, and walks back over them.
+#pragma once
+
+#include <algorithm>
+
+#include "selective_scan.cuh"
+
+namespace hb {
+namespace scan {
+namespace {
+
+// Lanes, channels and shared memory as in the forward kernel.  dB and dC are sums over channels: a thread
+// adds its CH channels, then they are added over the lanes of a warp, over the warps in shared memory,
+// and over the blocks from partial rows [ctiles][T][N][G][2][SP], all in a fixed order.
+template <int Q, int CH>
+struct Shared {
+  using F = Tile<Q, CH, CKPT>;
+  float4 B[CKPT][Q], C[CKPT][Q];
+  float2 dd[CKPT][F::CT];                     // delta, delta x
+  float dy[CKPT][F::CT];
+  float red[THREADS / 32][CKPT][2 * F::SP];
+  float part[3][CKPT][Q][F::YC];              // each lane's part of lam . B, lam . (A a h), C . h
+  // What a thread keeps from tile to tile, each word its own: registers are what limits this kernel.
+  float4 dA[CH][THREADS];
+  float4 start[CH][THREADS];                  // the state in front of the next tile
+  float sums[2][THREADS][F::V];               // of dskip and ddt_bias
+};
+
+#ifndef HH1
+#define HH1 4
+#endif
+#ifndef HH2
+#define HH2 4
+#endif
+#ifndef MINB
+#define MINB 3
+#endif
+template <typename T, int Q, int CH, int V, bool Gate>
+__global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> a) {
+  using M = Shared<Q, CH>;
+  using F = Tile<Q, CH, CKPT>;
+  constexpr int TT = CKPT, CB = F::CB, CT = F::CT, SP = F::SP, YC = F::YC, BR = F::BR, PB = F::PB, WARPS = THREADS / 32;
+  constexpr int SL = F::PER / V, ROWS = THREADS * V / CT;
+  constexpr int LANES = 32 / Q;  // channels of a warp
+  constexpr int H = CH == 1 ? HH1 : HH2;  // steps whose states and decays a thread holds
+  extern __shared__ __align__(16) char memory[];
+  M& m = *reinterpret_cast<M*>(memory);
+  const Place at(a, CT);
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int q = tid % Q, c = tid / Q, s0 = q * NS;
+  const int n = at.n, len = row_length(a.lengths, n, a.T_);
+  const int cs = tid * V % CT, ts = tid * V / CT;
+  const bool has = cs < at.count && ts < TT;
+  const int ds = at.d0 + (has ? cs : 0);
+  const long long pairs = (long long)a.N * a.D, rown = (long long)n * a.D + at.d0;
+  // (parameters are read again for every tile, from the L1 cache)
+  auto parameter = [&](const float* p, float (&out)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = has && p ? __ldg(p + ds + v) : 0.f;
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v) m.sums[0][tid][v] = m.sums[1][tid][v] = 0.f;
+  float2 A2[CH][2] = {}, carry[CH][2] = {};  // A2: A log2(e); carry: a_{t+1} lam_{t+1}, from dfinal through the pieces behind
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int ch = j * CB + c;
+    m.dA[j][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ch >= at.count) continue;
+    const long long row = (rown + ch) * a.S;
+    load_states(a.A + (long long)(at.d0 + ch) * a.S, s0, a.S, A2[j]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) A2[j][i] = __fmul2_rn(A2[j][i], both(LOG2E));
+    if (a.dfinal) load_states(a.dfinal + row, s0, a.S, carry[j]);
+#pragma unroll 4
+    for (int p = a.chunks - 1; p > at.piece; --p) {
+      float2 e[2];
+      load_states(a.ends + p * pairs * a.S + row, s0, a.S, e);
+      const float sum = a.sums[p * pairs + rown + ch];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) carry[j][i] = __ffma2_rn(decay(both(sum), A2[j][i]), carry[j][i], e[i]);
+    }
+  }
+
+  const int tiles = (at.last - at.first + TT - 1) / TT;
+  Raw<T, V> xn[SL], dn[SL], zn[SL], gn[SL];
+  Raw<T, 1> bn[PB], cn[PB];
+  const int bt = tid / SP, bs = tid % SP;
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int t = t0 + ts + i * ROWS;
+      const bool ok = has && t < len;
+      xn[i] = load_if<T, V>(ok, a.x.at(t, n) + ds);
+      dn[i] = load_if<T, V>(ok, a.dt.at(t, n) + ds);
+      gn[i] = load_if<T, V>(ok, a.dy.at(t, n) + ds);
+      if (Gate) zn[i] = load_if<T, V>(ok, a.z.at(t, n) + ds);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      const int k = i * BR + bt, t = t0 + k;
+      const bool ok = bs < a.S && t < len && (TT % BR == 0 || k < TT);
+      bn[i] = load_if<T, 1>(ok, a.B.at(t, n) + at.g * a.B_g + bs);
+      cn[i] = load_if<T, 1>(ok, a.C.at(t, n) + at.g * a.C_g + bs);
+    }
+  };
+  // the states in front of a tile, on their way to shared memory
+  const bool fours = a.S % NS == 0 && (reinterpret_cast<uintptr_t>(a.checkpoints) & 15) == 0;
+  auto before = [&](int t0) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const float* p = a.checkpoints + t0 / CKPT * (pairs * a.S) + (rown + j * CB + c) * a.S + s0;
+      const bool mine = j * CB + c < at.count;
+      float* to = &m.start[j][tid].x;
+      if (fours) copy_async<16>(to, mine && s0 < a.S ? p : a.checkpoints, mine && s0 < a.S);
+      else
+#pragma unroll
+        for (int i = 0; i < NS; ++i) copy_async<4>(to + i, mine && s0 + i < a.S ? p + i : a.checkpoints, mine && s0 + i < a.S);
+    }
+  };
+  if (tiles > 0) {
+    fetch(at.first + (tiles - 1) * TT);
+    before(at.first + (tiles - 1) * TT);
+  }
+#pragma unroll 1
+  for (int tile = tiles - 1; tile >= 0; --tile) {
+    const int t0 = at.first + tile * TT;
+    Raw<T, V> x[SL], z[SL], dy[SL];
+    float slope[SL][V], bias[V];
+    copies_done();
+    float2 h0[CH][2];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) load_pairs(&m.start[j][tid].x, h0[j]);
+    parameter(a.dt_bias, bias);
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int k = ts + i * ROWS;
+      x[i] = xn[i];
+      z[i] = zn[i];
+      dy[i] = gn[i];
+      float xv[V], delta[V], g[V];
+      unpack<T, V>(x[i], xv);
+      unpack<T, V>(dn[i], delta);
+      unpack<T, V>(dy[i], g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        delta[v] += bias[v];
+        slope[i][v] = 1.f;
+      }
+      if (a.softplus)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const Softplus sp(delta[v]);
+          delta[v] = sp.value;
+          slope[i][v] = sp.slope;
+        }
+      if (Gate) {
+        float zv[V];
+        unpack<T, V>(z[i], zv);
+#pragma unroll
+        for (int v = 0; v < V; ++v) g[v] *= silu(zv[v]);
+      }
+      if (t0 + k >= len)
+#pragma unroll
+        for (int v = 0; v < V; ++v) delta[v] = slope[i][v] = 0.f;
+      if (ts < TT) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) m.dd[k][cs + v] = make_float2(delta[v], delta[v] * xv[v]);
+        store<float, V>(&m.dy[k][cs], g);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i)
+      if (TT % BR == 0 || i * BR + bt < TT) {
+        (&m.B[i * BR + bt][0].x)[bs] = one(bn[i]);
+        (&m.C[i * BR + bt][0].x)[bs] = one(cn[i]);
+      }
+    __syncthreads();
+    if (tile > 0) {
+      fetch(t0 - TT);
+      before(t0 - TT);
+    }
+    float2 sum[CH][2] = {};  // dA of these steps: short sums keep their bits
+#pragma unroll 1
+    for (int k0 = TT - H; k0 >= 0; k0 -= H) {
+      float2 hs[CH][2], decays[CH][H][2], h[CH][H][2];
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        hs[j][0] = h0[j][0];
+        hs[j][1] = h0[j][1];
+      }
+      // up to the H steps at hand, then over them
+#pragma unroll 1
+      for (int k = 0; k < k0; k += H)
+#pragma unroll
+        for (int l = 0; l < H; ++l) {
+          float2 b[2];
+          load_pairs(&m.B[k + l][q].x, b);
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const float2 w = m.dd[k + l][j * CB + c];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) hs[j][i] = __ffma2_rn(decay(both(w.x), A2[j][i]), hs[j][i], __fmul2_rn(both(w.y), b[i]));
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        float2 b[2];
+        load_pairs(&m.B[k0 + k][q].x, b);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          const float2 w = m.dd[k0 + k][j * CB + c];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            decays[j][k][i] = decay(both(w.x), A2[j][i]);
+            h[j][k][i] = __fmul2_rn(both(w.y), b[i]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        float2 g[2];
+        if (Gate) load_pairs(&m.C[k0 + k][q].x, g);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            h[j][k][i] = __ffma2_rn(decays[j][k][i], k ? h[j][k ? k - 1 : 0][i] : hs[j][i], h[j][k][i]);
+          if (Gate) {
+            const float2 s = __ffma2_rn(h[j][k][1], g[1], __fmul2_rn(h[j][k][0], g[0]));
+            m.part[2][k0 + k][q][j * CB + c] = s.x + s.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = H - 1; k >= 0; --k) {
+        float2 b[2], g[2], dB[2], dC[2];
+        load_pairs(&m.B[k0 + k][q].x, b);
+        load_pairs(&m.C[k0 + k][q].x, g);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          const float2 w = m.dd[k0 + k][j * CB + c], dyk = both(m.dy[k0 + k][j * CB + c]);
+          float2 lb, da;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 lam = __ffma2_rn(g[i], dyk, carry[j][i]);
+            dB[i] = j ? __ffma2_rn(lam, both(w.y), dB[i]) : __fmul2_rn(lam, both(w.y));
+            dC[i] = j ? __ffma2_rn(dyk, h[j][k][i], dC[i]) : __fmul2_rn(dyk, h[j][k][i]);
+            lb = i ? __ffma2_rn(lam, b[i], lb) : __fmul2_rn(lam, b[i]);
+            carry[j][i] = __fmul2_rn(decays[j][k][i], lam);
+            const float2 u = __fmul2_rn(carry[j][i], k ? h[j][k ? k - 1 : 0][i] : hs[j][i]);  // lam a h_{t-1}
+            da = i ? __ffma2_rn(u, A2[j][i], da) : __fmul2_rn(u, A2[j][i]);
+            sum[j][i] = __ffma2_rn(u, both(w.x), sum[j][i]);
+          }
+          m.part[0][k0 + k][q][j * CB + c] = lb.x + lb.y;
+          m.part[1][k0 + k][q][j * CB + c] = da.x + da.y;
+        }
+        float bc[2 * NS] = {dB[0].x, dB[0].y, dB[1].x, dB[1].y, dC[0].x, dC[0].y, dC[1].x, dC[1].y};
+        bool owner;
+        const int first = lane_sums<2 * NS, LANES, Q>(bc, lane, owner);
+        if (owner)
+#pragma unroll
+          for (int i = 0; i < (2 * NS > LANES ? 2 * NS / LANES : 1); ++i) {
+            const int e = first + i;  // 0..3 dB, 4..7 dC of the thread's states
+            m.red[warp][k0 + k][(e / NS) * SP + s0 + e % NS] = bc[i];
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      float2 v[2];
+      load_pairs(&m.dA[j][tid].x, v);
+      v[0] = __fadd2_rn(v[0], sum[j][0]);
+      v[1] = __fadd2_rn(v[1], sum[j][1]);
+      m.dA[j][tid] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = tid; e < TT * 2 * SP; e += THREADS) {
+      const int k = e / (2 * SP), i = e % (2 * SP);
+      if (t0 + k >= at.last) break;
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) s += m.red[w][k][i];
+      a.part[((((long long)at.ct * a.T_ + t0 + k) * a.N + n) * a.G + at.g) * (2 * SP) + i] = s;
+    }
+    float skip[V];
+    parameter(a.skip, skip);
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int k = ts + i * ROWS;
+      if (!has || t0 + k >= at.last) continue;
+      float g[V], xv[V], lb[V], da[V], dx[V], ddt[V];
+      load<float, V>(&m.dy[k][cs], g);
+      unpack<T, V>(x[i], xv);
+      sum_parts_of<Q, V, YC>(&m.part[0][k][0][cs], lb);
+      sum_parts_of<Q, V, YC>(&m.part[1][k][0][cs], da);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        dx[v] = fmaf(m.dd[k][cs + v].x, lb[v], skip[v] * g[v]);
+        ddt[v] = fmaf(lb[v], xv[v], da[v] * LN2) * slope[i][v];
+        m.sums[0][tid][v] = fmaf(g[v], xv[v], m.sums[0][tid][v]);
+        m.sums[1][tid][v] += ddt[v];
+      }
+      store<T, V>(a.dx.at(t0 + k, n) + ds, dx);
+      store<T, V>(a.ddt.at(t0 + k, n) + ds, ddt);
+      if (Gate) {
+        float zv[V], dyv[V], y[V];
+        unpack<T, V>(z[i], zv);
+        unpack<T, V>(dy[i], dyv);
+        sum_parts_of<Q, V, YC>(&m.part[2][k][0][cs], y);
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = dyv[v] * fmaf(skip[v], xv[v], y[v]) * silu_slope(zv[v], sigmoid(zv[v]));
+        store<T, V>(a.dz.at(t0 + k, n) + ds, y);
+      }
+    }
+  }
+  // row (piece, n) of the partial sums: dA [D][S], dskip [D], ddt_bias [D]
+  float* sums = a.part + (long long)a.ctiles * a.T_ * a.N * a.G * (2 * SP) +
+                ((long long)at.piece * a.N + n) * a.D * (a.S + 2);
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int ch = j * CB + c;
+    if (ch >= at.count) continue;
+    const float4 w = m.dA[j][tid];
+    const float e[NS] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (s0 + i < a.S) sums[(long long)(at.d0 + ch) * a.S + s0 + i] = e[i];
+    if (at.piece == 0 && a.dstate) store_states(a.dstate + (rown + ch) * a.S, s0, a.S, carry[j]);
+  }
+  // the threads that staged a channel
+  __syncthreads();
+  if (ts == 0 && has)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float dskip = 0.f, dbias = 0.f;
+      for (int j = 0; j < ROWS && j < TT; ++j) {
+        const int other = (j * CT + cs) / V;
+        dskip += m.sums[0][other][v];
+        dbias += m.sums[1][other][v];
+      }
+      sums[(long long)a.D * a.S + ds + v] = dskip;
+      sums[(long long)a.D * (a.S + 1) + ds + v] = dbias;
+    }
+}
+
+// What a piece hands to the one in front of it if nothing comes from behind: the recursion of lam alone.
+template <typename T, int Q, int V, bool Gate>
+__global__ void __launch_bounds__(THREADS) scan_bwd_ends(Args<T> a) {
+  constexpr int TT = fwd_steps(Q);
+  using F = Tile<Q, 1, TT>;
+  constexpr int CB = F::CB, SP = F::SP, BR = F::BR, PB = F::PB;
+  constexpr int SL = F::PER / V, ROWS = THREADS * V / CB;
+  __shared__ __align__(16) float2 in[TT][CB];  // delta, dy
+  __shared__ __align__(16) float Cs[TT][SP];
+  Place at(a, CB);
+  at.piece += 1;  // the first piece hands to nobody
+  at.first += a.chunk;
+  at.last = min(a.T_, at.first + a.chunk);
+  const int tid = threadIdx.x, q = tid % Q, c = tid / Q, s0 = q * NS;
+  const int n = at.n, len = row_length(a.lengths, n, a.T_);
+  const int cs = tid * V % CB, ts = tid * V / CB;
+  const bool has = cs < at.count && ts < TT, mine = c < at.count;
+  const int ds = at.d0 + (has ? cs : 0);
+  float bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = has && a.dt_bias ? a.dt_bias[ds + v] : 0.f;
+  float2 A[2] = {}, carry[2] = {};
+  float total = 0.f;
+  if (mine) load_states(a.A + (long long)(at.d0 + c) * a.S, s0, a.S, A);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) A[i] = __fmul2_rn(A[i], both(LOG2E));
+  const int tiles = (at.last - at.first + TT - 1) / TT;
+  Raw<T, V> dn[SL], gn[SL], zn[SL];
+  Raw<T, 1> cn[PB];
+  const int bt = tid / SP, bs = tid % SP;
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int t = t0 + ts + i * ROWS;
+      const bool ok = has && t < len;
+      dn[i] = load_if<T, V>(ok, a.dt.at(t, n) + ds);
+      gn[i] = load_if<T, V>(ok, a.dy.at(t, n) + ds);
+      if (Gate) zn[i] = load_if<T, V>(ok, a.z.at(t, n) + ds);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      const int k = i * BR + bt;
+      cn[i] = load_if<T, 1>(k < TT && t0 + k < len && bs < a.S, a.C.at(t0 + k, n) + at.g * a.C_g + bs);
+    }
+  };
+  fetch(at.first + (tiles - 1) * TT);
+#pragma unroll 1
+  for (int tile = tiles - 1; tile >= 0; --tile) {
+    const int t0 = at.first + tile * TT;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int k = ts + i * ROWS;
+      float delta[V], g[V];
+      unpack<T, V>(dn[i], delta);
+      unpack<T, V>(gn[i], g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) delta[v] += bias[v];
+      if (a.softplus)
+#pragma unroll
+        for (int v = 0; v < V; ++v) delta[v] = Softplus(delta[v]).value;
+      if (Gate) {
+        float zv[V];
+        unpack<T, V>(zn[i], zv);
+#pragma unroll
+        for (int v = 0; v < V; ++v) g[v] *= silu(zv[v]);
+      }
+      if (t0 + k >= len)
+#pragma unroll
+        for (int v = 0; v < V; ++v) delta[v] = 0.f;
+      if (ts < TT)
+#pragma unroll
+        for (int v = 0; v < V; ++v) in[k][cs + v] = make_float2(delta[v], g[v]);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i)
+      if (TT % BR == 0 || i * BR + bt < TT) Cs[i * BR + bt][bs] = one(cn[i]);
+    __syncthreads();
+    if (tile > 0) fetch(t0 - TT);
+#pragma unroll 8
+    for (int k = TT - 1; k >= 0; --k) {
+      const float2 w = in[k][c];
+      float2 g[2];
+      load_pairs(&Cs[k][s0], g);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) carry[i] = __fmul2_rn(decay(both(w.x), A[i]), __ffma2_rn(g[i], both(w.y), carry[i]));
+      total += w.x;
+    }
+    __syncthreads();
+  }
+  if (!mine) return;
+  const long long pairs = (long long)a.N * a.D, pair = (long long)n * a.D + at.d0 + c;
+  store_states(a.ends + at.piece * pairs * a.S + pair * a.S, s0, a.S, carry);
+  if (q == 0) a.sums[at.piece * pairs + pair] = total;
+}
+
+// dB and dC from the blocks' partial rows.
+template <typename T>
+__global__ void __launch_bounds__(256) scan_bwd_finish(Args<T> a, int SP, long long rows) {
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long r = e / (2 * a.S);
+  if (r >= rows) return;
+  const int j = (int)(e % (2 * a.S)), which = j / a.S, s = j % a.S;
+  const float* p = a.part + r * (2 * SP) + which * SP + s;
+  float v = 0.f;
+  for (int ct = 0; ct < a.ctiles; ++ct) v += p[(long long)ct * rows * (2 * SP)];
+  const int g = (int)(r % a.G), n = (int)(r / a.G % a.N);
+  const long long t = r / a.G / a.N;
+  if (which == 0) st(a.dB.at(t, n) + g * a.dB_g + s, v);
+  else st(a.dC.at(t, n) + g * a.dC_g + s, v);
+}
+
+template <typename T, int Q, int CH, int V, bool Gate>
+int launch_scan(const Args<T>& k, const BwdShape& sh, cudaStream_t s) {
+  constexpr int bytes = sizeof(Shared<Q, CH>);
+  if (bytes > 48 * 1024)
+    HB_CUDA_OK(cudaFuncSetAttribute(scan_bwd<T, Q, CH, V, Gate>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  scan_bwd<T, Q, CH, V, Gate><<<(int)(sh.blocks * sh.chunks), THREADS, bytes, s>>>(k);
+  HB_LAUNCH_OK();
+  return HASTE_B200_OK;
+}
+template <typename T, int Q, int CH, int V>
+int by_gate(const Args<T>& k, const BwdShape& sh, cudaStream_t s) {
+  return k.z.p ? launch_scan<T, Q, CH, V, true>(k, sh, s) : launch_scan<T, Q, CH, V, false>(k, sh, s);
+}
+
+template <typename T, int Q>
+int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
+  const BwdShape sh(a);
+  HB_REQUIRE(sh.blocks * sh.chunks < (1LL << 31), "N*D too large");
+  Args<T> k = pack<T>(a, THREADS / Q * sh.CH);
+  k.chunks = sh.chunks;
+  k.chunk = sh.chunk;
+  if (sh.chunks > 1) {
+    k.ends = a.scratch + sh.bc_floats(a) + sh.sum_floats(a);
+    k.sums = k.ends + (long long)sh.chunks * a.N * a.D * a.S;
+    Args<T> e = k;
+    e.ctiles = ceil_div(k.per, THREADS / Q);
+    const int blocks = a.N * a.G * e.ctiles * (sh.chunks - 1);
+    constexpr int V = Tile<Q, 1, fwd_steps(Q)>::V;
+    if (V > 1 && wide(a, V, true)) {
+      if (k.z.p) scan_bwd_ends<T, Q, V, true><<<blocks, THREADS, 0, s>>>(e);
+      else scan_bwd_ends<T, Q, V, false><<<blocks, THREADS, 0, s>>>(e);
+    } else {
+      if (k.z.p) scan_bwd_ends<T, Q, 1, true><<<blocks, THREADS, 0, s>>>(e);
+      else scan_bwd_ends<T, Q, 1, false><<<blocks, THREADS, 0, s>>>(e);
+    }
+    HB_LAUNCH_OK();
+    count_launch(1);
+  }
+  constexpr int V1 = Tile<Q, 1, CKPT>::V, V2 = Tile<Q, 2, CKPT>::V;
+  if (sh.CH == 2) {
+    if (wide(a, V2, true)) HB_TRY((by_gate<T, Q, 2, V2>(k, sh, s)));
+    else HB_TRY((by_gate<T, Q, 2, 1>(k, sh, s)));
+  } else {
+    if (wide(a, V1, true)) HB_TRY((by_gate<T, Q, 1, V1>(k, sh, s)));
+    else HB_TRY((by_gate<T, Q, 1, 1>(k, sh, s)));
+  }
+  const long long rows = (long long)a.T * a.N * a.G;
+  if (rows) {
+    HB_REQUIRE(rows * 2 * a.S / 256 < (1LL << 31) - 1, "T*N too large");
+    scan_bwd_finish<T><<<ceil_div(rows * 2 * a.S, 256), 256, 0, s>>>(k, Q * NS, rows);
+    HB_LAUNCH_OK();
+  }
+  count_launch(rows ? 2 : 1);
+  SumJobs jobs;
+  jobs.add(a.dA, 0, 1, a.D * a.S, HASTE_B200_F32);
+  jobs.add(a.dskip, (long long)a.D * a.S, 1, a.D, HASTE_B200_F32);
+  jobs.add(a.ddt_bias, (long long)a.D * (a.S + 1), 1, a.D, HASTE_B200_F32);
+  return sum_parts(a.scratch + sh.bc_floats(a), sh.chunks * a.N, (long long)a.D * (a.S + 2), jobs, s);
+}
+
+}  // namespace
+
+template <typename T>
+int backward(const haste_b200_selective_scan& a, cudaStream_t s) {
+  switch (lanes(a.S)) {
+    case 1: return launch<T, 1>(a, s);
+    case 2: return launch<T, 2>(a, s);
+    case 4: return launch<T, 4>(a, s);
+    case 8: return launch<T, 8>(a, s);
+    case 16: return launch<T, 16>(a, s);
+    default: return launch<T, 32>(a, s);
+  }
+}
+
+}  // namespace scan
+}  // namespace hb

@@ -1,0 +1,8 @@
+// The selective scan's forward kernels for float sequences.
+#include "selective_scan_fwd.cuh"
+
+namespace hb {
+namespace scan {
+template int forward<float>(const haste_b200_selective_scan&, cudaStream_t);
+}  // namespace scan
+}  // namespace hb
