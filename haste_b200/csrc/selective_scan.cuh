@@ -154,34 +154,17 @@ __device__ __forceinline__ void sum_parts_of(const float* p, float (&s)[V]) {
   }
 }
 
-// Sums COUNT values over the LANES lanes that differ in the bits of LANES / 2 * STRIDE .. STRIDE.  While
-// there are several values a lane hands half of them over and keeps the other half (COUNT - 1
-// shuffles for COUNT = LANES); afterwards v[0 .. max(1, COUNT / LANES) - 1] are the sums of the values
-// from the returned index on.  Of lanes that end with the same value, `owner` is set for one.
-template <int COUNT, int LANES, int STRIDE>
-__device__ __forceinline__ int lane_sums(float (&v)[COUNT], int lane, bool& owner) {
-  int base = 0;
-  owner = true;
-  int count = COUNT;
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o /= 2) {
-    const bool up = lane & (o * STRIDE);
-    if (count > 1) {
-      const int half = count / 2;
-#pragma unroll
-      for (int i = 0; i < COUNT / 2; ++i)
-        if (i < half) {
-          const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o * STRIDE);
-        }
-      base += up ? half : 0;
-      count = half;
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o * STRIDE);
-      owner = owner && !up;
-    }
+// A thread's four states in another order: register i gets state i ^ order.
+__device__ __forceinline__ void reorder(float2 (&v)[2], int order) {
+  if (order & 2) {
+    const float2 w = v[0];
+    v[0] = v[1];
+    v[1] = w;
   }
-  return base;
+  if (order & 1) {
+    v[0] = make_float2(v[0].y, v[0].x);
+    v[1] = make_float2(v[1].y, v[1].x);
+  }
 }
 
 // Whether a group's width, the strides and the starts allow accesses of V channels.

@@ -23,7 +23,9 @@ namespace {
 template <int Q, int CH>
 struct Shared {
   using F = Tile<Q, CH, CKPT>;
-  float4 B[CKPT][Q], C[CKPT][Q];
+  // B and C, once for each order in which a thread's four states may come: see add_channels
+  static constexpr int NP = Q <= 8 ? 4 : 32 / Q;
+  float B[NP][CKPT][F::SP], C[NP][CKPT][F::SP];
   float2 dd[CKPT][F::CT];                     // delta, delta x
   float dy[CKPT][F::CT];
   float red[THREADS / 32][CKPT][2 * F::SP];
@@ -56,6 +58,10 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
   const Place at(a, CT);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int q = tid % Q, c = tid / Q, s0 = q * NS;
+  // Order of this thread's states: register i is state s0 + (i ^ order).  Lanes that exchange sums of
+  // different states then have the values to keep and to give in the same registers.
+  const int order = (LANES >= 2 && (lane & LANES / 2 * Q) ? 2 : 0) + (LANES >= 4 && (lane & LANES / 4 * Q) ? 1 : 0);
+  const int copy = LANES >= 4 ? order : order / 2;
   const int n = at.n, len = row_length(a.lengths, n, a.T_);
   const int cs = tid * V % CT, ts = tid * V / CT;
   const bool has = cs < at.count && ts < TT;
@@ -76,13 +82,16 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     if (ch >= at.count) continue;
     const long long row = (rown + ch) * a.S;
     load_states(a.A + (long long)(at.d0 + ch) * a.S, s0, a.S, A2[j]);
+    reorder(A2[j], order);
 #pragma unroll
     for (int i = 0; i < 2; ++i) A2[j][i] = __fmul2_rn(A2[j][i], both(LOG2E));
     if (a.dfinal) load_states(a.dfinal + row, s0, a.S, carry[j]);
+    reorder(carry[j], order);
 #pragma unroll 4
     for (int p = a.chunks - 1; p > at.piece; --p) {
       float2 e[2];
       load_states(a.ends + p * pairs * a.S + row, s0, a.S, e);
+      reorder(e, order);
       const float sum = a.sums[p * pairs + rown + ch];
 #pragma unroll
       for (int i = 0; i < 2; ++i) carry[j][i] = __ffma2_rn(decay(both(sum), A2[j][i]), carry[j][i], e[i]);
@@ -111,6 +120,37 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
       cn[i] = load_if<T, 1>(ok, a.C.at(t, n) + at.g * a.C_g + bs);
     }
   };
+  // Sums over the channels of the warp.  Lanes that differ in the bit behind order's first exchange two states
+  // for two, those in the second one for one, without a select; then the one half goes on with dB, the other with dC.
+  auto add_channels = [&](int k, const float2 (&dB)[2], const float2 (&dC)[2]) {
+    float v[8] = {dB[0].x, dB[0].y, dB[1].x, dB[1].y, dC[0].x, dC[0].y, dC[1].x, dC[1].y};
+    constexpr unsigned all = 0xffffffffu;
+    if (LANES >= 2) {
+      v[0] += __shfl_xor_sync(all, v[2], LANES / 2 * Q);
+      v[1] += __shfl_xor_sync(all, v[3], LANES / 2 * Q);
+      v[4] += __shfl_xor_sync(all, v[6], LANES / 2 * Q);
+      v[5] += __shfl_xor_sync(all, v[7], LANES / 2 * Q);
+    }
+    if (LANES >= 4) {
+      v[0] += __shfl_xor_sync(all, v[1], LANES / 4 * Q);
+      v[4] += __shfl_xor_sync(all, v[5], LANES / 4 * Q);
+    }
+    float* to = m.red[warp][k] + s0;
+    if constexpr (LANES >= 8) {
+      const bool up = lane & LANES / 8 * Q;
+      const float give = up ? v[0] : v[4];
+      v[0] = (up ? v[4] : v[0]) + __shfl_xor_sync(all, give, LANES / 8 * Q);
+#pragma unroll
+      for (int o = LANES / 16; o > 0; o /= 2) v[0] += __shfl_xor_sync(all, v[0], o * Q);
+      if (LANES == 8 || (lane & (LANES / 8 - 1) * Q) == 0) to[(up ? SP : 0) + order] = v[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < (LANES == 1 ? 4 : LANES == 2 ? 2 : 1); ++i) {
+        to[i ^ order] = v[i];
+        to[SP + (i ^ order)] = v[4 + i];
+      }
+    }
+  };
   // the states in front of a tile, on their way to shared memory
   const bool fours = a.S % NS == 0 && (reinterpret_cast<uintptr_t>(a.checkpoints) & 15) == 0;
   auto before = [&](int t0) {
@@ -137,7 +177,11 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     copies_done();
     float2 h0[CH][2];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) load_pairs(&m.start[j][tid].x, h0[j]);
+    for (int j = 0; j < CH; ++j) {
+      const float* p = &m.start[j][tid].x;
+      h0[j][0] = make_float2(p[order], p[order ^ 1]);
+      h0[j][1] = make_float2(p[order ^ 2], p[order ^ 3]);
+    }
     parameter(a.dt_bias, bias);
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
@@ -179,8 +223,13 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
     for (int i = 0; i < PB; ++i)
       if (TT % BR == 0 || i * BR + bt < TT) {
-        (&m.B[i * BR + bt][0].x)[bs] = one(bn[i]);
-        (&m.C[i * BR + bt][0].x)[bs] = one(cn[i]);
+        const float b = one(bn[i]), g = one(cn[i]);
+#pragma unroll
+        for (int p = 0; p < M::NP; ++p) {
+          const int to = bs ^ (M::NP == 2 ? 2 * p : p);
+          m.B[p][i * BR + bt][to] = b;
+          m.C[p][i * BR + bt][to] = g;
+        }
       }
     __syncthreads();
     if (tile > 0) {
@@ -202,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
         for (int l = 0; l < H; ++l) {
           float2 b[2];
-          load_pairs(&m.B[k + l][q].x, b);
+          load_pairs(&m.B[copy][k + l][s0], b);
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
             const float2 w = m.dd[k + l][j * CB + c];
@@ -213,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         float2 b[2];
-        load_pairs(&m.B[k0 + k][q].x, b);
+        load_pairs(&m.B[copy][k0 + k][s0], b);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
           const float2 w = m.dd[k0 + k][j * CB + c];
@@ -227,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         float2 g[2];
-        if (Gate) load_pairs(&m.C[k0 + k][q].x, g);
+        if (Gate) load_pairs(&m.C[copy][k0 + k][s0], g);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
 #pragma unroll
@@ -242,8 +291,8 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
       for (int k = H - 1; k >= 0; --k) {
         float2 b[2], g[2], dB[2], dC[2];
-        load_pairs(&m.B[k0 + k][q].x, b);
-        load_pairs(&m.C[k0 + k][q].x, g);
+        load_pairs(&m.B[copy][k0 + k][s0], b);
+        load_pairs(&m.C[copy][k0 + k][s0], g);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
           const float2 w = m.dd[k0 + k][j * CB + c], dyk = both(m.dy[k0 + k][j * CB + c]);
@@ -262,15 +311,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
           m.part[0][k0 + k][q][j * CB + c] = lb.x + lb.y;
           m.part[1][k0 + k][q][j * CB + c] = da.x + da.y;
         }
-        float bc[2 * NS] = {dB[0].x, dB[0].y, dB[1].x, dB[1].y, dC[0].x, dC[0].y, dC[1].x, dC[1].y};
-        bool owner;
-        const int first = lane_sums<2 * NS, LANES, Q>(bc, lane, owner);
-        if (owner)
-#pragma unroll
-          for (int i = 0; i < (2 * NS > LANES ? 2 * NS / LANES : 1); ++i) {
-            const int e = first + i;  // 0..3 dB, 4..7 dC of the thread's states
-            m.red[warp][k0 + k][(e / NS) * SP + s0 + e % NS] = bc[i];
-          }
+        add_channels(k0 + k, dB, dC);
       }
     }
 #pragma unroll
@@ -330,10 +371,13 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     const int ch = j * CB + c;
     if (ch >= at.count) continue;
     const float4 w = m.dA[j][tid];
-    const float e[NS] = {w.x, w.y, w.z, w.w};
+    float2 e4[2] = {make_float2(w.x, w.y), make_float2(w.z, w.w)};
+    reorder(e4, order);
+    const float e[NS] = {e4[0].x, e4[0].y, e4[1].x, e4[1].y};
 #pragma unroll
     for (int i = 0; i < NS; ++i)
       if (s0 + i < a.S) sums[(long long)(at.d0 + ch) * a.S + s0 + i] = e[i];
+    reorder(carry[j], order);
     if (at.piece == 0 && a.dstate) store_states(a.dstate + (rown + ch) * a.S, s0, a.S, carry[j]);
   }
   // the threads that staged a channel

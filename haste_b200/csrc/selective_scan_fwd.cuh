@@ -82,21 +82,21 @@ __global__ void __launch_bounds__(THREADS) scan_fwd(Args<T> a) {
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const bool ok = i * ROWS < left;
-      xn[i] = load_if<T, V>(ok, px + i * ROWS * a.x.t);
-      dn[i] = load_if<T, V>(ok, pd + i * ROWS * a.dt.t);
-      if (Gate && !Ends) zn[i] = load_if<T, V>(ok, pz + i * ROWS * a.z.t);
+      xn[i] = load_if<T, V>(ok, px + (long long)(i * ROWS) * a.x.t);
+      dn[i] = load_if<T, V>(ok, pd + (long long)(i * ROWS) * a.dt.t);
+      if (Gate && !Ends) zn[i] = load_if<T, V>(ok, pz + (long long)(i * ROWS) * a.z.t);
     }
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
       const bool ok = i * BR < bleft && (TT % BR == 0 || i * BR + bt < TT);
-      bn[i] = load_if<T, 1>(ok, pb + i * BR * a.B.t);
-      if (!Ends) cn[i] = load_if<T, 1>(ok, pc + i * BR * a.C.t);
+      bn[i] = load_if<T, 1>(ok, pb + (long long)(i * BR) * a.B.t);
+      if (!Ends) cn[i] = load_if<T, 1>(ok, pc + (long long)(i * BR) * a.C.t);
     }
-    px += TT * a.x.t;
-    pd += TT * a.dt.t;
-    if (Gate) pz += TT * a.z.t;
-    pb += TT * a.B.t;
-    pc += TT * a.C.t;
+    px += (long long)TT * a.x.t;
+    pd += (long long)TT * a.dt.t;
+    if (Gate) pz += (long long)TT * a.z.t;
+    pb += (long long)TT * a.B.t;
+    pc += (long long)TT * a.C.t;
     left -= TT;
     bleft -= TT;
   };
@@ -195,9 +195,9 @@ __global__ void __launch_bounds__(THREADS) scan_fwd(Args<T> a) {
       if (t >= len)
 #pragma unroll
         for (int v = 0; v < V; ++v) y[v] = 0.f;
-      store<T, V>(py + i * ROWS * a.y.t, y);
+      store<T, V>(py + (long long)(i * ROWS) * a.y.t, y);
     }
-    py += TT * a.y.t;
+    py += (long long)TT * a.y.t;
   }
 #pragma unroll
   for (int j = 0; j < CH; ++j) {

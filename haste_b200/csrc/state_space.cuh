@@ -119,11 +119,15 @@ __device__ __forceinline__ float ldp(const void* p, bool f32, long long i) {
 template <typename T>
 struct Seq {
   T* p;
-  long long t, n;
+  int t;  // a step's stride: below 2^31 elements (strides_fit), so that an address is one multiplication
+  long long n;
   __host__ Seq() {}
-  __host__ explicit Seq(const haste_b200_sequence& s) : p(static_cast<T*>(s.data)), t(s.t_stride), n(s.n_stride) {}
-  __device__ __forceinline__ T* at(long long ti, long long ni) const { return p + ti * t + ni * n; }
+  __host__ explicit Seq(const haste_b200_sequence& s) : p(static_cast<T*>(s.data)), t((int)s.t_stride), n(s.n_stride) {}
+  __device__ __forceinline__ T* at(int ti, int ni) const { return p + ni * n + (long long)ti * t; }
 };
+inline bool strides_fit(int T, const haste_b200_sequence& s) {
+  return !s.data || T <= 1 || (s.t_stride < (1LL << 31) && s.t_stride > -(1LL << 31));
+}
 
 // Whether every row of a sequence starts on a multiple of `bytes`.
 inline bool aligned(const haste_b200_sequence& s, int elem, int bytes) {
