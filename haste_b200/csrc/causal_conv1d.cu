@@ -14,7 +14,9 @@ namespace {
 
 using namespace ss;
 
-constexpr int GROUP = 4;  // steps whose loads go out together
+// Steps of one group: 64 bytes of a thread's channels.  The next group is under way while one is computed.
+template <typename T, int V>
+constexpr int GROUP = sizeof(T) == 4 ? 4 : 8;
 
 template <typename T>
 struct ConvArgs {
@@ -44,44 +46,73 @@ __device__ __forceinline__ void input_at(const ConvArgs<T>& a, int t, int len, i
   }
 }
 
+// The taps of V neighbouring channels, W packs as they lie in memory, and their bias.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
-  const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
-  const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
-  if (d >= a.D) return;
-  const int len = row_length(a.lengths, n, a.T_);
-  const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk);
-  float w[W][V], b[V], xs[W][V];  // xs: the window, its last row the step at hand
+__device__ __forceinline__ void parameters(const ConvArgs<T>& a, int d, float (&w)[W][V], float (&b)[V]) {
+  float flat[W * V];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    float part[V];
+    if (a.param_f32) load<float, V>(static_cast<const float*>(a.w) + (long long)d * W + k * V, part);
+    else load<T, V>(static_cast<const T*>(a.w) + (long long)d * W + k * V, part);
+#pragma unroll
+    for (int i = 0; i < V; ++i) flat[k * V + i] = part[i];
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     b[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[k][i] = ldp<T>(a.w, a.param_f32, (long long)(d + i) * W + k);
+    for (int k = 0; k < W; ++k) w[k][i] = flat[i * W + k];
   }
+}
+
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
+  constexpr int G = GROUP<T, V>;
+  const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
+  const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
+  if (d >= a.D) return;
+  const int len = row_length(a.lengths, n, a.T_);
+  const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk), live = min(t1, len);
+  Raw<T, V> in[G];
+  const T* px = a.x.at(t0, n) + d;
+  auto fetch = [&](int t, Raw<T, V> (&to)[G]) {
+#pragma unroll
+    for (int u = 0; u < G; ++u) to[u] = load_if<T, V>(t + u < live, px + (long long)u * a.x.t);
+    px += (long long)G * a.x.t;
+  };
+  fetch(t0, in);
+  float w[W][V], b[V], xs[W][V];  // xs: the window, its last row the step at hand
+  parameters<T, V, W>(a, d, w, b);
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
-  for (int t = t0; t < t1; t += GROUP) {
-    Pack<T, V> in[GROUP];
+  T* py = a.y.at(t0, n) + d;
+  for (int t = t0; t < t1; t += G) {
+    Raw<T, V> next[G];
+    fetch(t + G, next);
 #pragma unroll
-    for (int u = 0; u < GROUP; ++u)
-      if (t + u < t1 && t + u < len) in[u] = *reinterpret_cast<const Pack<T, V>*>(a.x.at(t + u, n) + d);
+    for (int u = 0; u < G; ++u) {
 #pragma unroll
-    for (int u = 0; u < GROUP; ++u) {
-      if (t + u >= t1) break;
-      const bool live = t + u < len;
+      for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) xs[k][i] = xs[k + 1][i];
+      unpack<T, V>(in[u], xs[W - 1]);
       float y[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) xs[k][i] = xs[k + 1][i];
-        xs[W - 1][i] = live ? ld(&in[u].v[i]) : 0.f;
         float p = b[i];
 #pragma unroll
         for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
-        y[i] = !live ? 0.f : a.silu ? silu(p) : p;
+        y[i] = a.silu ? silu(p) : p;
       }
-      store<T, V>(a.y.at(t + u, n) + d, y);
+      if (t + u >= len)
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = 0.f;
+      if (t + u < t1) store<T, V>(py + (long long)u * a.y.t, y);
     }
+    py += (long long)G * a.y.t;
+#pragma unroll
+    for (int u = 0; u < G; ++u) in[u] = next[u];
   }
   // The last W - 1 inputs of the row.  Row k comes from row k + len of the state at the earliest, so
   // in ascending order the two may be one buffer; what this thread has read above is in registers,
@@ -101,24 +132,34 @@ __global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
 // the chunks that a block takes in turn; its partial rows are added in a fixed order afterwards.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
+  constexpr int G = 4;
   const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
   const int part = blockIdx.x / a.dtiles;
   if (d >= a.D) return;
   float w[W][V], b[V], dw[W][V], db[V];
+  parameters<T, V, W>(a, d, w, b);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    b[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
     db[i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      w[k][i] = ldp<T>(a.w, a.param_f32, (long long)(d + i) * W + k);
-      dw[k][i] = 0.f;
-    }
+    for (int k = 0; k < W; ++k) dw[k][i] = 0.f;
   }
   for (int item = part; item < a.items; item += a.parts) {
     const int n = item % a.N, c = item / a.N;
     const int len = row_length(a.lengths, n, a.T_);
-    const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk);
+    const int t0 = c * a.chunk, t1 = min(a.T_, t0 + a.chunk), end = t1 + W - 1, live = min(end, len);
+    Raw<T, V> in[G], gr[G];
+    const T *px = a.x.at(t0, n) + d, *pg = a.dy.at(t0, n) + d;
+    auto fetch = [&](int t, Raw<T, V> (&x)[G], Raw<T, V> (&g)[G]) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        x[u] = load_if<T, V>(t + u < live, px + (long long)u * a.x.t);
+        g[u] = load_if<T, V>(t + u < live, pg + (long long)u * a.dy.t);
+      }
+      px += (long long)G * a.x.t;
+      pg += (long long)G * a.dy.t;
+    };
+    fetch(t0, in, gr);
     float xs[W][V], dp[W][V];
 #pragma unroll
     for (int k = 0; k < W; ++k)
@@ -126,48 +167,46 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
       for (int i = 0; i < V; ++i) dp[k][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
-    for (int t = t0; t < t1 + W - 1; t += GROUP) {
-      Pack<T, V> in[GROUP], gr[GROUP];
+    for (int t = t0; t < end; t += G) {
+      Raw<T, V> xn[G], gn[G];
+      fetch(t + G, xn, gn);
 #pragma unroll
-      for (int u = 0; u < GROUP; ++u)
-        if (t + u < t1 + W - 1 && t + u < len) {
-          in[u] = *reinterpret_cast<const Pack<T, V>*>(a.x.at(t + u, n) + d);
-          gr[u] = *reinterpret_cast<const Pack<T, V>*>(a.dy.at(t + u, n) + d);
-        }
-#pragma unroll
-      for (int u = 0; u < GROUP; ++u) {
-        if (t + u >= t1 + W - 1) break;
-        const bool live = t + u < len, mine = live && t + u < t1;
+      for (int u = 0; u < G; ++u) {
+        const bool mine = t + u < t1;
         const int te = t + u - (W - 1);  // the step whose dx is complete now
-        float dx[V];
+        float dx[V], g[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+        for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-          for (int k = 0; k < W - 1; ++k) {
+          for (int i = 0; i < V; ++i) {
             xs[k][i] = xs[k + 1][i];
             dp[k][i] = dp[k + 1][i];
           }
-          xs[W - 1][i] = live ? ld(&in[u].v[i]) : 0.f;
-          float g = live ? ld(&gr[u].v[i]) : 0.f;
+        unpack<T, V>(in[u], xs[W - 1]);
+        unpack<T, V>(gr[u], g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
           if (a.silu) {
             float p = b[i];
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
-            // a step behind the row's end has g = 0, and p there comes from the row's own values
-            g = live ? g * silu_slope(p, sigmoid(p)) : 0.f;
+            // (behind the row's end the incoming gradient counts for nothing, whatever p is)
+            g[i] = t + u < len ? g[i] * silu_slope(p, sigmoid(p)) : 0.f;
           }
-          dp[W - 1][i] = g;
-          if (mine) {
-            db[i] += g;
+          dp[W - 1][i] = g[i];
+          dx[i] = w[0][i] * dp[W - 1][i];
 #pragma unroll
-            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, xs[k][i], dw[k][i]);
-          }
-          dx[i] = 0.f;
-#pragma unroll
-          for (int k = 0; k < W; ++k) dx[i] = fmaf(w[k][i], dp[W - 1 - k][i], dx[i]);
+          for (int k = 1; k < W; ++k) dx[i] = fmaf(w[k][i], dp[W - 1 - k][i], dx[i]);
         }
+        if (mine)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            db[i] += g[i];
+#pragma unroll
+            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g[i], xs[k][i], dw[k][i]);
+          }
         const bool before = te < 0;  // a row of the initial state
-        if (before ? c != 0 : te < t0) continue;
+        if (t + u >= end || (before ? c != 0 : te < t0)) continue;
         if (a.dfinal && te >= len - (W - 1) && te < len) {
           float f[V];
           load<T, V>(a.dfinal + ((long long)n * (W - 1) + te - len + W - 1) * a.D + d, f);
@@ -180,16 +219,23 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
           store<T, V>(a.dstate + ((long long)n * (W - 1) + te + W - 1) * a.D + d, dx);
         }
       }
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        in[u] = xn[u];
+        gr[u] = gn[u];
+      }
     }
   }
   // partial row of this block: [D][W] of dw, then [D] of db
   float* row = a.part + (long long)part * a.D * (W + 1);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int k = 0; k < W; ++k) {  // in memory order
+    float flat[V];
 #pragma unroll
-    for (int k = 0; k < W; ++k) row[(long long)(d + i) * W + k] = dw[k][i];
-    row[(long long)a.D * W + d + i] = db[i];
+    for (int i = 0; i < V; ++i) flat[i] = dw[(k * V + i) % W][(k * V + i) / W];
+    store<float, V>(row + (long long)d * W + k * V, flat);
   }
+  store<float, V>(row + (long long)a.D * W + d, db);
 }
 
 int check(const haste_b200_causal_conv1d& a, bool backward) {
@@ -207,12 +253,12 @@ int check(const haste_b200_causal_conv1d& a, bool backward) {
   return HASTE_B200_OK;
 }
 
-// Channels per thread: as many as 16 bytes hold, less where a width, a stride or a start forbids it.
-// Half as many in the backward pass, whose windows and sums take twice the registers.
+// Channels per thread: four, less where a width, a stride or a start forbids it.  (Eight 16-bit channels take
+// 150 registers for their windows and taps, and too few threads are resident to fill the memory pipes.)
 int width(const haste_b200_causal_conv1d& a, bool backward) {
-  const int e = (int)dtype_size(a.dtype);
-  for (int v = backward ? 4 : 16 / e; v > 1; v /= 2) {
-    bool ok = a.D % v == 0 && aligned(a.x, e, v * e) && aligned(a.state, v * e) && aligned(a.final_state, v * e);
+  const int e = (int)dtype_size(a.dtype), f = (int)dtype_size(a.param_dtype);
+  for (int v = 4; v > 1; v /= 2) {
+    bool ok = a.D % v == 0 && aligned(a.weight, v * f) && aligned(a.x, e, v * e) && aligned(a.state, v * e) && aligned(a.final_state, v * e);
     ok &= backward ? aligned(a.dy, e, v * e) && aligned(a.dx, e, v * e) && aligned(a.dfinal_state, v * e) &&
                          aligned(a.dstate, v * e)
                    : aligned(a.y, e, v * e);
@@ -228,8 +274,12 @@ struct Shape {
     threads = std::min(128, ceil_div(lanes, 32) * 32);
     dtiles = ceil_div(lanes, threads);
     // A chunk reads W - 1 steps twice, so long chunks while there are threads to fill the GPU.
-    chunk = 64;
-    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < 1024LL * sm_count()) chunk /= 2;
+#ifndef CH0
+#define CH0 64
+#define CHT 512LL
+#endif
+    chunk = CH0;
+    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < CHT * sm_count()) chunk /= 2;
     chunks = std::max(1, ceil_div(a.T, chunk));
   }
   long long items(int N) const { return (long long)chunks * N; }
@@ -265,7 +315,7 @@ int launch(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t st) {
   HB_REQUIRE(s.items(a.N) * s.dtiles < (1LL << 31), "T*N too large");
   const ConvArgs<T> k = pack<T>(a, s);
   if (backward) {
-    if constexpr (V <= 4) conv_bwd<T, V, W><<<k.parts * s.dtiles, s.threads, 0, st>>>(k);
+    conv_bwd<T, V, W><<<k.parts * s.dtiles, s.threads, 0, st>>>(k);
   } else {
     conv_fwd<T, V, W><<<k.items * s.dtiles, s.threads, 0, st>>>(k);
   }
@@ -288,7 +338,6 @@ int by_taps(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t s) {
 template <typename T>
 int by_width(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t s) {
   switch (width(a, backward)) {
-    case 8: if constexpr (sizeof(T) == 2) return by_taps<T, 8>(a, backward, s);
     case 4: return by_taps<T, 4>(a, backward, s);
     case 2: return by_taps<T, 2>(a, backward, s);
     default: return by_taps<T, 1>(a, backward, s);

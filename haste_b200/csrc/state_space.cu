@@ -5,10 +5,10 @@ namespace hb {
 namespace ss {
 namespace {
 
-constexpr int kCols = 32, kRows = 8;
+constexpr int kCols = 32, kRows = 32;
 
-// 32 columns x 8 groups of rows: thread (r, c) adds rows r, r + 8, ... of its column, four loads ahead,
-// and the eight sums are added in order.  The partials were written just before and lie in L2.
+// 32 columns x 32 groups of rows: thread (r, c) adds rows r, r + 32, ... of its column, four loads ahead,
+// and the sums are added in order.  The partials were written just before and lie in L2.
 __global__ void __launch_bounds__(kCols* kRows) sum_parts_kernel(const float* __restrict__ part, int P,
                                                                  long long stride, SumJobs jobs) {
   __shared__ float sums[kRows][kCols];
@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kCols* kRows) sum_parts_kernel(const float* __
   sums[r][c] = s;
   __syncthreads();
   if (r != 0 || j >= job.width) return;
-#pragma unroll
+#pragma unroll 8
   for (int k = 1; k < kRows; ++k) s += sums[k][c];
   if (job.dtype == HASTE_B200_F32) static_cast<float*>(job.out)[j * job.stride] = s;
   else if (job.dtype == HASTE_B200_BF16) st(static_cast<__nv_bfloat16*>(job.out) + j * job.stride, s);
