@@ -43,6 +43,8 @@ struct Place {
   }
 };
 
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // 2^v on the special function unit, whose results are low by 2.4e-8 of their value on average for v in
 // [-1/64, 0] and by 5.4e-8 below (measured).  A state that decays slowly adds that bias up over
 // 1 / (1 - a) steps, so decay() shifts the argument by half of it, in the same instruction.
@@ -62,26 +64,37 @@ __device__ __forceinline__ float2 decay(float2 delta, float2 A) {
 // delta = log(1 + exp(v)) = max(v, 0) + log(1 + e) and its slope, with e = exp(-|v|).  The product
 // -|v| log2(e) is taken in two parts, so that e keeps its bits for large |v|; log(1 + e) / e on [0, 1] is a
 // polynomial of degree 8, fitted for the least relative error (3e-8).
-struct Softplus {
-  float value, slope;
-  __device__ __forceinline__ explicit Softplus(float v) {
-    float m = fabsf(v);
-    m = m > 128.f ? 128.f : m;  // (a NaN stays)
-    const float hi = -m * LOG2E, lo = fmaf(m, -1.925963033500e-8f, fmaf(-m, LOG2E, -hi));
-    const float r = exp2_fast(hi), e = fmaf(r, lo * 0.69314718f, r);
-    float p = 0.00523269070233413f;
-    p = fmaf(p, e, -0.02950522894050519f);
-    p = fmaf(p, e, 0.0782259443637453f);
-    p = fmaf(p, e, -0.13663246046340774f);
-    p = fmaf(p, e, 0.191060074281249f);
-    p = fmaf(p, e, -0.2484298258665141f);
-    p = fmaf(p, e, 0.33319096896971945f);
-    p = fmaf(p, e, -0.4999949314926837f);
-    p = fmaf(p, e, 0.9999999698819679f);
-    value = fmaf(p, e, fmaxf(v, 0.f));
-    slope = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
+template <int V, bool Slope>
+__device__ __forceinline__ void softplus(float (&v)[V], float (&slope)[V]) {
+  constexpr float c[] = {0.00523269070233413f, -0.02950522894050519f, 0.0782259443637453f, -0.13663246046340774f,
+                         0.191060074281249f,   -0.2484298258665141f,  0.33319096896971945f, -0.4999949314926837f,
+                         0.9999999698819679f};
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {  // two values to an instruction
+    const float2 x = make_float2(v[i], v[i + 1 < V ? i + 1 : i]);
+    float2 m = make_float2(fabsf(x.x), fabsf(x.y));
+    m.x = m.x > 128.f ? 128.f : m.x;  // (a NaN stays)
+    m.y = m.y > 128.f ? 128.f : m.y;
+    const float2 hi = __fmul2_rn(m, both(-LOG2E));
+    const float2 lo = __ffma2_rn(m, both(-1.925963033500e-8f), __ffma2_rn(m, both(-LOG2E), make_float2(-hi.x, -hi.y)));
+    const float2 r = make_float2(exp2_fast(hi.x), exp2_fast(hi.y)), e = __ffma2_rn(r, __fmul2_rn(lo, both(LN2)), r);
+    float2 p = both(c[0]);
+#pragma unroll
+    for (int k = 1; k < 9; ++k) p = __ffma2_rn(p, e, both(c[k]));
+    p = __ffma2_rn(p, e, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+    v[i] = p.x;
+    if (Slope) slope[i] = (x.x >= 0.f ? 1.f : e.x) * reciprocal(1.f + e.x);
+    if (i + 1 < V) {
+      v[i + 1] = p.y;
+      if (Slope) slope[i + 1] = (x.y >= 0.f ? 1.f : e.y) * reciprocal(1.f + e.y);
+    }
   }
-};
+}
+__device__ __forceinline__ float softplus(float v) {
+  float x[1] = {v}, none[1];
+  softplus<1, false>(x, none);
+  return x[0];
+}
 
 // A thread's NS neighbouring values of a row of S, zero beyond its end.
 __device__ __forceinline__ void load_states(const float* p, int s0, int S, float2 (&v)[NS / 2]) {
@@ -125,8 +138,6 @@ __device__ __forceinline__ void copy_async(float* to, const float* from, bool ok
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // How a block is laid out: Q lanes of NS states a channel, CH channels a thread, tiles of TT staged steps.
 constexpr int THREADS = 128;

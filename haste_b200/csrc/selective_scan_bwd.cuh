@@ -33,7 +33,7 @@ struct Shared {
   // What a thread keeps from tile to tile, each word its own: registers are what limits this kernel.
   float4 dA[CH][THREADS];
   float4 start[CH][THREADS];                  // the state in front of the next tile
-  float sums[2][THREADS][F::V];               // of dskip and ddt_bias
+  float4 sums[2][THREADS];                    // of dskip and ddt_bias
 };
 
 #ifndef HH1
@@ -65,15 +65,14 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
   const int n = at.n, len = row_length(a.lengths, n, a.T_);
   const int cs = tid * V % CT, ts = tid * V / CT;
   const bool has = cs < at.count && ts < TT;
-  const int ds = at.d0 + (has ? cs : 0);
+  const int d = at.d0 + (has ? cs : 0);
   const long long pairs = (long long)a.N * a.D, rown = (long long)n * a.D + at.d0;
   // (parameters are read again for every tile, from the L1 cache)
   auto parameter = [&](const float* p, float (&out)[V]) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = has && p ? __ldg(p + ds + v) : 0.f;
+    for (int v = 0; v < V; ++v) out[v] = has && p ? __ldg(p + d + v) : 0.f;
   };
-#pragma unroll
-  for (int v = 0; v < V; ++v) m.sums[0][tid][v] = m.sums[1][tid][v] = 0.f;
+  m.sums[0][tid] = m.sums[1][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
   float2 A2[CH][2] = {}, carry[CH][2] = {};  // A2: A log2(e); carry: a_{t+1} lam_{t+1}, from dfinal through the pieces behind
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
@@ -107,10 +106,10 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     for (int i = 0; i < SL; ++i) {
       const int t = t0 + ts + i * ROWS;
       const bool ok = has && t < len;
-      xn[i] = load_if<T, V>(ok, a.x.at(t, n) + ds);
-      dn[i] = load_if<T, V>(ok, a.dt.at(t, n) + ds);
-      gn[i] = load_if<T, V>(ok, a.dy.at(t, n) + ds);
-      if (Gate) zn[i] = load_if<T, V>(ok, a.z.at(t, n) + ds);
+      xn[i] = load_if<T, V>(ok, a.x.at(t, n) + d);
+      dn[i] = load_if<T, V>(ok, a.dt.at(t, n) + d);
+      gn[i] = load_if<T, V>(ok, a.dy.at(t, n) + d);
+      if (Gate) zn[i] = load_if<T, V>(ok, a.z.at(t, n) + d);
     }
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
   };
   // Sums over the channels of the warp.  Lanes that differ in the bit behind order's first exchange two states
   // for two, those in the second one for one, without a select; then the one half goes on with dB, the other with dC.
-  auto add_channels = [&](int k, const float2 (&dB)[2], const float2 (&dC)[2]) {
+  auto add_channels = [&](float* to, const float2 (&dB)[2], const float2 (&dC)[2]) {
     float v[8] = {dB[0].x, dB[0].y, dB[1].x, dB[1].y, dC[0].x, dC[0].y, dC[1].x, dC[1].y};
     constexpr unsigned all = 0xffffffffu;
     if (LANES >= 2) {
@@ -135,7 +134,6 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
       v[0] += __shfl_xor_sync(all, v[1], LANES / 4 * Q);
       v[4] += __shfl_xor_sync(all, v[5], LANES / 4 * Q);
     }
-    float* to = m.red[warp][k] + s0;
     if constexpr (LANES >= 8) {
       const bool up = lane & LANES / 8 * Q;
       const float give = up ? v[0] : v[4];
@@ -178,9 +176,8 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     float2 h0[CH][2];
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      const float* p = &m.start[j][tid].x;
-      h0[j][0] = make_float2(p[order], p[order ^ 1]);
-      h0[j][1] = make_float2(p[order ^ 2], p[order ^ 3]);
+      load_pairs(&m.start[j][tid].x, h0[j]);
+      reorder(h0[j], order);
     }
     parameter(a.dt_bias, bias);
 #pragma unroll
@@ -198,13 +195,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
         delta[v] += bias[v];
         slope[i][v] = 1.f;
       }
-      if (a.softplus)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Softplus sp(delta[v]);
-          delta[v] = sp.value;
-          slope[i][v] = sp.slope;
-        }
+      if (a.softplus) softplus<V, true>(delta, slope[i]);
       if (Gate) {
         float zv[V];
         unpack<T, V>(z[i], zv);
@@ -239,6 +230,12 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
     float2 sum[CH][2] = {};  // dA of these steps: short sums keep their bits
 #pragma unroll 1
     for (int k0 = TT - H; k0 >= 0; k0 -= H) {
+      // the H steps at hand in shared memory, from this thread's first word on
+      const float *pB = &m.B[copy][k0][s0], *pC = &m.C[copy][k0][s0], *pdy = &m.dy[k0][c];
+      const float2* pdd = &m.dd[k0][c];
+      float* pp = &m.part[0][k0][q][c];
+      float* pred = &m.red[warp][k0][s0];
+      constexpr int PK = Q * YC, PW = TT * Q * YC;  // from step to step of the parts, and from one kind to the next
       float2 hs[CH][2], decays[CH][H][2], h[CH][H][2];
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
@@ -262,10 +259,10 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         float2 b[2];
-        load_pairs(&m.B[copy][k0 + k][s0], b);
+        load_pairs(pB + k * SP, b);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-          const float2 w = m.dd[k0 + k][j * CB + c];
+          const float2 w = pdd[k * CT + j * CB];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             decays[j][k][i] = decay(both(w.x), A2[j][i]);
@@ -276,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         float2 g[2];
-        if (Gate) load_pairs(&m.C[copy][k0 + k][s0], g);
+        if (Gate) load_pairs(pC + k * SP, g);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
 #pragma unroll
@@ -284,18 +281,18 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
             h[j][k][i] = __ffma2_rn(decays[j][k][i], k ? h[j][k ? k - 1 : 0][i] : hs[j][i], h[j][k][i]);
           if (Gate) {
             const float2 s = __ffma2_rn(h[j][k][1], g[1], __fmul2_rn(h[j][k][0], g[0]));
-            m.part[2][k0 + k][q][j * CB + c] = s.x + s.y;
+            pp[2 * PW + k * PK + j * CB] = s.x + s.y;
           }
         }
       }
 #pragma unroll
       for (int k = H - 1; k >= 0; --k) {
         float2 b[2], g[2], dB[2], dC[2];
-        load_pairs(&m.B[copy][k0 + k][s0], b);
-        load_pairs(&m.C[copy][k0 + k][s0], g);
+        load_pairs(pB + k * SP, b);
+        load_pairs(pC + k * SP, g);
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-          const float2 w = m.dd[k0 + k][j * CB + c], dyk = both(m.dy[k0 + k][j * CB + c]);
+          const float2 w = pdd[k * CT + j * CB], dyk = both(pdy[k * CT + j * CB]);
           float2 lb, da;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -308,10 +305,10 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
             da = i ? __ffma2_rn(u, A2[j][i], da) : __fmul2_rn(u, A2[j][i]);
             sum[j][i] = __ffma2_rn(u, both(w.x), sum[j][i]);
           }
-          m.part[0][k0 + k][q][j * CB + c] = lb.x + lb.y;
-          m.part[1][k0 + k][q][j * CB + c] = da.x + da.y;
+          pp[k * PK + j * CB] = lb.x + lb.y;
+          pp[PW + k * PK + j * CB] = da.x + da.y;
         }
-        add_channels(k0 + k, dB, dC);
+        add_channels(pred + k * 2 * SP, dB, dC);
       }
     }
 #pragma unroll
@@ -332,8 +329,10 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
       for (int w = 0; w < WARPS; ++w) s += m.red[w][k][i];
       a.part[((((long long)at.ct * a.T_ + t0 + k) * a.N + n) * a.G + at.g) * (2 * SP) + i] = s;
     }
-    float skip[V];
+    float skip[V], ds[V], db[V];
     parameter(a.skip, skip);
+    load<float, V>(&m.sums[0][tid].x, ds);
+    load<float, V>(&m.sums[1][tid].x, db);
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const int k = ts + i * ROWS;
@@ -347,11 +346,11 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
       for (int v = 0; v < V; ++v) {
         dx[v] = fmaf(m.dd[k][cs + v].x, lb[v], skip[v] * g[v]);
         ddt[v] = fmaf(lb[v], xv[v], da[v] * LN2) * slope[i][v];
-        m.sums[0][tid][v] = fmaf(g[v], xv[v], m.sums[0][tid][v]);
-        m.sums[1][tid][v] += ddt[v];
+        ds[v] = fmaf(g[v], xv[v], ds[v]);
+        db[v] += ddt[v];
       }
-      store<T, V>(a.dx.at(t0 + k, n) + ds, dx);
-      store<T, V>(a.ddt.at(t0 + k, n) + ds, ddt);
+      store<T, V>(a.dx.at(t0 + k, n) + d, dx);
+      store<T, V>(a.ddt.at(t0 + k, n) + d, ddt);
       if (Gate) {
         float zv[V], dyv[V], y[V];
         unpack<T, V>(z[i], zv);
@@ -359,9 +358,11 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
         sum_parts_of<Q, V, YC>(&m.part[2][k][0][cs], y);
 #pragma unroll
         for (int v = 0; v < V; ++v) y[v] = dyv[v] * fmaf(skip[v], xv[v], y[v]) * silu_slope(zv[v], sigmoid(zv[v]));
-        store<T, V>(a.dz.at(t0 + k, n) + ds, y);
+        store<T, V>(a.dz.at(t0 + k, n) + d, y);
       }
     }
+    store<float, V>(&m.sums[0][tid].x, ds);
+    store<float, V>(&m.sums[1][tid].x, db);
   }
   // row (piece, n) of the partial sums: dA [D][S], dskip [D], ddt_bias [D]
   float* sums = a.part + (long long)a.ctiles * a.T_ * a.N * a.G * (2 * SP) +
@@ -388,11 +389,11 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> 
       float dskip = 0.f, dbias = 0.f;
       for (int j = 0; j < ROWS && j < TT; ++j) {
         const int other = (j * CT + cs) / V;
-        dskip += m.sums[0][other][v];
-        dbias += m.sums[1][other][v];
+        dskip += (&m.sums[0][other].x)[v];
+        dbias += (&m.sums[1][other].x)[v];
       }
-      sums[(long long)a.D * a.S + ds + v] = dskip;
-      sums[(long long)a.D * (a.S + 1) + ds + v] = dbias;
+      sums[(long long)a.D * a.S + d + v] = dskip;
+      sums[(long long)a.D * (a.S + 1) + d + v] = dbias;
     }
 }
 
@@ -453,9 +454,7 @@ __global__ void __launch_bounds__(THREADS) scan_bwd_ends(Args<T> a) {
       unpack<T, V>(gn[i], g);
 #pragma unroll
       for (int v = 0; v < V; ++v) delta[v] += bias[v];
-      if (a.softplus)
-#pragma unroll
-        for (int v = 0; v < V; ++v) delta[v] = Softplus(delta[v]).value;
+      if (a.softplus) softplus<V, false>(delta, delta);
       if (Gate) {
         float zv[V];
         unpack<T, V>(zn[i], zv);

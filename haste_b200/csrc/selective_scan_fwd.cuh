@@ -114,9 +114,7 @@ __global__ void __launch_bounds__(THREADS) scan_fwd(Args<T> a) {
       unpack<T, V>(dn[i], delta);
 #pragma unroll
       for (int v = 0; v < V; ++v) delta[v] += bias[v];
-      if (a.softplus)
-#pragma unroll
-        for (int v = 0; v < V; ++v) delta[v] = Softplus(delta[v]).value;
+      if (a.softplus) softplus<V, false>(delta, delta);
       if (t0 + k >= len)
 #pragma unroll
         for (int v = 0; v < V; ++v) delta[v] = 0.f;  // the state stays
@@ -229,7 +227,7 @@ __global__ void __launch_bounds__(256) scan_step(Args<T> a) {
   if (live) {
     x = ld(a.x.at(0, n) + d);
     const float v = ld(a.dt.at(0, n) + d) + (a.dt_bias ? a.dt_bias[d] : 0.f);
-    const float delta = a.softplus ? Softplus(v).value : v, u = delta * x;
+    const float delta = a.softplus ? softplus(v) : v, u = delta * x;
     const T *B = a.B.at(0, n) + g * a.B_g, *C = a.C.at(0, n) + g * a.C_g;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

@@ -144,11 +144,15 @@ __device__ __forceinline__ int row_length(const long long* lengths, int n, int T
 
 // sigmoid(v) = 1 / (1 + 2^(-v log2 e)), two approximate instructions (2^-22 relative and one unit in the last
 // place); an overflowing exponential gives zero.  silu(v) = v s and its slope from s = sigmoid(v).
-__device__ __forceinline__ float sigmoid(float v) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+__device__ __forceinline__ float sigmoid(float v) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+  return reciprocal(1.0f + e);
 }
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 __device__ __forceinline__ float silu_slope(float v, float s) { return fmaf(v * s, 1.0f - s, s); }
