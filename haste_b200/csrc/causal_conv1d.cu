@@ -274,12 +274,8 @@ struct Shape {
     threads = std::min(128, ceil_div(lanes, 32) * 32);
     dtiles = ceil_div(lanes, threads);
     // A chunk reads W - 1 steps twice, so long chunks while there are threads to fill the GPU.
-#ifndef CH0
-#define CH0 64
-#define CHT 512LL
-#endif
-    chunk = CH0;
-    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < CHT * sm_count()) chunk /= 2;
+    chunk = 64;
+    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < 512LL * sm_count()) chunk /= 2;
     chunks = std::max(1, ceil_div(a.T, chunk));
   }
   long long items(int N) const { return (long long)chunks * N; }

@@ -347,16 +347,10 @@ int threads(int H, int per) { return ceil_div(ceil_div(H, per), 32) * 32; }
 
 // Blocks of the backward pass, each of which leaves a row of partial sums: enough threads to fill the SMs.
 int parts(const haste_b200_fused_norm& a) {
-#ifndef NB
-#define NB 512
-#endif
-  const int th = threads(a.H, a.H <= 4096 ? 8 : 16), per_sm = std::max(1, std::min(16, NB / th));
+  const int th = threads(a.H, a.H <= 4096 ? 8 : 16), per_sm = std::max(1, std::min(16, 512 / th));
   return std::max(1, std::min(a.T * a.N, per_sm * sm_count()));
 }
 
-#ifndef NF
-#define NF 768
-#endif
 template <typename T, typename R, typename P, int V, int K>
 int launch(const haste_b200_fused_norm& a, bool backward, cudaStream_t s) {
   NormArgs<T, R, P> k;
@@ -378,7 +372,7 @@ int launch(const haste_b200_fused_norm& a, bool backward, cudaStream_t s) {
   const int th = threads(a.H, V * K);
   if (!backward) {
     if (k.rows == 0) return HASTE_B200_OK;
-    const int blocks = std::min(k.rows, std::max(1, std::min(32, NF / th)) * sm_count());
+    const int blocks = std::min(k.rows, std::max(1, std::min(32, 768 / th)) * sm_count());
     norm_fwd<T, R, P, V, K><<<blocks, th, 0, s>>>(k);
     HB_LAUNCH_OK();
     count_launch(1);

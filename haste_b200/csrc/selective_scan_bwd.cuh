@@ -36,23 +36,14 @@ struct Shared {
   float4 sums[2][THREADS];                    // of dskip and ddt_bias
 };
 
-#ifndef HH1
-#define HH1 4
-#endif
-#ifndef HH2
-#define HH2 4
-#endif
-#ifndef MINB
-#define MINB 3
-#endif
 template <typename T, int Q, int CH, int V, bool Gate>
-__global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : MINB) scan_bwd(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) {
   using M = Shared<Q, CH>;
   using F = Tile<Q, CH, CKPT>;
   constexpr int TT = CKPT, CB = F::CB, CT = F::CT, SP = F::SP, YC = F::YC, BR = F::BR, PB = F::PB, WARPS = THREADS / 32;
   constexpr int SL = F::PER / V, ROWS = THREADS * V / CT;
   constexpr int LANES = 32 / Q;  // channels of a warp
-  constexpr int H = CH == 1 ? HH1 : HH2;  // steps whose states and decays a thread holds
+  constexpr int H = 4;  // steps whose states and decays a thread holds; of 8, all would not fit the registers
   extern __shared__ __align__(16) char memory[];
   M& m = *reinterpret_cast<M*>(memory);
   const Place at(a, CT);
@@ -499,6 +490,7 @@ __global__ void __launch_bounds__(256) scan_bwd_finish(Args<T> a, int SP, long l
   const int j = (int)(e % (2 * a.S)), which = j / a.S, s = j % a.S;
   const float* p = a.part + r * (2 * SP) + which * SP + s;
   float v = 0.f;
+#pragma unroll 8
   for (int ct = 0; ct < a.ctiles; ++ct) v += p[(long long)ct * rows * (2 * SP)];
   const int g = (int)(r % a.G), n = (int)(r / a.G % a.N);
   const long long t = r / a.G / a.N;

@@ -26,7 +26,7 @@ namespace {
 // (Ends) each piece but the last computes what it adds to a state that is zero in front of it, and its
 // sum of delta; then each piece starts from the state that those of the pieces before it give.
 template <typename T, int Q, int CH, int V, bool Gate, bool Ends>
-__global__ void __launch_bounds__(THREADS) scan_fwd(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) {
   constexpr int TT = fwd_steps(Q);
   using F = Tile<Q, CH, TT>;
   constexpr int CB = F::CB, CT = F::CT, SP = F::SP, YC = F::YC, BR = F::BR, PB = F::PB;
@@ -174,28 +174,29 @@ __global__ void __launch_bounds__(THREADS) scan_fwd(Args<T> a) {
       }
     }
     __syncthreads();
-    if (Ends) continue;
+    if constexpr (!Ends) {
 #pragma unroll
-    for (int i = 0; i < SL; ++i) {
-      const int k = ts + i * ROWS, t = t0 + k;
-      if (!has || t >= at.last) continue;
-      float y[V], xv[V];
-      sum_parts_of<Q, V, YC>(&ys[k][0][cs], y);
-      unpack<T, V>(x[i], xv);
+      for (int i = 0; i < SL; ++i) {
+        const int k = ts + i * ROWS, t = t0 + k;
+        if (!has || t >= at.last) continue;
+        float y[V], xv[V];
+        sum_parts_of<Q, V, YC>(&ys[k][0][cs], y);
+        unpack<T, V>(x[i], xv);
 #pragma unroll
-      for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], xv[v], y[v]);
-      if (Gate) {
-        float zv[V];
-        unpack<T, V>(z[i], zv);
+        for (int v = 0; v < V; ++v) y[v] = fmaf(skip[v], xv[v], y[v]);
+        if (Gate) {
+          float zv[V];
+          unpack<T, V>(z[i], zv);
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] *= silu(zv[v]);
+          for (int v = 0; v < V; ++v) y[v] *= silu(zv[v]);
+        }
+        if (t >= len)
+#pragma unroll
+          for (int v = 0; v < V; ++v) y[v] = 0.f;
+        store<T, V>(py + (long long)(i * ROWS) * a.y.t, y);
       }
-      if (t >= len)
-#pragma unroll
-        for (int v = 0; v < V; ++v) y[v] = 0.f;
-      store<T, V>(py + (long long)(i * ROWS) * a.y.t, y);
+      py += (long long)TT * a.y.t;
     }
-    py += (long long)TT * a.y.t;
   }
 #pragma unroll
   for (int j = 0; j < CH; ++j) {

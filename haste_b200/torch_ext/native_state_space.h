@@ -8,14 +8,14 @@ using OptTensor = c10::optional<Tensor>;
 
 [[noreturn]] void refuse(const std::string& what) { throw py::value_error("haste_b200: " + what); }
 
-std::string sizes_of(std::initializer_list<int64_t> want) {
-  std::string s = "[";
-  for (int64_t n : want) s += (s.size() > 1 ? "," : "") + std::to_string(n);
-  return s + "]";
-}
-void shape(const Tensor& t, const char* name, std::initializer_list<int64_t> want) {
-  if (t.sizes() != at::IntArrayRef(want.begin(), want.size()))
-    refuse(std::string(name) + " must be " + sizes_of(want) + ", got " + shape_of(t));
+void shape(const Tensor& t, const char* name, std::initializer_list<int64_t> want, bool step = false) {
+  at::IntArrayRef w(want.begin(), want.size());
+  if (step) w = w.slice(1);  // without the axis of time
+  if (t.sizes() != w) {
+    std::string s = "[";
+    for (int64_t n : w) s += (s.size() > 1 ? "," : "") + std::to_string(n);
+    refuse(std::string(name) + " must be " + s + "], got " + shape_of(t));
+  }
 }
 void dims(const Tensor& t, const char* name, int64_t n) {
   if (t.dim() != n) refuse(std::string(name) + " must have " + std::to_string(n) + " dimensions, got " + shape_of(t));
@@ -54,9 +54,10 @@ Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 // The kernels take any strides but along the last axis.
 Tensor unit_strided(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
-haste_b200_sequence view(const Tensor& t) {
+// [T,N,...], or one step of it, [N,...].
+haste_b200_sequence view(const Tensor& t, bool step = false) {
   if (!t.defined() || !t.numel()) return {nullptr, 0, 0};
-  return {t.data_ptr(), t.stride(0), t.stride(1)};
+  return {t.data_ptr(), step ? 0 : t.stride(0), t.stride(step ? 0 : 1)};
 }
 // An output [T,N,...] that lies like `like`: time-major, or batch-first where that one is.
 Tensor output(const Tensor& like, std::vector<int64_t> sizes, at::TensorOptions o) {
@@ -83,10 +84,10 @@ struct Conv {
   haste_b200_causal_conv1d a{};
   Tensor x, weight, bias, state, lengths;
   Conv(const Tensor& x_, const Tensor& weight_, const OptTensor& bias_, const OptTensor& state_,
-       const OptTensor& lengths_, bool silu) {
-    dims(x_, "x", 3);
+       const OptTensor& lengths_, bool silu, bool step = false) {
+    dims(x_, "x", step ? 2 : 3);
     dims(weight_, "weight", 2);
-    const int64_t T = x_.size(0), N = x_.size(1), D = x_.size(2), W = weight_.size(1);
+    const int64_t T = step ? 1 : x_.size(0), N = x_.size(step ? 0 : 1), D = x_.size(-1), W = weight_.size(1);
     a.dtype = storage(x_);
     if (W < 2 || W > 4) refuse("weight must have 2, 3 or 4 taps, got " + shape_of(weight_));
     shape(weight_, "weight", {D, W});
@@ -110,7 +111,7 @@ struct Conv {
     state = contiguous(state);
     a.T = limited(T, "T"); a.N = limited(N, "N"); a.D = limited(D, "D"); a.W = (int)W;
     a.silu = silu;
-    a.x = view(x);
+    a.x = view(x, step);
     a.weight = ptr(weight); a.bias = ptr(bias); a.state = ptr(state);
     a.lengths = data<long long>(lengths);
   }
@@ -143,9 +144,14 @@ std::tuple<Tensor, Tensor> causal_conv1d_forward(const Tensor& x, const Tensor& 
 // One token: x [N,D].
 std::tuple<Tensor, Tensor> causal_conv1d_step(const Tensor& x, const Tensor& weight, const OptTensor& bias,
                                               const Tensor& state, bool silu, const OptTensor& out_state) {
-  dims(x, "x", 2);
-  auto [y, last] = causal_conv1d_forward(x.unsqueeze(0), weight, bias, state, {}, silu, out_state);
-  return {y.squeeze(0), last};
+  Conv c(x, weight, bias, state, {}, silu, true);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty({c.a.N, c.a.D}, x.options());
+  Tensor last = buffer(out_state, "out_state", x, {c.a.N, c.a.W - 1, c.a.D}, x.scalar_type());
+  c.a.y = view(y, true);
+  c.a.final_state = ptr(last);
+  CALL(causal_conv1d_forward, &c.a, stream());
+  return {y, last};
 }
 
 // Gradients of x, weight, bias, state (the last two only where given).
@@ -186,18 +192,24 @@ struct Scan {
   haste_b200_selective_scan a{};
   Tensor x, dt, A, B, C, skip, z, dt_bias, state, lengths;
   Scan(const Tensor& x_, const Tensor& dt_, const Tensor& A_, const Tensor& B_, const Tensor& C_, const OptTensor& skip_,
-       const OptTensor& z_, const OptTensor& dt_bias_, const OptTensor& state_, const OptTensor& lengths_, bool softplus) {
-    dims(x_, "x", 3);
+       const OptTensor& z_, const OptTensor& dt_bias_, const OptTensor& state_, const OptTensor& lengths_, bool softplus,
+       bool step = false) {
+    dims(x_, "x", step ? 2 : 3);
     dims(A_, "A", 2);
-    dims(B_, "B", 4);
-    const int64_t T = x_.size(0), N = x_.size(1), D = x_.size(2), S = A_.size(1), G = B_.size(2);
+    const bool grouped = !step || B_.dim() == 3;  // a step's B and C may be [N,S]
+    dims(B_, "B", grouped ? (step ? 3 : 4) : 2);
+    dims(C_, "C", B_.dim());
+    const int64_t T = step ? 1 : x_.size(0), N = x_.size(step ? 0 : 1), D = x_.size(-1), S = A_.size(1),
+                  G = grouped ? B_.size(-2) : 1;
     a.dtype = storage(x_);
     if (S < 1 || S > 128) refuse("A must have 1 to 128 states a channel, got " + shape_of(A_));
     if (G < 1 || D % G) refuse("the groups of B must divide the channels: " + std::to_string(G) + " and " + std::to_string(D));
     shape(A_, "A", {D, S});
-    shape(dt_, "dt", {T, N, D});
-    shape(B_, "B", {T, N, G, S});
-    shape(C_, "C", {T, N, G, S});
+    shape(dt_, "dt", {T, N, D}, step);
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(B_, "B"), {C_, "C"}}) {
+      if (grouped) shape(t, name, {T, N, G, S}, step);
+      else shape(t, name, {T, N, S}, step);
+    }
     skip = given(skip_); z = given(z_); dt_bias = given(dt_bias_); state = given(state_);
     const at::ScalarType t = x_.scalar_type();
     type(dt_, "dt", t);
@@ -205,7 +217,7 @@ struct Scan {
     type(C_, "C", t);
     type(A_, "A", at::kFloat);
     if (skip.defined()) { shape(skip, "D", {D}); type(skip, "D", at::kFloat); }
-    if (z.defined()) { shape(z, "z", {T, N, D}); type(z, "z", t); }
+    if (z.defined()) { shape(z, "z", {T, N, D}, step); type(z, "z", t); }
     if (dt_bias.defined()) { shape(dt_bias, "dt_bias", {D}); type(dt_bias, "dt_bias", at::kFloat); }
     if (state.defined()) { shape(state, "state", {N, D, S}); type(state, "state", at::kFloat); }
     lengths = row_lengths(lengths_, N);
@@ -214,8 +226,9 @@ struct Scan {
     A = A_.contiguous(); skip = contiguous(skip); dt_bias = contiguous(dt_bias); state = contiguous(state);
     a.T = limited(T, "T"); a.N = limited(N, "N"); a.D = limited(D, "D"); a.G = limited(G, "G"); a.S = (int)S;
     a.softplus = softplus;
-    a.x = view(x); a.dt = view(dt); a.z = view(z); a.B = view(B); a.C = view(C);
-    a.B_g = B.stride(2); a.C_g = C.stride(2);
+    a.x = view(x, step); a.dt = view(dt, step); a.z = view(z, step); a.B = view(B, step); a.C = view(C, step);
+    a.B_g = grouped ? B.stride(-2) : 0;
+    a.C_g = grouped ? C.stride(-2) : 0;
     a.A = data<float>(A); a.skip = data<float>(skip); a.dt_bias = data<float>(dt_bias); a.state = data<float>(state);
     a.lengths = data<long long>(lengths);
   }
@@ -248,13 +261,14 @@ std::tuple<Tensor, Tensor> selective_scan_step(const Tensor& x, const Tensor& dt
                                                const Tensor& C, const Tensor& state, const OptTensor& skip,
                                                const OptTensor& z, const OptTensor& dt_bias, bool softplus,
                                                const OptTensor& out_state) {
-  dims(x, "x", 2);
-  auto one = [](const Tensor& t) { return t.unsqueeze(0); };
-  auto group = [](const Tensor& t) { return t.dim() == 2 ? t.unsqueeze(1).unsqueeze(0) : t.unsqueeze(0); };
-  auto [y, last, saved] = selective_scan_forward(one(x), one(dt), A, group(B), group(C), skip,
-                                                 z ? OptTensor(one(*z)) : OptTensor(), dt_bias, state, {}, softplus, false,
-                                                 out_state);
-  return {y.squeeze(0), last};
+  Scan c(x, dt, A, B, C, skip, z, dt_bias, state, {}, softplus, true);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty({c.a.N, c.a.D}, x.options());
+  Tensor last = buffer(out_state, "out_state", x, {c.a.N, c.a.D, c.a.S}, at::kFloat);
+  c.a.y = view(y, true);
+  c.a.final_state = data<float>(last);
+  CALL(selective_scan_forward, &c.a, stream());
+  return {y, last};
 }
 
 // Gradients of x, dt, A, B, C, D, z, dt_bias, state (those of the optional ones where they are given).
