@@ -15,6 +15,7 @@ operators run on CUDA only, on the current stream, deterministically, and may be
 The reference has no counterpart of them.
 """
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _C, ops
@@ -22,12 +23,24 @@ from . import _C, ops
 __all__ = ["causal_conv1d", "causal_conv1d_step", "selective_scan", "selective_scan_step", "fused_norm"]
 
 
+_tracing_state = torch._C._get_tracing_state
+
+
+def _shown():
+    """Whether the tracer or forward-mode AD looks on: the compiled nodes do not show them what they
+    do, the autograd functions below say what can be recorded or differentiated."""
+    return _forward_ad._current_level >= 0 or _tracing_state() is not None
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _lengths(lengths, x):
-    return None if lengths is None else torch.as_tensor(lengths, device=x.device)
+    return torch.as_tensor(lengths, device=x.device)
+
+
+_native = _C.native
 
 
 def _float(t):
@@ -96,23 +109,24 @@ def causal_conv1d(x, weight, bias=None, initial_state=None, lengths=None, silu=T
     x [T,N,D], weight [D,W] with 2 to 4 taps, bias [D]; `initial_state` [N,W-1,D] holds the inputs
     before the first (zeros without it).  weight and bias have x's type or float32.
     Returns (y, final_state): the last W-1 inputs of each row."""
-    lengths = _lengths(lengths, x)
-    if _wants_grad(x, weight, bias, initial_state):
+    if lengths is not None:
+        lengths = _lengths(lengths, x)
+    if _shown():
         return _CausalConv1d.apply(silu, lengths, x, weight, bias, initial_state)
-    return _C.native().causal_conv1d_forward(x, weight, bias, initial_state, lengths, silu, None)
+    return _native().causal_conv1d(x, weight, bias, initial_state, lengths, silu)
 
 
 def causal_conv1d_step(x, state, weight, bias=None, silu=True, out_state=None):
     """One token: x [N,D].  Returns (y [N,D], new state); the new state goes into `out_state` where
     given, which may be `state` itself."""
-    if _wants_grad(x, state, weight, bias):
+    if _shown() or _wants_grad(x, state, weight, bias):
         if out_state is not None:
             raise ValueError("haste_b200: out_state is for calls without gradients")
         if x.dim() != 2:
             raise ValueError(f"haste_b200: x must have 2 dimensions, got {list(x.shape)}")
         y, state = causal_conv1d(x[None], weight, bias, state, silu=silu)
         return y[0], state
-    return _C.native().causal_conv1d_step(x, weight, bias, state, silu, out_state)
+    return _native().causal_conv1d_step(x, weight, bias, state, silu, out_state)
 
 
 def _grouped(m, dims):
@@ -126,20 +140,20 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     x, dt, z [T,N,D], A [D,S] (S up to 128), B, C [T,N,S] or, with G groups of D / G channels,
     [T,N,G,S]; D, dt_bias [D]; `initial_state` [N,D,S] float32 (zeros without it).  Without
     `softplus`, delta = dt + dt_bias.  Returns (y, final_state)."""
-    lengths = _lengths(lengths, x)
+    if lengths is not None:
+        lengths = _lengths(lengths, x)
     A, D, dt_bias = _float(A), _float(D), _float(dt_bias)
     B, C = _grouped(B, 3), _grouped(C, 3)
-    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
+    if _shown():
         return _SelectiveScan.apply(softplus, lengths, x, dt, A, B, C, D, z, dt_bias, initial_state)
-    return _C.native().selective_scan_forward(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths, softplus,
-                                              False, None)[:2]
+    return _native().selective_scan(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths, softplus)
 
 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=True, out_state=None):
     """One token: x, dt, z [N,D], B, C [N,S] or [N,G,S], state [N,D,S] float32.  Returns (y [N,D], new
     state); the new state goes into `out_state` where given, which may be `state` itself."""
     A, D, dt_bias = _float(A), _float(D), _float(dt_bias)
-    if _wants_grad(x, dt, A, B, C, state, D, z, dt_bias):
+    if _shown() or _wants_grad(x, dt, A, B, C, state, D, z, dt_bias):
         if out_state is not None:
             raise ValueError("haste_b200: out_state is for calls without gradients")
         if x.dim() != 2:
@@ -147,7 +161,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
         y, state = selective_scan(x[None], dt[None], A, _grouped(B, 2)[None], _grouped(C, 2)[None], D,
                                   None if z is None else z[None], dt_bias, state, softplus=softplus)
         return y[0], state
-    return _C.native().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, softplus, out_state)
+    return _native().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, softplus, out_state)
 
 
 def fused_norm(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1e-5, kind="rms"):
@@ -160,6 +174,6 @@ def fused_norm(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1
     if kind not in ("rms", "layer"):
         raise ValueError(f"haste_b200: kind must be 'rms' or 'layer', got {kind!r}")
     layer = kind == "layer"
-    if _wants_grad(x, weight, bias, gate, residual, scale):
+    if _shown():
         return _FusedNorm.apply(eps, layer, x, weight, bias, gate, residual, scale)
-    return _C.native().fused_norm_forward(x, weight, bias, gate, residual, scale, eps, layer, False)[:2]
+    return _native().fused_norm(x, weight, bias, gate, residual, scale, eps, layer)

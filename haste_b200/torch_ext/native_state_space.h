@@ -50,6 +50,7 @@ void devices(const Tensor& x, at::ArrayRef<Tensor> ts) {
   }
 }
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
+OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 // The kernels take any strides but along the last axis.
 Tensor unit_strided(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
@@ -183,7 +184,6 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> causal_conv1d_backward(
   Tensor scratch = floats(x, lib.causal_conv1d_scratch(&c.a));
   c.a.scratch = data<float>(scratch);
   CALL(causal_conv1d_backward, &c.a, stream());
-  auto maybe = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   return {dx, dw, maybe(db), maybe(ds)};
 }
 
@@ -362,7 +362,6 @@ std::tuple<Tensor, OptTensor, OptTensor> fused_norm_forward(const Tensor& x, con
   c.a.r = view(r);
   c.a.stats = data<float>(stats);
   CALL(fused_norm_forward, &c.a, stream());
-  auto maybe = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   return {y, maybe(r), maybe(stats)};
 }
 
@@ -402,9 +401,153 @@ std::vector<OptTensor> fused_norm_backward(const Tensor& x, const Tensor& weight
   return out;
 }
 
+// ------------------------------------------------------------------ with gradients
+// One autograd node a call.  The backward pass of a Python function costs a hundred microseconds of host
+// work, more than the kernels of a small batch.
+
+bool wants_grad(std::initializer_list<const OptTensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const OptTensor& t : ts)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that may be used but not differentiated again: that raises an error instead of giving zeros.
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list some;
+  for (const Tensor& t : grads)
+    if (t.defined()) some.push_back(t.detach().requires_grad_(true));
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("haste_b200: ") + name + " cannot be differentiated twice", (int64_t)some.size());
+  some = (*error)(std::move(some));
+  size_t i = 0;
+  for (Tensor& t : grads)
+    if (t.defined()) t = some[i++];
+  return grads;
+}
+
+// Runs a backward pass; the library's errors keep their Python type on the way through the engine.
+template <typename F>
+variable_list guarded(const char* name, const F& f) {
+  try {
+    variable_list grads;
+    {
+      const at::AutoGradMode off(false);
+      grads = f();
+    }
+    return once(std::move(grads), name);
+  } catch (const LibraryError& e) {
+    py::gil_scoped_acquire gil;
+    PyErr_SetString(haste_error, e.what());
+    python_error error;
+    error.persist();
+    throw error;
+  }
+}
+
+struct ConvNode : public torch::autograd::Function<ConvNode> {
+  static variable_list forward(AutogradContext* ctx, bool silu, OptTensor lengths, Tensor x, Tensor weight, OptTensor bias,
+                               OptTensor state) {
+    auto [y, last] = causal_conv1d_forward(x, weight, bias, state, lengths, silu, {});
+    ctx->save_for_backward({x, weight, given(bias), given(state), given(lengths)});
+    ctx->saved_data["silu"] = silu;
+    ctx->set_materialize_grads(false);
+    return {y, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    return guarded("causal_conv1d", [&]() -> variable_list {
+      const variable_list v = ctx->get_saved_variables();
+      const Tensor dy = grad[0].defined() ? grad[0] : at::zeros_like(v[0]);
+      auto [dx, dw, db, ds] = causal_conv1d_backward(v[0], v[1], maybe(v[2]), maybe(v[3]), maybe(v[4]),
+                                                     ctx->saved_data["silu"].toBool(), dy, maybe(grad[1]));
+      return {Tensor(), Tensor(), dx, dw, given(db), given(ds)};
+    });
+  }
+};
+
+std::tuple<Tensor, Tensor> causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& state,
+                                         const OptTensor& lengths, bool silu) {
+  if (!wants_grad({x, weight, bias, state})) return causal_conv1d_forward(x, weight, bias, state, lengths, silu, {});
+  const variable_list out = ConvNode::apply(silu, lengths, x, weight, bias, state);
+  return {out[0], out[1]};
+}
+
+struct ScanNode : public torch::autograd::Function<ScanNode> {
+  static variable_list forward(AutogradContext* ctx, bool softplus, OptTensor lengths, Tensor x, Tensor dt, Tensor A, Tensor B,
+                               Tensor C, OptTensor skip, OptTensor z, OptTensor dt_bias, OptTensor state) {
+    auto [y, last, saved] = selective_scan_forward(x, dt, A, B, C, skip, z, dt_bias, state, lengths, softplus, true, {});
+    ctx->save_for_backward({x, dt, A, B, C, given(skip), given(z), given(dt_bias), given(state), given(lengths), given(saved)});
+    ctx->saved_data["softplus"] = softplus;
+    ctx->set_materialize_grads(false);
+    return {y, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    return guarded("selective_scan", [&]() -> variable_list {
+      const variable_list v = ctx->get_saved_variables();
+      const Tensor dy = grad[0].defined() ? grad[0] : at::zeros_like(v[0]);
+      variable_list out(2);
+      for (const OptTensor& t :
+           selective_scan_backward(v[0], v[1], v[2], v[3], v[4], maybe(v[5]), maybe(v[6]), maybe(v[7]), maybe(v[8]),
+                                   maybe(v[9]), ctx->saved_data["softplus"].toBool(), v[10], dy, maybe(grad[1])))
+        out.push_back(given(t));
+      return out;
+    });
+  }
+};
+
+std::tuple<Tensor, Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                                          const OptTensor& skip, const OptTensor& z, const OptTensor& dt_bias,
+                                          const OptTensor& state, const OptTensor& lengths, bool softplus) {
+  if (!wants_grad({x, dt, A, B, C, skip, z, dt_bias, state})) {
+    auto [y, last, saved] = selective_scan_forward(x, dt, A, B, C, skip, z, dt_bias, state, lengths, softplus, false, {});
+    return {y, last};
+  }
+  const variable_list out = ScanNode::apply(softplus, lengths, x, dt, A, B, C, skip, z, dt_bias, state);
+  return {out[0], out[1]};
+}
+
+struct NormNode : public torch::autograd::Function<NormNode> {
+  static variable_list forward(AutogradContext* ctx, double eps, bool layer_norm, Tensor x, Tensor weight, OptTensor bias,
+                               OptTensor gate, OptTensor residual, OptTensor scale) {
+    auto [y, r, stats] = fused_norm_forward(x, weight, bias, gate, residual, scale, eps, layer_norm, true);
+    ctx->save_for_backward({x, weight, given(bias), given(gate), given(residual), given(scale), given(stats)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["layer_norm"] = layer_norm;
+    ctx->set_materialize_grads(false);
+    if (r) return {y, *r};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    return guarded("fused_norm", [&]() -> variable_list {
+      const variable_list v = ctx->get_saved_variables();
+      const Tensor dy = grad[0].defined() ? grad[0] : at::zeros_like(v[0]);
+      variable_list out(2);
+      for (const OptTensor& t :
+           fused_norm_backward(v[0], v[1], maybe(v[2]), maybe(v[3]), maybe(v[4]), maybe(v[5]), ctx->saved_data["eps"].toDouble(),
+                               ctx->saved_data["layer_norm"].toBool(), v[6], dy, grad.size() > 1 ? maybe(grad[1]) : OptTensor()))
+        out.push_back(given(t));
+      return out;
+    });
+  }
+};
+
+std::tuple<Tensor, OptTensor> fused_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& gate,
+                                         const OptTensor& residual, const OptTensor& scale, double eps, bool layer_norm) {
+  if (!wants_grad({x, weight, bias, gate, residual, scale})) {
+    auto [y, r, stats] = fused_norm_forward(x, weight, bias, gate, residual, scale, eps, layer_norm, false);
+    return {y, r};
+  }
+  const variable_list out = NormNode::apply(eps, layer_norm, x, weight, bias, gate, residual, scale);
+  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+}
+
 void bind(py::module& m) {
   const py::call_guard<py::gil_scoped_release> free;
   m.def("causal_conv1d_forward", &causal_conv1d_forward, free);
+  m.def("causal_conv1d", &causal_conv1d, free);
+  m.def("selective_scan", &selective_scan, free);
+  m.def("fused_norm", &fused_norm, free);
   m.def("causal_conv1d_step", &causal_conv1d_step, free);
   m.def("selective_scan_step", &selective_scan_step, free);
   m.def("causal_conv1d_backward", &causal_conv1d_backward, free);

@@ -478,3 +478,82 @@ def test_offsets_beyond_32_bits():
     off = (y[-100:].float() - tail[-100:].float()).abs().max()
     assert off <= 2 ** -7 * tail[-100:].float().abs().max()
     assert (state - last).abs().max() <= 1e-5 * last.abs().max()
+
+
+# ------------------------------------------------------------------ automatic differentiation
+def _calls(g, dtype=F32):
+    """One call of each operator: (function of its first input, that input)."""
+    from haste_b200 import ssm
+    d = scan_inputs(g, 5, 2, 8, 4, 1, dtype, {})
+    x = d.pop("x")
+    w, weight = torch.randn(8, 4, generator=g, device="cuda").to(dtype), torch.randn(8, generator=g, device="cuda").to(dtype)
+    return [(lambda v: ssm.causal_conv1d(v, w)[0], x), (lambda v: ssm.selective_scan(v, **d)[0], x),
+            (lambda v: ssm.fused_norm(v, weight, gate=d["z"])[0], x)]
+
+
+def test_a_second_derivative_is_refused():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for call, x in _calls(g):
+        x = x.detach().requires_grad_()
+        dx, = torch.autograd.grad(call(x).square().sum(), x, create_graph=True)
+        again, = torch.autograd.grad(call(x).square().sum(), x)
+        assert torch.equal(dx, again)
+        with pytest.raises(RuntimeError, match="differentiate.* twice"):
+            dx.sum().backward()
+
+
+def test_forward_mode_and_tracing_are_refused_or_right():
+    import torch.autograd.forward_ad as forward_ad
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for call, x in _calls(g):
+        with forward_ad.dual_level():
+            call(x)
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+        try:
+            traced = torch.jit.trace(call, x, check_trace=False)
+        except RuntimeError:
+            continue
+        other = torch.randn_like(x)
+        torch.testing.assert_close(traced(other), call(other))
+
+
+def test_saved_tensors_may_move():
+    d, w, weight = _block_inputs(9)
+    want = _block(d, w, weight)
+    with torch.autograd.graph.save_on_cpu():
+        got = _block(d, w, weight)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+def test_frozen_parameters():
+    """Only some inputs want gradients; the others' are dropped."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(4)
+    d = scan_inputs(g, 19, 2, 24, 16, 1, BF16, dict(state=True))
+    full = {k: v.detach().requires_grad_() for k, v in d.items()}
+    dy = seq(g, 19, 2, 24, BF16)
+    want = torch.autograd.grad(ssm.selective_scan(**full)[0], [full["dt"], full["B"]], dy)
+    some = d | {"dt": d["dt"].detach().requires_grad_(), "B": d["B"].detach().requires_grad_()}
+    got = torch.autograd.grad(ssm.selective_scan(**some)[0], [some["dt"], some["B"]], dy)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+def test_checkpointed_and_repeated_backward():
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for call, x in _calls(g):
+        x = x.detach().requires_grad_()
+        y = call(x)
+        a, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+        b, = torch.autograd.grad(y.sum(), x)
+        c, = torch.autograd.grad(checkpoint(call, x, use_reentrant=False).sum(), x)
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_library_errors_keep_their_type():
+    from haste_b200 import _C
+    with pytest.raises(_C.HasteError, match="dtype"):
+        _C.call("haste_b200_causal_conv1d_forward", b"\x07" * 512, None)
