@@ -46,29 +46,56 @@ __device__ __forceinline__ void input_at(const ConvArgs<T>& a, int t, int len, i
   }
 }
 
+// Two neighbouring channels to an instruction; V of them are (V + 1) / 2 pairs, one channel a pair with nothing.
+template <int V>
+__device__ __forceinline__ void pairs(const float (&v)[V], float2 (&p)[(V + 1) / 2]) {
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) p[i] = make_float2(v[2 * i], 2 * i + 1 < V ? v[2 * i + 1 < V ? 2 * i + 1 : 0] : 0.f);
+}
+template <int V>
+__device__ __forceinline__ void single(const float2 (&p)[(V + 1) / 2], float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = i % 2 ? p[i / 2].y : p[i / 2].x;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 sigmoid(float2 v) { return make_float2(ss::sigmoid(v.x), ss::sigmoid(v.y)); }
+
 // The taps of V neighbouring channels, W packs as they lie in memory, and their bias.
 template <typename T, int V, int W>
-__device__ __forceinline__ void parameters(const ConvArgs<T>& a, int d, float (&w)[W][V], float (&b)[V]) {
-  float flat[W * V];
+__device__ __forceinline__ void parameters(const ConvArgs<T>& a, int d, float2 (&w)[W][(V + 1) / 2], float2 (&b)[(V + 1) / 2]) {
+  float flat[W * V], row[V];
 #pragma unroll
   for (int k = 0; k < W; ++k) {
-    float part[V];
-    if (a.param_f32) load<float, V>(static_cast<const float*>(a.w) + (long long)d * W + k * V, part);
-    else load<T, V>(static_cast<const T*>(a.w) + (long long)d * W + k * V, part);
+    if (a.param_f32) load<float, V>(static_cast<const float*>(a.w) + (long long)d * W + k * V, row);
+    else load<T, V>(static_cast<const T*>(a.w) + (long long)d * W + k * V, row);
 #pragma unroll
-    for (int i = 0; i < V; ++i) flat[k * V + i] = part[i];
+    for (int i = 0; i < V; ++i) flat[k * V + i] = row[i];
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    b[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
+  for (int k = 0; k < W; ++k) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[k][i] = flat[i * W + k];
+    for (int i = 0; i < V; ++i) row[i] = flat[i * W + k];
+    pairs<V>(row, w[k]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) row[i] = a.b ? ldp<T>(a.b, a.param_f32, d + i) : 0.f;
+  pairs<V>(row, b);
+}
+
+// bias + sum_k w_k x_k of a window
+template <int P, int W>
+__device__ __forceinline__ void convolve(const float2 (&w)[W][P], const float2 (&b)[P], const float2 (&x)[W][P], float2 (&p)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    p[i] = b[i];
+#pragma unroll
+    for (int k = 0; k < W; ++k) p[i] = __ffma2_rn(w[k][i], x[k][i], p[i]);
   }
 }
 
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
-  constexpr int G = GROUP<T, V>;
+  constexpr int G = GROUP<T, V>, P = (V + 1) / 2;
   const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
   const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
   if (d >= a.D) return;
@@ -82,33 +109,42 @@ __global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
     px += (long long)G * a.x.t;
   };
   fetch(t0, in);
-  float w[W][V], b[V], xs[W][V];  // xs: the window, its last row the step at hand
+  float2 w[W][P], b[P], xs[W][P];  // xs: the window, its last row the step at hand
+  float row[V];
   parameters<T, V, W>(a, d, w, b);
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
+  for (int k = 0; k < W - 1; ++k) {
+    input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, row);
+    pairs<V>(row, xs[k + 1]);
+  }
   T* py = a.y.at(t0, n) + d;
   for (int t = t0; t < t1; t += G) {
     Raw<T, V> next[G];
     fetch(t + G, next);
+    float2 y[G][P];
 #pragma unroll
     for (int u = 0; u < G; ++u) {
 #pragma unroll
       for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) xs[k][i] = xs[k + 1][i];
-      unpack<T, V>(in[u], xs[W - 1]);
-      float y[V];
+        for (int i = 0; i < P; ++i) xs[k][i] = xs[k + 1][i];
+      unpack<T, V>(in[u], row);
+      pairs<V>(row, xs[W - 1]);
+      convolve<P, W>(w, b, xs, y[u]);
+    }
+    // (all sigmoids of the group together: each is a chain of two slow instructions)
+    if (a.silu)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float p = b[i];
+      for (int u = 0; u < G; ++u)
 #pragma unroll
-        for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
-        y[i] = a.silu ? silu(p) : p;
-      }
+        for (int i = 0; i < P; ++i) y[u][i] = __fmul2_rn(y[u][i], sigmoid(y[u][i]));
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
       if (t + u >= len)
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = 0.f;
-      if (t + u < t1) store<T, V>(py + (long long)u * a.y.t, y);
+        for (int i = 0; i < P; ++i) y[u][i] = both(0.f);
+      single<V>(y[u], row);
+      if (t + u < t1) store<T, V>(py + (long long)u * a.y.t, row);
     }
     py += (long long)G * a.y.t;
 #pragma unroll
@@ -120,9 +156,8 @@ __global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
   if (c == 0 && a.final_state) {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
-      float v[V];
-      input_at<T, V, W>(a, len - (W - 1) + k, len, n, d, v);
-      store<T, V>(a.final_state + ((long long)n * (W - 1) + k) * a.D + d, v);
+      input_at<T, V, W>(a, len - (W - 1) + k, len, n, d, row);
+      store<T, V>(a.final_state + ((long long)n * (W - 1) + k) * a.D + d, row);
     }
   }
 }
@@ -132,17 +167,18 @@ __global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
 // the chunks that a block takes in turn; its partial rows are added in a fixed order afterwards.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
-  constexpr int G = 4;
+  constexpr int G = 4, P = (V + 1) / 2;
   const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
   const int part = blockIdx.x / a.dtiles;
   if (d >= a.D) return;
-  float w[W][V], b[V], dw[W][V], db[V];
+  float2 w[W][P], b[P], dw[W][P], db[P];
+  float row[V];
   parameters<T, V, W>(a, d, w, b);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    db[i] = 0.f;
+  for (int i = 0; i < P; ++i) {
+    db[i] = both(0.f);
 #pragma unroll
-    for (int k = 0; k < W; ++k) dw[k][i] = 0.f;
+    for (int k = 0; k < W; ++k) dw[k][i] = both(0.f);
   }
   for (int item = part; item < a.items; item += a.parts) {
     const int n = item % a.N, c = item / a.N;
@@ -160,63 +196,73 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
       pg += (long long)G * a.dy.t;
     };
     fetch(t0, in, gr);
-    float xs[W][V], dp[W][V];
+    float2 xs[W][P], dp[W][P];
 #pragma unroll
     for (int k = 0; k < W; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) dp[k][i] = 0.f;
+      for (int i = 0; i < P; ++i) dp[k][i] = both(0.f);
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, xs[k + 1]);
+    for (int k = 0; k < W - 1; ++k) {
+      input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, row);
+      pairs<V>(row, xs[k + 1]);
+    }
     for (int t = t0; t < end; t += G) {
       Raw<T, V> xn[G], gn[G];
       fetch(t + G, xn, gn);
 #pragma unroll
       for (int u = 0; u < G; ++u) {
-        const bool mine = t + u < t1;
         const int te = t + u - (W - 1);  // the step whose dx is complete now
-        float dx[V], g[V];
+        float2 dx[P], g[P];
 #pragma unroll
         for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
+          for (int i = 0; i < P; ++i) {
             xs[k][i] = xs[k + 1][i];
             dp[k][i] = dp[k + 1][i];
           }
-        unpack<T, V>(in[u], xs[W - 1]);
-        unpack<T, V>(gr[u], g);
+        unpack<T, V>(in[u], row);
+        pairs<V>(row, xs[W - 1]);
+        unpack<T, V>(gr[u], row);
+        pairs<V>(row, g);
+        if (a.silu) {
+          float2 p[P];
+          convolve<P, W>(w, b, xs, p);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (a.silu) {
-            float p = b[i];
-#pragma unroll
-            for (int k = 0; k < W; ++k) p = fmaf(w[k][i], xs[k][i], p);
-            // (behind the row's end the incoming gradient counts for nothing, whatever p is)
-            g[i] = t + u < len ? g[i] * silu_slope(p, sigmoid(p)) : 0.f;
+          for (int i = 0; i < P; ++i) {
+            const float2 s = sigmoid(p[i]), rest = __ffma2_rn(s, both(-1.f), both(1.f));
+            g[i] = __fmul2_rn(g[i], __ffma2_rn(__fmul2_rn(p[i], s), rest, s));
           }
-          dp[W - 1][i] = g[i];
-          dx[i] = w[0][i] * dp[W - 1][i];
+          if (t + u >= len)  // (the incoming gradient counts for nothing, whatever p is)
 #pragma unroll
-          for (int k = 1; k < W; ++k) dx[i] = fmaf(w[k][i], dp[W - 1 - k][i], dx[i]);
+            for (int i = 0; i < P; ++i) g[i] = both(0.f);
         }
-        if (mine)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            db[i] += g[i];
+        for (int i = 0; i < P; ++i) {
+          dp[W - 1][i] = g[i];
+          dx[i] = __fmul2_rn(w[0][i], g[i]);
 #pragma unroll
-            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g[i], xs[k][i], dw[k][i]);
+          for (int k = 1; k < W; ++k) dx[i] = __ffma2_rn(w[k][i], dp[W - 1 - k][i], dx[i]);
+        }
+        if (t + u < t1)
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            db[i] = __fadd2_rn(db[i], g[i]);
+#pragma unroll
+            for (int k = 0; k < W; ++k) dw[k][i] = __ffma2_rn(g[i], xs[k][i], dw[k][i]);
           }
         const bool before = te < 0;  // a row of the initial state
         if (t + u >= end || (before ? c != 0 : te < t0)) continue;
+        single<V>(dx, row);
         if (a.dfinal && te >= len - (W - 1) && te < len) {
           float f[V];
           load<T, V>(a.dfinal + ((long long)n * (W - 1) + te - len + W - 1) * a.D + d, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) dx[i] += f[i];
+          for (int i = 0; i < V; ++i) row[i] += f[i];
         }
         if (!before) {
-          if (a.dx.p) store<T, V>(a.dx.at(te, n) + d, dx);
+          if (a.dx.p) store<T, V>(a.dx.at(te, n) + d, row);
         } else if (a.dstate) {
-          store<T, V>(a.dstate + ((long long)n * (W - 1) + te + W - 1) * a.D + d, dx);
+          store<T, V>(a.dstate + ((long long)n * (W - 1) + te + W - 1) * a.D + d, row);
         }
       }
 #pragma unroll
@@ -227,15 +273,18 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
     }
   }
   // partial row of this block: [D][W] of dw, then [D] of db
-  float* row = a.part + (long long)part * a.D * (W + 1);
+  float* sums = a.part + (long long)part * a.D * (W + 1);
 #pragma unroll
   for (int k = 0; k < W; ++k) {  // in memory order
-    float flat[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) flat[i] = dw[(k * V + i) % W][(k * V + i) / W];
-    store<float, V>(row + (long long)d * W + k * V, flat);
+    for (int i = 0; i < V; ++i) {
+      const int at = k * V + i;
+      row[i] = at / W % 2 ? dw[at % W][at / W / 2].y : dw[at % W][at / W / 2].x;
+    }
+    store<float, V>(sums + (long long)d * W + k * V, row);
   }
-  store<float, V>(row + (long long)a.D * W + d, db);
+  single<V>(db, row);
+  store<float, V>(sums + (long long)a.D * W + d, row);
 }
 
 int check(const haste_b200_causal_conv1d& a, bool backward) {
@@ -268,23 +317,24 @@ int width(const haste_b200_causal_conv1d& a, bool backward) {
 }
 
 struct Shape {
-  int threads, dtiles, chunk, chunks;
-  Shape(const haste_b200_causal_conv1d& a, int v) {
+  int threads, dtiles, chunk, chunks, parts;
+  Shape(const haste_b200_causal_conv1d& a, int v, bool backward) {
     const int lanes = ceil_div(a.D, v);
     threads = std::min(128, ceil_div(lanes, 32) * 32);
     dtiles = ceil_div(lanes, threads);
-    // A chunk reads W - 1 steps twice, so long chunks while there are threads to fill the GPU.
-    chunk = 64;
-    while (chunk > 8 && (long long)lanes * a.N * ceil_div(a.T, chunk) < 512LL * sm_count()) chunk /= 2;
+    // One wave: as many chunks as the resident blocks (five an SM; three in the backward pass, whose
+    // windows and sums take 150 registers), of 16 steps at least.  A chunk reads W - 1 steps twice.
+    // fp32 T=400 N=64 D=1024, us forward / backward: chunks of 64 steps, 1.2 / 2 waves, 47 / 69.
+    const int per = std::max(1, (backward ? 3 : 5) * sm_count() / dtiles);
+    chunks = std::max(1, std::min(per / a.N, ceil_div(a.T, 16)));
+    chunk = std::max(4, ceil_div(ceil_div(a.T, chunks), 4) * 4);
     chunks = std::max(1, ceil_div(a.T, chunk));
+    // rows of partial sums in the backward pass; a block takes as many items as the next one
+    const long long rounds = (items(a.N) + per - 1) / per;
+    parts = (int)((items(a.N) + rounds - 1) / rounds);
   }
   long long items(int N) const { return (long long)chunks * N; }
 };
-
-// Blocks of the backward pass that share a row of partial sums: about eight per SM.
-int parts(const haste_b200_causal_conv1d& a, const Shape& s) {
-  return (int)std::max(1LL, std::min(s.items(a.N), (long long)ceil_div(8LL * sm_count(), s.dtiles)));
-}
 
 template <typename T>
 ConvArgs<T> pack(const haste_b200_causal_conv1d& a, const Shape& s) {
@@ -301,13 +351,13 @@ ConvArgs<T> pack(const haste_b200_causal_conv1d& a, const Shape& s) {
   k.dstate = static_cast<T*>(a.dstate);
   k.part = a.scratch;
   k.items = (int)s.items(a.N);
-  k.parts = parts(a, s);
+  k.parts = s.parts;
   return k;
 }
 
 template <typename T, int V, int W>
 int launch(const haste_b200_causal_conv1d& a, bool backward, cudaStream_t st) {
-  const Shape s(a, V);
+  const Shape s(a, V, backward);
   HB_REQUIRE(s.items(a.N) * s.dtiles < (1LL << 31), "T*N too large");
   const ConvArgs<T> k = pack<T>(a, s);
   if (backward) {
@@ -362,7 +412,7 @@ long long causal_conv1d_scratch(const haste_b200_causal_conv1d& a) {
   // (enough for every width: the pointers that decide on it may not be there yet)
   if (a.N <= 0 || a.D <= 0 || a.T < 0) return 0;
   long long rows = 0;
-  for (int v = 1; v <= 4; v *= 2) rows = std::max(rows, (long long)parts(a, Shape(a, v)));
+  for (int v = 1; v <= 4; v *= 2) rows = std::max(rows, (long long)Shape(a, v, true).parts);
   return rows * a.D * (a.W + 1);
 }
 

@@ -218,6 +218,9 @@ __global__ void __launch_bounds__(512) norm_bwd(NormArgs<T, R, P> a) {
   int turn = 0;
   Row<true, T, R, P, V, K> now, next;
   now.fetch(a, blockIdx.x, col);
+  // By twos: copying `next` would wait for its loads, two turns exchange the registers instead.  (184 -> 171 us at
+  // 64000 x 1024 in bf16; in fp32 the registers do not suffice, and the forward pass has enough blocks without.)
+#pragma unroll(sizeof(T) == 2 ? 2 : 1)
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const Where at(a, row);
     Line<R, V> dr[K];

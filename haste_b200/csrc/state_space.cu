@@ -7,7 +7,7 @@ namespace {
 
 constexpr int kCols = 32, kRows = 32;
 
-// 32 columns x 32 groups of rows: thread (r, c) adds rows r, r + 32, ... of its column, four loads ahead,
+// 32 columns x 32 groups of rows: thread (r, c) adds rows r, r + 32, ... of its column, eight loads ahead,
 // and the sums are added in order.  The partials were written just before and lie in L2.
 __global__ void __launch_bounds__(kCols* kRows) sum_parts_kernel(const float* __restrict__ part, int P,
                                                                  long long stride, SumJobs jobs) {
@@ -20,11 +20,11 @@ __global__ void __launch_bounds__(kCols* kRows) sum_parts_kernel(const float* __
   float s = 0.f;
   if (j < job.width) {
     int i = r;
-    for (; i + 3 * kRows < P; i += 4 * kRows) {
-      float v[4];
+    for (; i + 7 * kRows < P; i += 8 * kRows) {
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = p[(i + k * kRows) * stride];
-      s += (v[0] + v[1]) + (v[2] + v[3]);
+      for (int k = 0; k < 8; ++k) v[k] = p[(i + k * kRows) * stride];
+      s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     }
     for (; i < P; i += kRows) s += p[i * stride];
   }
