@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
 int check(const haste_b200_causal_conv1d& a, bool backward) {
   HB_REQUIRE(storage_dtype(a.dtype), "dtype");
   HB_REQUIRE(a.param_dtype == HASTE_B200_F32 || a.param_dtype == a.dtype, "param_dtype");
-  HB_REQUIRE(a.T >= 0 && a.N >= 0 && a.D >= 0, "T,N,D");
+  HB_REQUIRE(a.T >= 0 && a.T <= (1 << 30) && a.N >= 0 && a.D >= 0, "T,N,D");
   HB_REQUIRE(a.W >= 2 && a.W <= 4, "W must be 2, 3 or 4");
   HB_REQUIRE((long long)a.D * (a.W + 1) < (1LL << 31), "D");
   HB_REQUIRE(strides_fit(a.T, a.x) && strides_fit(a.T, a.y) && strides_fit(a.T, a.dy) && strides_fit(a.T, a.dx),

@@ -15,7 +15,7 @@ extern template int backward<__half>(const haste_b200_selective_scan&, cudaStrea
 
 int check(const haste_b200_selective_scan& a, bool backward) {
   HB_REQUIRE(storage_dtype(a.dtype), "dtype");
-  HB_REQUIRE(a.T >= 0 && a.N >= 0 && a.D >= 0, "T,N,D");
+  HB_REQUIRE(a.T >= 0 && a.T <= (1 << 30) && a.N >= 0 && a.D >= 0, "T,N,D");
   HB_REQUIRE(a.S >= 1 && a.S <= 128, "S must be 1..128");
   HB_REQUIRE(a.G >= 1 && a.D % a.G == 0, "G must divide D");
   HB_REQUIRE((long long)a.D * (a.S + 2) < (1LL << 31) && (long long)a.N * a.D < (1LL << 31), "N*D too large");

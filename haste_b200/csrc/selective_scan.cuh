@@ -14,6 +14,7 @@ constexpr int CKPT = 8;  // steps between the states that the forward pass leave
 template <typename T>
 struct Args {
   int T_, N, D, G, S, per, ctiles;  // per: channels of a group, ctiles: blocks that share them out
+  int n0, rows, most;               // the rows of this launch, and the most of any
   int chunks, chunk;                // pieces of the sequence that blocks work on side by side, steps of one
   bool softplus;
   Seq<const T> x, dt, z, B, C, dy;
@@ -34,8 +35,8 @@ struct Place {
     ct = blockIdx.x % a.ctiles;
     g = r % a.G;
     r /= a.G;
-    n = r % a.N;
-    piece = r / a.N;
+    n = a.n0 + r % a.rows;
+    piece = r / a.rows;
     d0 = g * a.per + ct * CB;
     count = min(CB, a.per - ct * CB);
     first = piece * a.chunk;
@@ -205,15 +206,16 @@ int forward_pieces(const haste_b200_selective_scan& a);
 // How a backward call is cut: channels per thread, and pieces of the sequence.
 struct BwdShape {
   int Q, CH, ctiles, chunks, chunk;
-  long long blocks;  // of a piece
+  int rows;          // of one launch
+  long long blocks;  // of a piece and all rows
   explicit BwdShape(const haste_b200_selective_scan& a) {
     Q = lanes(a.S);
     const int per = a.D / a.G, CB = THREADS / Q;
-    const long long rows = (long long)a.N * a.G;
+    const long long lines = (long long)a.N * a.G;
     // two channels a thread while their blocks fill the GPU (bf16 T=1000 N=64 D=1024 S=16: 1735 us with one, 1617 with two)
-    CH = rows * ceil_div(per, 2 * CB) >= 3LL * sm_count() ? 2 : 1;
+    CH = lines * ceil_div(per, 2 * CB) >= 3LL * sm_count() ? 2 : 1;
     ctiles = ceil_div(per, CB * CH);
-    blocks = rows * ctiles;
+    blocks = lines * ctiles;
     chunks = 1;
     chunk = a.T > 0 ? a.T : 1;
     // As in the forward pass; the walk that pieces add is a quarter of the pass.  fp32 T=333 N=7 D=250 S=24, us:
@@ -225,9 +227,15 @@ struct BwdShape {
         chunks = ceil_div(a.T, chunk);
       }
     }
+    // Many states make few channels a block and many partial rows of dB and dC: beyond a GB of them the rows
+    // of the batch are taken in turn, as long as each turn fills the GPU.
+    const long long a_row = (long long)ctiles * a.T * a.G * 2 * Q * NS, fill = (3LL * sm_count() * a.N + blocks * chunks - 1) / (blocks * chunks);
+    long long most = a_row > 0 ? (1LL << 28) / a_row : a.N;
+    if (most < fill) most = fill;
+    rows = most < 1 ? 1 : most < a.N ? (int)most : a.N;
   }
   // scratch: partial rows of dB and dC, sums of dA, dskip and ddt_bias, the pieces' ends
-  long long bc_floats(const haste_b200_selective_scan& a) const { return (long long)ctiles * a.T * a.N * a.G * 2 * Q * NS; }
+  long long bc_floats(const haste_b200_selective_scan& a) const { return (long long)ctiles * a.T * rows * a.G * 2 * Q * NS; }
   long long sum_floats(const haste_b200_selective_scan& a) const { return (long long)chunks * a.N * a.D * (a.S + 2); }
   long long floats(const haste_b200_selective_scan& a) const {
     return bc_floats(a) + sum_floats(a) + (chunks > 1 ? (long long)chunks * a.N * a.D * (a.S + 1) : 0);
@@ -237,7 +245,7 @@ struct BwdShape {
 template <typename T>
 Args<T> pack(const haste_b200_selective_scan& a, int CB) {
   Args<T> k;
-  k.T_ = a.T; k.N = a.N; k.D = a.D; k.G = a.G; k.S = a.S;
+  k.T_ = a.T; k.N = a.N; k.n0 = 0; k.rows = k.most = a.N; k.D = a.D; k.G = a.G; k.S = a.S;
   k.per = a.D / a.G;
   k.ctiles = ceil_div(k.per, CB);
   k.chunks = 1;

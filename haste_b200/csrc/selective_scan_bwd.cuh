@@ -19,7 +19,7 @@ namespace {
 
 // Lanes, channels and shared memory as in the forward kernel.  dB and dC are sums over channels: a thread
 // adds its CH channels, then they are added over the lanes of a warp, over the warps in shared memory,
-// and over the blocks from partial rows [ctiles][T][N][G][2][SP], all in a fixed order.
+// and over the blocks from partial rows [ctiles][T][rows][G][2][SP], all in a fixed order.
 template <int Q, int CH>
 struct Shared {
   using F = Tile<Q, CH, CKPT>;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) s += m.red[w][k][i];
-      a.part[((((long long)at.ct * a.T_ + t0 + k) * a.N + n) * a.G + at.g) * (2 * SP) + i] = s;
+      a.part[((((long long)at.ct * a.T_ + t0 + k) * a.rows + n - a.n0) * a.G + at.g) * (2 * SP) + i] = s;
     }
     float skip[V], ds[V], db[V];
     parameter(a.skip, skip);
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
     store<float, V>(&m.sums[1][tid].x, db);
   }
   // row (piece, n) of the partial sums: dA [D][S], dskip [D], ddt_bias [D]
-  float* sums = a.part + (long long)a.ctiles * a.T_ * a.N * a.G * (2 * SP) +
+  float* sums = a.part + (long long)a.ctiles * a.T_ * a.most * a.G * (2 * SP) +
                 ((long long)at.piece * a.N + n) * a.D * (a.S + 2);
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
@@ -492,39 +492,32 @@ __global__ void __launch_bounds__(256) scan_bwd_finish(Args<T> a, int SP, long l
   float v = 0.f;
 #pragma unroll 8
   for (int ct = 0; ct < a.ctiles; ++ct) v += p[(long long)ct * rows * (2 * SP)];
-  const int g = (int)(r % a.G), n = (int)(r / a.G % a.N);
-  const long long t = r / a.G / a.N;
+  const int g = (int)(r % a.G), n = a.n0 + (int)(r / a.G % a.rows);
+  const int t = (int)(r / a.G / a.rows);
   if (which == 0) st(a.dB.at(t, n) + g * a.dB_g + s, v);
   else st(a.dC.at(t, n) + g * a.dC_g + s, v);
 }
 
 template <typename T, int Q, int CH, int V, bool Gate>
-int launch_scan(const Args<T>& k, const BwdShape& sh, cudaStream_t s) {
+int launch_scan(const Args<T>& k, cudaStream_t s) {
   constexpr int bytes = sizeof(Shared<Q, CH>);
   if (bytes > 48 * 1024)
     HB_CUDA_OK(cudaFuncSetAttribute(scan_bwd<T, Q, CH, V, Gate>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  scan_bwd<T, Q, CH, V, Gate><<<(int)(sh.blocks * sh.chunks), THREADS, bytes, s>>>(k);
+  scan_bwd<T, Q, CH, V, Gate><<<k.rows * k.G * k.ctiles * k.chunks, THREADS, bytes, s>>>(k);
   HB_LAUNCH_OK();
   return HASTE_B200_OK;
 }
 template <typename T, int Q, int CH, int V>
-int by_gate(const Args<T>& k, const BwdShape& sh, cudaStream_t s) {
-  return k.z.p ? launch_scan<T, Q, CH, V, true>(k, sh, s) : launch_scan<T, Q, CH, V, false>(k, sh, s);
+int by_gate(const Args<T>& k, cudaStream_t s) {
+  return k.z.p ? launch_scan<T, Q, CH, V, true>(k, s) : launch_scan<T, Q, CH, V, false>(k, s);
 }
 
 template <typename T, int Q>
-int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
-  const BwdShape sh(a);
-  HB_REQUIRE(sh.blocks * sh.chunks < (1LL << 31), "N*D too large");
-  Args<T> k = pack<T>(a, THREADS / Q * sh.CH);
-  k.chunks = sh.chunks;
-  k.chunk = sh.chunk;
+int launch_rows(const haste_b200_selective_scan& a, const Args<T>& k, const BwdShape& sh, cudaStream_t s) {
   if (sh.chunks > 1) {
-    k.ends = a.scratch + sh.bc_floats(a) + sh.sum_floats(a);
-    k.sums = k.ends + (long long)sh.chunks * a.N * a.D * a.S;
     Args<T> e = k;
     e.ctiles = ceil_div(k.per, THREADS / Q);
-    const int blocks = a.N * a.G * e.ctiles * (sh.chunks - 1);
+    const int blocks = k.rows * a.G * e.ctiles * (sh.chunks - 1);
     constexpr int V = Tile<Q, 1, fwd_steps(Q)>::V;
     if (V > 1 && wide(a, V, true)) {
       if (k.z.p) scan_bwd_ends<T, Q, V, true><<<blocks, THREADS, 0, s>>>(e);
@@ -538,19 +531,38 @@ int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
   }
   constexpr int V1 = Tile<Q, 1, CKPT>::V, V2 = Tile<Q, 2, CKPT>::V;
   if (sh.CH == 2) {
-    if (wide(a, V2, true)) HB_TRY((by_gate<T, Q, 2, V2>(k, sh, s)));
-    else HB_TRY((by_gate<T, Q, 2, 1>(k, sh, s)));
+    if (wide(a, V2, true)) HB_TRY((by_gate<T, Q, 2, V2>(k, s)));
+    else HB_TRY((by_gate<T, Q, 2, 1>(k, s)));
   } else {
-    if (wide(a, V1, true)) HB_TRY((by_gate<T, Q, 1, V1>(k, sh, s)));
-    else HB_TRY((by_gate<T, Q, 1, 1>(k, sh, s)));
+    if (wide(a, V1, true)) HB_TRY((by_gate<T, Q, 1, V1>(k, s)));
+    else HB_TRY((by_gate<T, Q, 1, 1>(k, s)));
   }
-  const long long rows = (long long)a.T * a.N * a.G;
+  const long long rows = (long long)a.T * k.rows * a.G;
   if (rows) {
     HB_REQUIRE(rows * 2 * a.S / 256 < (1LL << 31) - 1, "T*N too large");
     scan_bwd_finish<T><<<ceil_div(rows * 2 * a.S, 256), 256, 0, s>>>(k, Q * NS, rows);
     HB_LAUNCH_OK();
   }
   count_launch(rows ? 2 : 1);
+  return HASTE_B200_OK;
+}
+
+template <typename T, int Q>
+int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
+  const BwdShape sh(a);
+  HB_REQUIRE(sh.blocks * sh.chunks < (1LL << 31), "N*D too large");
+  Args<T> k = pack<T>(a, THREADS / Q * sh.CH);
+  k.chunks = sh.chunks;
+  k.chunk = sh.chunk;
+  k.most = sh.rows;
+  if (sh.chunks > 1) {
+    k.ends = a.scratch + sh.bc_floats(a) + sh.sum_floats(a);
+    k.sums = k.ends + (long long)sh.chunks * a.N * a.D * a.S;
+  }
+  for (k.n0 = 0; k.n0 < a.N; k.n0 += sh.rows) {
+    k.rows = std::min(sh.rows, a.N - k.n0);
+    HB_TRY((launch_rows<T, Q>(a, k, sh, s)));
+  }
   SumJobs jobs;
   jobs.add(a.dA, 0, 1, a.D * a.S, HASTE_B200_F32);
   jobs.add(a.dskip, (long long)a.D * a.S, 1, a.D, HASTE_B200_F32);

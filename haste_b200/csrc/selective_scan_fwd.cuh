@@ -212,44 +212,74 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
 }
 
 // A single step: the states are read and written once, so HBM (or, for few rows, the launch) bounds it.
-// Q lanes of four states per (row, channel).
-template <typename T, int Q>
-__global__ void __launch_bounds__(256) scan_step(Args<T> a) {
-  const long long pair = ((long long)blockIdx.x * 256 + threadIdx.x) / Q;
-  const int lane = threadIdx.x % 32, s0 = (threadIdx.x % Q) * NS;
-  const bool ok = pair < (long long)a.N * a.D;
-  const int n = ok ? (int)(pair / a.D) : 0, d = ok ? (int)(pair % a.D) : 0, g = d / a.per;
-  const bool live = row_length(a.lengths, n, 1) > 0;
-  float2 A[2], h[2] = {};
-  load_states(a.A + (long long)d * a.S, s0, a.S, A);
-  const long long row = ((long long)n * a.D + d) * a.S;
-  if (a.state) load_states(a.state + row, s0, a.S, h);
-  float x = 0.f, y = 0.f;
-  if (live) {
-    x = ld(a.x.at(0, n) + d);
-    const float v = ld(a.dt.at(0, n) + d) + (a.dt_bias ? a.dt_bias[d] : 0.f);
-    const float delta = a.softplus ? softplus(v) : v, u = delta * x;
-    const T *B = a.B.at(0, n) + g * a.B_g, *C = a.C.at(0, n) + g * a.C_g;
+// Q lanes of four states per channel; a thread takes R rows, whose loads go out together.
+template <typename T, int Q, int R, bool Fours>
+__global__ void __launch_bounds__(256) scan_step(Args<T> a, int dblocks) {
+  const int at = blockIdx.x % dblocks * 256 + threadIdx.x, d = at / Q, s0 = at % Q * NS;
+  const int n0 = blockIdx.x / dblocks * R;
+  const bool ok = d < a.D;
+  const int dd = ok ? d : 0, g = dd / a.per;
+  float2 A[2], h[R][2] = {};
+  Raw<T, 1> x[R], dt[R], z[R];
+  Raw<T, Fours ? 4 : 1> B[R][Fours ? 1 : 4], C[R][Fours ? 1 : 4];
+  load_states(a.A + (long long)dd * a.S, s0, a.S, A);
+  const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f, skip = a.skip ? a.skip[dd] : 0.f;
+  bool live[R];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = s0 + 2 * i;
-      const float2 b = make_float2(s < a.S ? ld(B + s) : 0.f, s + 1 < a.S ? ld(B + s + 1) : 0.f);
-      const float2 w = make_float2(s < a.S ? ld(C + s) : 0.f, s + 1 < a.S ? ld(C + s + 1) : 0.f);
-      h[i] = __ffma2_rn(decay(make_float2(delta, delta), __fmul2_rn(A[i], make_float2(LOG2E, LOG2E))), h[i],
-                        __fmul2_rn(make_float2(u, u), b));
-      y = fmaf(h[i].x, w.x, fmaf(h[i].y, w.y, y));
+  for (int r = 0; r < R; ++r) {
+    const int n = n0 + r;
+    live[r] = ok && n < a.N && row_length(a.lengths, n, 1) > 0;
+    if (ok && n < a.N && a.state) load_states(a.state + ((long long)n * a.D + d) * a.S, s0, a.S, h[r]);
+    x[r] = load_if<T, 1>(live[r], a.x.at(0, n) + dd);
+    dt[r] = load_if<T, 1>(live[r], a.dt.at(0, n) + dd);
+    z[r] = load_if<T, 1>(live[r] && a.z.p, a.z.at(0, n) + dd);
+    const T *pb = a.B.at(0, n) + g * a.B_g + s0, *pc = a.C.at(0, n) + g * a.C_g + s0;
+    if constexpr (Fours) {
+      B[r][0] = load_if<T, 4>(live[r] && s0 < a.S, pb);
+      C[r][0] = load_if<T, 4>(live[r] && s0 < a.S, pc);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        B[r][i] = load_if<T, 1>(live[r] && s0 + i < a.S, pb + i);
+        C[r][i] = load_if<T, 1>(live[r] && s0 + i < a.S, pc + i);
+      }
     }
   }
-  if (ok && a.final_state) store_states(a.final_state + row, s0, a.S, h);
 #pragma unroll
-  for (int o = Q / 2; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (ok && lane % Q == 0) {
-    y = live ? fmaf(a.skip ? a.skip[d] : 0.f, x, y) : 0.f;
-    if (live && a.z.p) y *= silu(ld(a.z.at(0, n) + d));
-    st(a.y.at(0, n) + d, y);
+  for (int i = 0; i < 2; ++i) A[i] = __fmul2_rn(A[i], both(LOG2E));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int n = n0 + r;
+    float b[4], c[4];
+    if constexpr (Fours) {
+      unpack<T, 4>(B[r][0], b);
+      unpack<T, 4>(C[r][0], c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b[i] = one(B[r][i]);
+        c[i] = one(C[r][i]);
+      }
+    }
+    const float xv = one(x[r]), v = one(dt[r]) + bias;
+    const float delta = !live[r] ? 0.f : a.softplus ? softplus(v) : v, u = delta * xv;
+    float2 y = both(0.f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (live[r]) h[r][i] = __ffma2_rn(decay(both(delta), A[i]), h[r][i], __fmul2_rn(both(u), make_float2(b[2 * i], b[2 * i + 1])));
+      y = __ffma2_rn(h[r][i], make_float2(c[2 * i], c[2 * i + 1]), y);
+    }
+    if (ok && n < a.N && a.final_state) store_states(a.final_state + ((long long)n * a.D + d) * a.S, s0, a.S, h[r]);
+    float sum = y.x + y.y;
+#pragma unroll
+    for (int o = Q / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (ok && n < a.N && at % Q == 0) {
+      sum = fmaf(skip, xv, sum);
+      if (a.z.p) sum *= silu(one(z[r]));
+      st(a.y.at(0, n) + d, live[r] ? sum : 0.f);
+    }
   }
 }
-
 
 template <typename T, int Q, int CH, int V>
 void launch_scan(const Args<T>& k, int blocks, cudaStream_t s) {
@@ -262,7 +292,18 @@ void launch_scan(const Args<T>& k, int blocks, cudaStream_t s) {
 template <typename T, int Q>
 int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
   if (a.T == 1 && !a.checkpoints) {
-    scan_step<T, Q><<<ceil_div((long long)a.N * a.D * Q, 256), 256, 0, s>>>(pack<T>(a, 1));
+    const Args<T> k = pack<T>(a, 1);
+    const int dblocks = ceil_div((long long)a.D * Q, 256), e = sizeof(T);
+    // four rows a thread once there are more threads than the GPU holds (bf16 N=128 D=2048 S=16: 16.4 us
+    // with one, 12.3 with four)
+    const bool many = (long long)a.N * a.D * Q > 2048LL * sm_count();
+    const bool fours = a.S % 4 == 0 && aligned(a.B, e, 4 * e) && aligned(a.C, e, 4 * e) && a.B_g % 4 == 0 && a.C_g % 4 == 0;
+    const long long blocks = (long long)dblocks * (many ? ceil_div(a.N, 4) : a.N);
+    HB_REQUIRE(blocks < (1LL << 31), "N*D too large");
+    if (many && fours) scan_step<T, Q, 4, true><<<(int)blocks, 256, 0, s>>>(k, dblocks);
+    else if (many) scan_step<T, Q, 4, false><<<(int)blocks, 256, 0, s>>>(k, dblocks);
+    else if (fours) scan_step<T, Q, 1, true><<<(int)blocks, 256, 0, s>>>(k, dblocks);
+    else scan_step<T, Q, 1, false><<<(int)blocks, 256, 0, s>>>(k, dblocks);
   } else {
     constexpr int TT = fwd_steps(Q), V1 = Tile<Q, 1, TT>::V, V2 = Tile<Q, 2, TT>::V;
     constexpr int CB = THREADS / Q;

@@ -120,13 +120,30 @@ struct Conv {
 
 void* stream() { return (void*)c10::cuda::getCurrentCUDAStream().stream(); }
 
-// A buffer of the caller's for an output, or a new one.
-Tensor buffer(const OptTensor& out, const char* name, const Tensor& like, at::IntArrayRef sizes, at::ScalarType t) {
+// Whether the memory between two tensors' first and last elements overlaps.
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return false;
+  auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return static_cast<char*>(a.data_ptr()) < end(b) && static_cast<char*>(b.data_ptr()) < end(a);
+}
+
+// The caller's buffer for the new state, or a new one.  It may be the old state's, which every thread reads
+// before it writes; it must not lie over anything else that the call reads.
+Tensor state_buffer(const OptTensor& out, const Tensor& like, const Tensor& state, at::ArrayRef<Tensor> read,
+                    at::IntArrayRef sizes, at::ScalarType t) {
   if (!out) return at::empty(sizes, like.options().dtype(t));
-  if (out->sizes() != sizes) refuse(std::string(name) + " has the wrong shape: " + shape_of(*out));
-  type(*out, name, t);
+  if (out->sizes() != sizes) refuse("out_state has the wrong shape: " + shape_of(*out));
+  type(*out, "out_state", t);
   devices(like, {*out});
-  if (!out->is_contiguous()) refuse(std::string(name) + " must be contiguous");
+  if (!out->is_contiguous()) refuse("out_state must be contiguous");
+  bool over = overlap(*out, state) && out->data_ptr() != state.data_ptr();
+  for (const Tensor& r : read) over |= overlap(*out, r);
+  if (over) refuse("out_state lies over an input other than the whole state");
+  if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();  // autograd notices that it changed
   return *out;
 }
 
@@ -135,7 +152,8 @@ std::tuple<Tensor, Tensor> causal_conv1d_forward(const Tensor& x, const Tensor& 
                                                  const OptTensor& out_state) {
   Conv c(x, weight, bias, state, lengths, silu);
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = output(c.x), last = buffer(out_state, "out_state", x, {c.a.N, c.a.W - 1, c.a.D}, x.scalar_type());
+  Tensor y = output(c.x);
+  Tensor last = state_buffer(out_state, x, c.state, {c.x, c.weight, c.bias}, {c.a.N, c.a.W - 1, c.a.D}, x.scalar_type());
   c.a.y = view(y);
   c.a.final_state = ptr(last);
   CALL(causal_conv1d_forward, &c.a, stream());
@@ -148,7 +166,7 @@ std::tuple<Tensor, Tensor> causal_conv1d_step(const Tensor& x, const Tensor& wei
   Conv c(x, weight, bias, state, {}, silu, true);
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor y = at::empty({c.a.N, c.a.D}, x.options());
-  Tensor last = buffer(out_state, "out_state", x, {c.a.N, c.a.W - 1, c.a.D}, x.scalar_type());
+  Tensor last = state_buffer(out_state, x, c.state, {c.x, c.weight, c.bias}, {c.a.N, c.a.W - 1, c.a.D}, x.scalar_type());
   c.a.y = view(y, true);
   c.a.final_state = ptr(last);
   CALL(causal_conv1d_forward, &c.a, stream());
@@ -241,7 +259,9 @@ std::tuple<Tensor, Tensor, OptTensor> selective_scan_forward(
     bool checkpoints, const OptTensor& out_state) {
   Scan c(x, dt, A, B, C, skip, z, dt_bias, state, lengths, softplus);
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = output(c.x), last = buffer(out_state, "out_state", x, {c.a.N, c.a.D, c.a.S}, at::kFloat), saved, scratch;
+  Tensor y = output(c.x), saved, scratch;
+  Tensor last = state_buffer(out_state, x, c.state, {c.x, c.dt, c.A, c.B, c.C, c.skip, c.z, c.dt_bias}, {c.a.N, c.a.D, c.a.S},
+                             at::kFloat);
   c.a.y = view(y);
   c.a.final_state = data<float>(last);
   if (checkpoints) {
@@ -264,7 +284,8 @@ std::tuple<Tensor, Tensor> selective_scan_step(const Tensor& x, const Tensor& dt
   Scan c(x, dt, A, B, C, skip, z, dt_bias, state, {}, softplus, true);
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor y = at::empty({c.a.N, c.a.D}, x.options());
-  Tensor last = buffer(out_state, "out_state", x, {c.a.N, c.a.D, c.a.S}, at::kFloat);
+  Tensor last = state_buffer(out_state, x, c.state, {c.x, c.dt, c.A, c.B, c.C, c.skip, c.z, c.dt_bias}, {c.a.N, c.a.D, c.a.S},
+                             at::kFloat);
   c.a.y = view(y, true);
   c.a.final_state = data<float>(last);
   CALL(selective_scan_forward, &c.a, stream());

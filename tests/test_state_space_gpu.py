@@ -557,3 +557,54 @@ def test_library_errors_keep_their_type():
     from haste_b200 import _C
     with pytest.raises(_C.HasteError, match="dtype"):
         _C.call("haste_b200_causal_conv1d_forward", b"\x07" * 512, None)
+
+
+# ------------------------------------------------------------------ buffers of the caller's, large scratch
+def test_out_state_is_checked_and_counted():
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(6)
+    w = torch.randn(8, 4, generator=g, device="cuda")
+    pool = torch.randn(4, 3, 8, generator=g, device="cuda")
+    x = torch.randn(2, 8, generator=g, device="cuda")
+    with pytest.raises(ValueError, match="lies over"):  # one row further than the state
+        ssm.causal_conv1d_step(x, pool[:2], w, out_state=pool[1:3])
+    with pytest.raises(ValueError, match="contiguous"):
+        ssm.causal_conv1d_step(x, pool[:2], w, out_state=torch.empty(3, 2, 8, device="cuda").transpose(0, 1))
+    with pytest.raises(ValueError, match="wrong shape"):
+        ssm.causal_conv1d_step(x, pool[:2], w, out_state=pool)
+    y0, s0 = ssm.causal_conv1d_step(x, pool[:2], w)
+    y1, s1 = ssm.causal_conv1d_step(x, pool[:2], w, out_state=pool[2:])  # another part of the pool
+    assert torch.equal(y0, y1) and torch.equal(s0, pool[2:]) and s1.data_ptr() == pool[2:].data_ptr()
+    y, _ = ssm.causal_conv1d(x[None], w.requires_grad_(), initial_state=pool[:2])
+    with torch.no_grad():
+        ssm.causal_conv1d_step(x, pool[:2], w, out_state=pool[:2])
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        s = pool[:2].clone()
+        ssm.causal_conv1d_step(x, s, w, out_state=s)
+    h = torch.randn(2, 8, 4, generator=g, device="cuda")
+    A = -torch.rand(8, 4, generator=g, device="cuda")
+    with pytest.raises(ValueError, match="lies over"):
+        ssm.selective_scan_step(x, x, A, h[:, 0], h[:, 1], h, out_state=h)
+
+
+def test_many_states_take_the_rows_in_turn():
+    """dB and dC of 128 states: more than a GB of partial sums for the whole batch."""
+    from haste_b200 import ssm
+    T, N, D, S = 1900, 26, 256, 128
+    g = torch.Generator(device="cuda").manual_seed(12)
+    d = scan_inputs(g, T, N, D, S, 1, BF16, dict(z=False))
+    leaves(d, ["B", "C", "A", "dt"])
+    dy = seq(g, T, N, D, BF16)
+    got = torch.autograd.grad(ssm.selective_scan(**d)[0], [d["B"], d["C"], d["dt"], d["A"]], dy)
+    total = 0.0
+    for rows in (slice(0, 3), slice(3, 20), slice(20, 26)):
+        part = {k: v[:, rows].detach().requires_grad_() if k in ("B", "C", "dt") else v.detach().requires_grad_(k == "A") if k == "A"
+                else v[:, rows] if v.dim() > 2 else v for k, v in d.items()}
+        want = torch.autograd.grad(ssm.selective_scan(**part)[0], [part["B"], part["C"], part["dt"], part["A"]], dy[:, rows])
+        for x, y in zip(got[:3], want[:3]):
+            # pieces differ with the batch: both within their roundings of bf16's half step, twice 2^-9
+            assert (x[:, rows].float() - y.float()).abs().max() <= 2 ** -8 * y.float().abs().max()
+        total = total + want[3]
+    assert (got[3] - total).abs().max() <= 1e-4 * total.abs().max()
