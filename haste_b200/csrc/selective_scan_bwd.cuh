@@ -6,7 +6,11 @@
 //   ddelta_t = x_t (lam_t . B_t) + lam_t . (A a_t h_{t-1}),   dA = sum_t lam_t delta_t a_t h_{t-1}
 //
 // The forward pass left the state in front of every CKPT steps; a thread computes those steps' states
-// and decays again, keeps them in registers, and walks back over them.
+// and decays again, H at a time, keeps them in registers, and walks back over them.  bf16 T=1000 N=64 D=1024
+// S=16: 1470 us.  A step of eight channels takes 102 instructions (28 of them pairs of products and sums) and
+// about 35 turns of shared memory against 15 clocks of exponentials; with 168 registers twelve warps are
+// resident, which issue every second clock.  Tried, us: one channel a thread 1735; H = 2 with sixteen
+// warps 1596; B and C as 16-bit values in shared memory 1504; pairs stored twice there 1680.
 #pragma once
 
 #include <algorithm>
