@@ -83,6 +83,10 @@ def lib():
         L.haste_b200_last_error.restype = ctypes.c_char_p
         L.haste_b200_version.restype = ctypes.c_char_p
         L.haste_b200_launch_count.restype = _ll
+        for op in ("causal_conv1d_scratch", "selective_scan_checkpoints", "selective_scan_scratch", "fused_norm_scratch"):
+            fn = getattr(L, f"haste_b200_{op}")
+            fn.argtypes = [_p, _i] if op == "selective_scan_scratch" else [_p]
+            fn.restype = _ll
         _lib = L
     return _lib
 

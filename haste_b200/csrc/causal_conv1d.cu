@@ -302,6 +302,7 @@ int check(const haste_b200_causal_conv1d& a, bool backward) {
   HB_REQUIRE(a.weight, "null pointer");
   HB_REQUIRE(a.T == 0 || (a.x.data && (backward ? a.dy.data != nullptr : a.y.data != nullptr)), "null pointer");
   HB_REQUIRE(!backward || (a.dweight && a.scratch), "null pointer");
+  HB_REQUIRE(!backward || aligned(a.scratch, 16), "scratch must be aligned to 16 bytes");
   return HASTE_B200_OK;
 }
 

@@ -7,7 +7,7 @@
 //
 // The forward pass left the state in front of every CKPT steps; a thread computes those steps' states
 // and decays again, H at a time, keeps them in registers, and walks back over them.  bf16 T=1000 N=64 D=1024
-// S=16: 1470 us.  A step of eight channels takes 102 instructions (28 of them pairs of products and sums) and
+// S=16: 1436 us.  A step of eight channels takes 102 instructions (28 of them pairs of products and sums) and
 // about 35 turns of shared memory against 15 clocks of exponentials; with 168 registers twelve warps are
 // resident, which issue every second clock.  Tried, us: one channel a thread 1735; H = 2 with sixteen
 // warps 1596; B and C as 16-bit values in shared memory 1504; pairs stored twice there 1680.
@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
           }
         }
       }
+      float2 lastB[2], lastC[2];
 #pragma unroll
       for (int k = H - 1; k >= 0; --k) {
         float2 b[2], g[2], dB[2], dC[2];
@@ -303,8 +304,15 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
           pp[k * PK + j * CB] = lb.x + lb.y;
           pp[PW + k * PK + j * CB] = da.x + da.y;
         }
-        add_channels(pred + k * 2 * SP, dB, dC);
+        // the step before's, whose shuffles then run beside this one's arithmetic
+        if (k < H - 1) add_channels(pred + (k + 1) * 2 * SP, lastB, lastC);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          lastB[i] = dB[i];
+          lastC[i] = dC[i];
+        }
       }
+      add_channels(pred, lastB, lastC);
     }
 #pragma unroll
     for (int j = 0; j < CH; ++j) {

@@ -313,7 +313,7 @@ int haste_b200_layer_norm_indrnn_backward(
  * data[t * t_stride + n * n_stride + j] (strides in elements, j unit-strided), so halves of a
  * projection and batch-first tensors are taken as they lie.  Outputs must not overlap inputs,
  * except where said.  dtype is the storage of all sequences (HASTE_B200_F32, BF16 or F16),
- * arithmetic and sums are fp32.  `lengths` [N] (device, 64-bit) ends each row early: from step
+ * arithmetic and sums are fp32.  Steps lie less than 2^31 elements apart, T is at most 2^30.  `lengths` [N] (device, 64-bit) ends each row early: from step
  * lengths[n] on (values are clamped to 0..T) inputs are not read, outputs are zero, and the final
  * state is the one after lengths[n] steps.
  * These entry points allocate nothing and keep no state: scratch comes from the caller, so calls
@@ -328,7 +328,8 @@ typedef struct {
  *   x, y [T,N,D]  weight [D,W]  bias [D]  state, final_state [N,W-1,D] dense, dtype
  *   final_state may be the same buffer as state.
  * backward: dy, dx [T,N,D], dfinal_state, dstate [N,W-1,D], dweight, dbias like their parameters;
- * dx, dstate and dbias may be NULL.  scratch: haste_b200_causal_conv1d_scratch() floats. */
+ * dx, dstate and dbias may be NULL.  scratch: haste_b200_causal_conv1d_scratch() floats, aligned to
+ * 16 bytes. */
 typedef struct {
   int dtype, param_dtype; /* param_dtype: of weight, bias and their gradients; F32 or dtype */
   int T, N, D, W, silu;
@@ -372,7 +373,8 @@ typedef struct {
 int haste_b200_selective_scan_forward(const haste_b200_selective_scan* args, void* stream);
 int haste_b200_selective_scan_backward(const haste_b200_selective_scan* args, void* stream);
 long long haste_b200_selective_scan_checkpoints(const haste_b200_selective_scan* args);
-/* floats of scratch that the forward (backward != 0: backward) call needs */
+/* Floats of scratch that the forward (backward != 0: backward) call needs.  The forward call does without
+ * if `scratch` is NULL, at a cost in time where there are few channels. */
 long long haste_b200_selective_scan_scratch(const haste_b200_selective_scan* args, int backward);
 
 /* u = x * silu(gate);  r = residual + scale * u;  y = norm(r) * weight + bias
@@ -380,7 +382,7 @@ long long haste_b200_selective_scan_scratch(const haste_b200_selective_scan* arg
  *   x, gate, y [T,N,H] dtype   residual, r [T,N,H] residual_dtype (F32 or dtype; without a residual
  *   pass dtype)   scale, weight, bias [H] param_dtype (F32 or dtype); scale needs a residual
  *   stats [T,N,2] float: mean (0 without layer_norm) and 1 / deviation; NULL if there will be no
- *   backward pass.  r may be NULL, or the same buffer as residual.  H is 1..8192.
+ *   backward pass; aligned to 8 bytes.  r may be NULL, or the same buffer as residual.  H is 1..8192.
  * backward: reads dy and dr (may be NULL: no gradient of r); writes dx, dgate, dresidual, dscale,
  * dweight, dbias like their tensors.  Any of dx, dgate, dresidual may be NULL.
  * scratch: haste_b200_fused_norm_scratch() floats. */
