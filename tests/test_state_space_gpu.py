@@ -608,3 +608,15 @@ def test_many_states_take_the_rows_in_turn():
             assert (x[:, rows].float() - y.float()).abs().max() <= 2 ** -8 * y.float().abs().max()
         total = total + want[3]
     assert (got[3] - total).abs().max() <= 1e-4 * total.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("T,N,H,opt", [
+    (37, 5, 100, dict(gate=True, residual=True, scale=True, bias=True)), (9, 3, 128, dict(residual=True, scale=True)),
+    (50, 7, 33, dict(gate=True, batch_first=True)), (1, 17, 63, dict(bias=True)), (600, 40, 64, dict(residual=True, scale=True)),
+    (4, 9, 129, dict(gate=True)), (3, 5, 2, dict(residual=True, wide=True)),
+])
+def test_fused_norm_of_short_rows(T, N, H, opt, kind, dtype):
+    """Rows that share a warp, and blocks whose last rows do not exist."""
+    test_fused_norm(T, N, H, opt, kind, dtype)
