@@ -314,7 +314,8 @@ int launch(const haste_b200_selective_scan& a, cudaStream_t s) {
     const bool two = rows * ceil_div(a.D / a.G, 2 * CB) >= 4LL * sm_count() && wide(a, V2, false);
     Args<T> k = pack<T>(a, two ? 2 * CB : CB);
     const long long blocks = rows * k.ctiles;
-    k.chunks = two || !a.scratch ? 1 : forward_pieces(a);
+    // (every piece reads the initial state, so a final state in its place takes whole sequences)
+    k.chunks = two || !a.scratch || (a.state && a.final_state == a.state) ? 1 : forward_pieces(a);
     if (k.chunks > 1) {
       k.chunk = ceil_div(ceil_div(a.T, k.chunks), TT) * TT;
       k.ends = a.scratch;

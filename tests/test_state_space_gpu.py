@@ -620,3 +620,27 @@ def test_many_states_take_the_rows_in_turn():
 def test_fused_norm_of_short_rows(T, N, H, opt, kind, dtype):
     """Rows that share a warp, and blocks whose last rows do not exist."""
     test_fused_norm(T, N, H, opt, kind, dtype)
+
+
+# ------------------------------------------------------------------ rows that end early, pieces, states in place
+def test_a_long_prompt_may_leave_its_state_in_place():
+    """Through the native call: pieces all start from the initial state, so it must outlive them."""
+    from haste_b200 import _C
+    g = torch.Generator(device="cuda").manual_seed(14)
+    T, N, D, S = 900, 1, 64, 16
+    d = scan_inputs(g, T, N, D, S, 1, F32, dict(state=True))
+    h = d["initial_state"]
+    args = [d["x"], d["dt"], d["A"], d["B"], d["C"], d["D"], d["z"], d["dt_bias"]]
+    want, major, K = ref.scan(*args, h)
+    for _ in range(5):
+        state = h.clone()
+        y, last, _ = _C.native().selective_scan_forward(*args, state, None, True, False, state)
+        assert last.data_ptr() == state.data_ptr()
+        ref.check(y, want["y"], major["y"], K, "y")
+        ref.check(state, want["final"], major["final"], K, "state")
+    x = torch.randn(900, 2, 8, generator=g, device="cuda")
+    w = torch.randn(8, 4, generator=g, device="cuda")
+    s = torch.randn(2, 3, 8, generator=g, device="cuda")
+    y0, last = _C.native().causal_conv1d_forward(x, w, None, s, None, True, None)
+    y1, _ = _C.native().causal_conv1d_forward(x, w, None, s, None, True, s)
+    assert torch.equal(y0, y1) and torch.equal(s, last)
