@@ -296,8 +296,8 @@ int check(const haste_b200_causal_conv1d& a, bool backward) {
   HB_REQUIRE(a.T >= 0 && a.T <= (1 << 30) && a.N >= 0 && a.D >= 0, "T,N,D");
   HB_REQUIRE(a.W >= 2 && a.W <= 4, "W must be 2, 3 or 4");
   HB_REQUIRE((long long)a.D * (a.W + 1) < (1LL << 31), "D");
-  HB_REQUIRE(strides_fit(a.T, a.x) && strides_fit(a.T, a.y) && strides_fit(a.T, a.dy) && strides_fit(a.T, a.dx),
-             "a step's stride must be below 2^31 elements");
+  for (const haste_b200_sequence* q : {&a.x, &a.y, &a.dy, &a.dx})
+    HB_REQUIRE(strides_fit(a.T, *q), "a step's stride must be below 2^31 elements");
   if (a.N == 0 || a.D == 0) return HASTE_B200_OK;
   HB_REQUIRE(a.weight, "null pointer");
   HB_REQUIRE(a.T == 0 || (a.x.data && (backward ? a.dy.data != nullptr : a.y.data != nullptr)), "null pointer");

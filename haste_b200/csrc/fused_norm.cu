@@ -24,8 +24,8 @@ int check(const haste_b200_fused_norm& a, bool backward) {
   HB_REQUIRE((long long)a.T * a.N < (1LL << 31) - 65536, "T*N too large");
   HB_REQUIRE(a.H >= 1 && a.H <= 8192, "H must be 1..8192");
   HB_REQUIRE(a.eps >= 0.f, "eps");
-  HB_REQUIRE(strides_fit(a.T, a.x) && strides_fit(a.T, a.gate) && strides_fit(a.T, a.residual) && strides_fit(a.T, a.y) && strides_fit(a.T, a.r) && strides_fit(a.T, a.dy) && strides_fit(a.T, a.dr) && strides_fit(a.T, a.dx) && strides_fit(a.T, a.dgate) && strides_fit(a.T, a.dresidual),
-             "a step's stride must be below 2^31 elements");
+  for (const haste_b200_sequence* q : {&a.x, &a.gate, &a.residual, &a.y, &a.r, &a.dy, &a.dr, &a.dx, &a.dgate, &a.dresidual})
+    HB_REQUIRE(strides_fit(a.T, *q), "a step's stride must be below 2^31 elements");
   HB_REQUIRE(!a.scale || a.residual.data || a.T == 0 || a.N == 0, "scale needs a residual");
   HB_REQUIRE(a.weight, "null pointer");
   HB_REQUIRE(aligned(a.stats, 8), "stats must be aligned to 8 bytes");

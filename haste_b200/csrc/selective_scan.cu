@@ -20,8 +20,8 @@ int check(const haste_b200_selective_scan& a, bool backward) {
   HB_REQUIRE(a.G >= 1 && a.D % a.G == 0, "G must divide D");
   HB_REQUIRE((long long)a.D * (a.S + 2) < (1LL << 31) && (long long)a.N * a.D < (1LL << 31), "N*D too large");
   HB_REQUIRE((long long)a.N * a.D * a.S < (1LL << 37), "N*D*S too large");
-  HB_REQUIRE(strides_fit(a.T, a.x) && strides_fit(a.T, a.dt) && strides_fit(a.T, a.z) && strides_fit(a.T, a.y) && strides_fit(a.T, a.B) && strides_fit(a.T, a.C) && strides_fit(a.T, a.dy) && strides_fit(a.T, a.dx) && strides_fit(a.T, a.ddt) && strides_fit(a.T, a.dz) && strides_fit(a.T, a.dB) && strides_fit(a.T, a.dC),
-             "a step's stride must be below 2^31 elements");
+  for (const haste_b200_sequence* q : {&a.x, &a.dt, &a.z, &a.y, &a.B, &a.C, &a.dy, &a.dx, &a.ddt, &a.dz, &a.dB, &a.dC})
+    HB_REQUIRE(strides_fit(a.T, *q), "a step's stride must be below 2^31 elements");
   if (a.N == 0 || a.D == 0) return HASTE_B200_OK;
   HB_REQUIRE(a.A, "null pointer");
   if (backward) HB_REQUIRE(a.dA && a.scratch, "null pointer");

@@ -92,7 +92,18 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
     }
   }
 
-  const int tiles = (at.last - at.first + TT - 1) / TT;
+  // Behind the row's end the carry stays and all gradients are zero: whole tiles of that are written at once.
+  const int tiles = (max(at.first, min(at.last, len)) - at.first + TT - 1) / TT;
+  for (int t = at.first + tiles * TT + ts; t < at.last; t += min(ROWS, TT)) {
+    if (!has) break;
+    const float none[V] = {};
+    store<T, V>(a.dx.at(t, n) + d, none);
+    store<T, V>(a.ddt.at(t, n) + d, none);
+    if (Gate) store<T, V>(a.dz.at(t, n) + d, none);
+  }
+  for (int t = at.first + tiles * TT; t < at.last; ++t)
+    for (int e = tid; e < 2 * SP; e += THREADS)
+      a.part[((((long long)at.ct * a.T_ + t) * a.rows + n - a.n0) * a.G + at.g) * (2 * SP) + e] = 0.f;
   Raw<T, V> xn[SL], dn[SL], zn[SL], gn[SL];
   Raw<T, 1> bn[PB], cn[PB];
   const int bt = tid / SP, bs = tid % SP;
@@ -426,7 +437,7 @@ __global__ void __launch_bounds__(THREADS) scan_bwd_ends(Args<T> a) {
   if (mine) load_states(a.A + (long long)(at.d0 + c) * a.S, s0, a.S, A);
 #pragma unroll
   for (int i = 0; i < 2; ++i) A[i] = __fmul2_rn(A[i], both(LOG2E));
-  const int tiles = (at.last - at.first + TT - 1) / TT;
+  const int tiles = (max(at.first, min(at.last, len)) - at.first + TT - 1) / TT;
   Raw<T, V> dn[SL], gn[SL], zn[SL];
   Raw<T, 1> cn[PB];
   const int bt = tid / SP, bs = tid % SP;
@@ -445,7 +456,7 @@ __global__ void __launch_bounds__(THREADS) scan_bwd_ends(Args<T> a) {
       cn[i] = load_if<T, 1>(k < TT && t0 + k < len && bs < a.S, a.C.at(t0 + k, n) + at.g * a.C_g + bs);
     }
   };
-  fetch(at.first + (tiles - 1) * TT);
+  if (tiles > 0) fetch(at.first + (tiles - 1) * TT);
 #pragma unroll 1
   for (int tile = tiles - 1; tile >= 0; --tile) {
     const int t0 = at.first + tile * TT;

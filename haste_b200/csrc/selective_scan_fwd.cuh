@@ -104,7 +104,9 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
   };
   fetch();
   T* py = Ends ? nullptr : a.y.at(at.first + ts, n) + ds;
-  for (int t0 = at.first; t0 < at.last; t0 += TT) {
+  // (behind the row's end the state stays and y is zero)
+  const int stop = len <= at.first ? at.first : min(at.last, at.first + (len - at.first + TT - 1) / TT * TT);
+  for (int t0 = at.first; t0 < stop; t0 += TT) {
     Raw<T, V> x[SL], z[SL];
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
         if (!Ends) Cs[i * BR + bt][bs] = one(cn[i]);
       }
     __syncthreads();
-    if (t0 + TT < at.last) fetch();
+    if (t0 + TT < stop) fetch();
 #pragma unroll 1
     for (int k0 = 0; k0 < TT; k0 += CKPT) {
       if (!Ends && a.checkpoints && t0 + k0 < at.last)
@@ -197,6 +199,15 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
           for (int v = 0; v < V; ++v) y[v] = 0.f;
         store<T, V>(py + (long long)(i * ROWS) * a.y.t, y);
       }
+      py += (long long)TT * a.y.t;
+    }
+  }
+  if constexpr (!Ends) {
+    for (int t0 = stop; t0 < at.last; t0 += TT) {
+      const float none[V] = {};
+#pragma unroll
+      for (int i = 0; i < SL; ++i)
+        if (has && t0 + ts + i * ROWS < at.last) store<T, V>(py + (long long)(i * ROWS) * a.y.t, none);
       py += (long long)TT * a.y.t;
     }
   }

@@ -623,6 +623,43 @@ def test_fused_norm_of_short_rows(T, N, H, opt, kind, dtype):
 
 
 # ------------------------------------------------------------------ rows that end early, pieces, states in place
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,N,D,S,G,opt", [
+    (300, 3, 24, 16, 1, dict(lengths=torch.int64, state=True)), (260, 5, 10, 5, 1, dict(lengths=torch.int64, batch_first=True)),
+    (530, 2, 33, 32, 1, dict(lengths=torch.int32, state=True, z=False)), (400, 4, 6, 100, 2, dict(lengths=torch.int64, state=True)),
+    (333, 2, 250, 3, 1, dict(state=True)),
+])
+def test_selective_scan_in_pieces(T, N, D, S, G, opt, dtype):
+    """Few channels, long sequences: pieces, some of them behind the rows' ends."""
+    test_selective_scan(T, N, D, S, G, opt, dtype)
+
+
+@pytest.mark.parametrize("T", [24, 200, 5000])
+def test_steps_behind_the_end_leave_the_state_alone(T):
+    """However many there are.  A row without steps keeps its bits: a piece of no steps multiplies by
+    exp(0) and adds zero.  A row with steps keeps them only while one piece holds the whole sequence: joined
+    pieces take exp(A (d1 + d2 + ..)) h + e, rounded elsewhere than the product of the steps' decays."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(13)
+    N, D, S = 3, 20, 16
+    d = scan_inputs(g, 5000, N, D, S, 1, F32, dict(state=True))
+    short = {k: v[:16] if v.dim() > 2 and v.shape[0] == 5000 else v for k, v in d.items()}
+    cut = {k: v[:T] if v.dim() > 2 and v.shape[0] == 5000 else v for k, v in d.items()}
+    lengths = torch.tensor([11, 0, 16], device="cuda")
+    want = ssm.selective_scan(**short, lengths=lengths)
+    y, final = ssm.selective_scan(**cut, lengths=lengths)
+    assert torch.equal(final[1], d["initial_state"][1])
+    exact, major, K = ref.scan(*[short[k] for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "initial_state")], lengths)
+    ref.check(final, exact["final"], major["final"], K, "final_state")
+    assert T > 24 or torch.equal(final, want[1])
+    assert torch.equal(y[:16], want[0]) and not y[16:].any()
+    h = d["initial_state"].clone().requires_grad_()
+    df = torch.randn(N, D, S, generator=g, device="cuda")
+    cut["initial_state"] = h
+    dh, = torch.autograd.grad(ssm.selective_scan(**cut, lengths=torch.zeros(N, dtype=torch.long, device="cuda"))[1], h, df)
+    assert torch.equal(dh, df)
+
+
 def test_a_long_prompt_may_leave_its_state_in_place():
     """Through the native call: pieces all start from the initial state, so it must outlive them."""
     from haste_b200 import _C
