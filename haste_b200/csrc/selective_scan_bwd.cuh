@@ -7,7 +7,7 @@
 //
 // The forward pass left the state in front of every CKPT steps; a thread computes those steps' states
 // and decays again, H at a time, keeps them in registers, and walks back over them.  bf16 T=1000 N=64 D=1024
-// S=16: 1436 us.  A step of eight channels takes 102 instructions (28 of them pairs of products and sums) and
+// S=16: 1400 us.  A step of eight channels takes 102 instructions (28 of them pairs of products and sums) and
 // about 35 turns of shared memory against 15 clocks of exponentials; with 168 registers twelve warps are
 // resident, which issue every second clock.  Tried, us: one channel a thread 1735; H = 2 with sixteen
 // warps 1596; B and C as 16-bit values in shared memory 1504; pairs stored twice there 1680.

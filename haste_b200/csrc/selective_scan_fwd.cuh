@@ -4,8 +4,8 @@
 //   y_t = (C_t . h_t + skip x_t) silu(z_t)
 //
 // S exponentials a (step, row, channel) on the special function units, 16 a clock and SM (measured), against
-// 8 to 16 bytes of sequences: for S = 16 those units bound it, not HBM.  bf16 T=1000 N=64 D=1024 S=16: 381 us
-// (415 with checkpoints); the units' floor, with softplus and SiLU, is 290 us, and they are busy 65 % of the
+// 8 to 16 bytes of sequences: for S = 16 those units bound it, not HBM.  bf16 T=1000 N=64 D=1024 S=16: 377 us
+// (413 with checkpoints); the units' floor, with softplus and SiLU, is 290 us, and they are busy 65 % of the
 // time, shared memory 63 %, the issue slots 56 % at 33 instructions per step of eight channels.
 #pragma once
 

@@ -1,4 +1,4 @@
-// What the state space operators (causal_conv1d.cu, selective_scan*.cu, fused_norm.cu) share.
+// What the state space operators (causal_conv1d.cu, selective_scan*.cu, fused_norm*) share.
 #pragma once
 
 #include <cstring>
