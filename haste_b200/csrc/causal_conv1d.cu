@@ -96,8 +96,11 @@ __device__ __forceinline__ void convolve(const float2 (&w)[W][P], const float2 (
   }
 }
 
+// (Five resident blocks, which the launch counts on.  Left alone, four channels of 16 bits and four taps take
+// 128 registers, and four blocks fit: bf16 1000 x 64 x 1024 72 us, with five 65; 400 x 64 x 1024 36 and 32.
+// Forced elsewhere it costs: fp32 300 x 64 x 1024 34 and 36, three taps 11 and 13.  0: no wish.)
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(128) conv_fwd(ConvArgs<T> a) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 && V == 4 && W == 4 ? 5 : 0) conv_fwd(ConvArgs<T> a) {
   constexpr int G = GROUP<T, V>, P = (V + 1) / 2;
   const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
   const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
