@@ -329,11 +329,16 @@ struct Shape {
     const int lanes = ceil_div(a.D, v);
     threads = std::min(128, ceil_div(lanes, 32) * 32);
     dtiles = ceil_div(lanes, threads);
-    // One wave: as many chunks as the resident blocks (five an SM; three in the backward pass, whose
-    // windows and sums take 150 registers), of 16 steps at least.  A chunk reads W - 1 steps twice.
+    // One wave: as many chunks as the resident blocks, of 16 steps at least.  A chunk reads W - 1 steps twice.
     // fp32 T=400 N=64 D=1024, us forward / backward: chunks of 64 steps, 1.2 / 2 waves, 47 / 69; one wave 39 / 63.
-    // (Blocks of 256 or 512 threads: 52 / 95, 54 / 200.)
-    const int per = std::max(1, (backward ? 3 : 5) * sm_count() / dtiles);
+    // (Blocks of 256 or 512 threads: 52 / 95, 54 / 200.)  How many blocks of 128 threads an SM holds follows from
+    // the registers; with five and three for every variant, against these (us forward / backward): bf16, two taps,
+    // 128 x 128 x 2048 34 / 70 and 34 / 56; bf16, three taps, 1000 x 64 x 1024 70 / 107 and 60 / 103; fp32, single
+    // channels, three taps, 400 x 40 x 1001 47 / 95 and 36 / 75.
+    const bool half = dtype_size(a.dtype) == 2;
+    const int resident = backward ? (v < 4 ? (!half && v == 2 && a.W == 4 ? 4 : 5) : a.W == 2 || (half && a.W == 3) ? 4 : 3)
+                                  : (v < 4 ? (half ? 5 : 9) : half && a.W < 4 ? 4 : 5);
+    const int per = std::max(1, resident * sm_count() / dtiles);
     chunks = std::max(1, std::min(per / a.N, ceil_div(a.T, 16)));
     chunk = std::max(4, ceil_div(ceil_div(a.T, chunks), 4) * 4);
     chunks = std::max(1, ceil_div(a.T, chunk));
