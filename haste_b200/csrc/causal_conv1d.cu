@@ -7,7 +7,7 @@
 // the last W - 1 inputs in registers; the next group of steps is loaded while one is computed, and two
 // channels go to an instruction.  fp32 T=400 N=64 D=1024: forward 39 us, 5.3 TB/s (0.82 of the measured
 // copy), backward 63 us, 5.0 TB/s with its sums.  16-bit sequences move half the bytes for the same
-// instructions, which then share the bound: bf16 T=4000 N=8 D=2048 64 us, 4.1 TB/s (60 without SiLU).
+// instructions, which then share the bound: bf16 T=4000 N=8 D=2048 56 us, 4.7 TB/s (48 without SiLU).
 #include <algorithm>
 
 #include "state_space.cuh"
