@@ -213,7 +213,10 @@ struct BwdShape {
     const int per = a.D / a.G, CB = THREADS / Q;
     const long long lines = (long long)a.N * a.G;
     // two channels a thread while their blocks fill the GPU (bf16 T=1000 N=64 D=1024 S=16: 1735 us with one, 1617 with two)
-    CH = lines * ceil_div(per, 2 * CB) >= 3LL * sm_count() ? 2 : 1;
+    // (One lane a channel takes one: two would be 256 channels a block, more than its threads stage one by one, and
+    // spill; bf16 T=400 N=64 D=2048 S=4 667 us with two, 470 with one; fp32 300 x 16 x 8192 709 and 428.  A rule on
+    // sizes alone: the scratch may be asked for before the pointers, whose alignment decides on wider staging, are there.)
+    CH = Q > 1 && lines * ceil_div(per, 2 * CB) >= 3LL * sm_count() ? 2 : 1;
     ctiles = ceil_div(per, CB * CH);
     blocks = lines * ctiles;
     chunks = 1;

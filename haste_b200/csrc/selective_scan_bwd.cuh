@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
   using F = Tile<Q, CH, CKPT>;
   constexpr int TT = CKPT, CB = F::CB, CT = F::CT, SP = F::SP, YC = F::YC, BR = F::BR, PB = F::PB, WARPS = THREADS / 32;
   constexpr int SL = F::PER / V, ROWS = THREADS * V / CT;
+  static_assert(ROWS >= 1 && SL * ROWS >= TT, "the threads stage every channel of every step");
   constexpr int LANES = 32 / Q;  // channels of a warp
   constexpr int H = 4;  // steps whose states and decays a thread holds; of 8, all would not fit the registers
   extern __shared__ __align__(16) char memory[];
@@ -418,6 +419,7 @@ __global__ void __launch_bounds__(THREADS) scan_bwd_ends(Args<T> a) {
   using F = Tile<Q, 1, TT>;
   constexpr int CB = F::CB, SP = F::SP, BR = F::BR, PB = F::PB;
   constexpr int SL = F::PER / V, ROWS = THREADS * V / CB;
+  static_assert(ROWS >= 1 && SL * ROWS >= TT, "the threads stage every channel of every step");
   __shared__ __align__(16) float2 in[TT][CB];  // delta, dy
   __shared__ __align__(16) float Cs[TT][SP];
   Place at(a, CB);
@@ -553,12 +555,12 @@ int launch_rows(const haste_b200_selective_scan& a, const Args<T>& k, const BwdS
     count_launch(1);
   }
   constexpr int V1 = Tile<Q, 1, CKPT>::V, V2 = Tile<Q, 2, CKPT>::V;
-  if (sh.CH == 2) {
-    if (wide(a, V2, true)) HB_TRY((by_gate<T, Q, 2, V2>(k, s)));
-    else HB_TRY((by_gate<T, Q, 2, 1>(k, s)));
-  } else {
+  if (sh.CH == 1) {
     if (wide(a, V1, true)) HB_TRY((by_gate<T, Q, 1, V1>(k, s)));
     else HB_TRY((by_gate<T, Q, 1, 1>(k, s)));
+  } else if constexpr (Q > 1) {
+    if (wide(a, V2, true)) HB_TRY((by_gate<T, Q, 2, V2>(k, s)));
+    else HB_TRY((by_gate<T, Q, 2, 1>(k, s)));
   }
   const long long rows = (long long)a.T * k.rows * a.G;
   if (rows) {

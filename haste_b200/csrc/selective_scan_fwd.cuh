@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
   using F = Tile<Q, CH, TT>;
   constexpr int CB = F::CB, CT = F::CT, SP = F::SP, YC = F::YC, BR = F::BR, PB = F::PB;
   constexpr int SL = F::PER / V, ROWS = THREADS * V / CT;  // slots of V channels, steps between them
+  static_assert(ROWS >= 1 && SL * ROWS >= TT, "the threads stage every channel of every step");
   __shared__ __align__(16) float2 dd[TT][CT];              // delta, delta x
   __shared__ __align__(16) float Bs[TT][SP], Cs[Ends ? 1 : TT][SP];
   __shared__ __align__(16) float ys[Ends ? 1 : TT][Q][YC];
