@@ -210,6 +210,9 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       input_at<T, V, W>(a, t0 - (W - 1) + k, len, n, d, row);
+      if (len == 0)  // (the state of a row without steps meets no tap, and may be no number)
+#pragma unroll
+        for (int i = 0; i < V; ++i) row[i] = 0.f;
       pairs<V>(row, xs[k + 1]);
     }
     for (int t = t0; t < end; t += G) {
@@ -241,6 +244,11 @@ __global__ void __launch_bounds__(128) conv_bwd(ConvArgs<T> a) {
           if (t + u >= len)  // (the incoming gradient counts for nothing, whatever p is)
 #pragma unroll
             for (int i = 0; i < P; ++i) g[i] = both(0.f);
+        } else if (t + u >= len) {  // (an infinite last input meets no step behind it; with SiLU its own step's g is no number)
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+#pragma unroll
+            for (int i = 0; i < P; ++i) xs[k][i] = both(0.f);
         }
 #pragma unroll
         for (int i = 0; i < P; ++i) {

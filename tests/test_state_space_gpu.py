@@ -681,3 +681,46 @@ def test_a_long_prompt_may_leave_its_state_in_place():
     y0, last = _C.native().causal_conv1d_forward(x, w, None, s, None, True, None)
     y1, _ = _C.native().causal_conv1d_forward(x, w, None, s, None, True, s)
     assert torch.equal(y0, y1) and torch.equal(s, last)
+
+
+# ------------------------------------------------------------------ values that are not numbers, overflow
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,D,W", [(5, 7, 4), (40, 64, 3), (33, 20, 2)])
+def test_a_row_without_steps_adds_nothing_to_the_taps_gradients(T, D, W, dtype):
+    """Its state goes through to the final state, whatever it holds, and takes part in nothing else."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(15)
+    N = 3
+    lengths = torch.tensor([T, 0, T // 2], device="cuda")
+    x = poison(seq(g, T, N, D, dtype), lengths)
+    state = torch.randn(N, W - 1, D, generator=g, device="cuda").to(dtype)
+    state[1] = float("nan")
+    state[1, 0, ::2] = float("inf")
+    w, b = torch.randn(D, W, generator=g, device="cuda").to(dtype), torch.randn(D, generator=g, device="cuda").to(dtype)
+    d = dict(x=x, weight=w, bias=b, initial_state=state)
+    names = leaves(d, list(d))
+    dy = seq(g, T, N, D, dtype)
+    y, final = ssm.causal_conv1d(**d, lengths=lengths)
+    got = dict(zip(names, torch.autograd.grad(y, [d[k] for k in names], dy)))
+    want, major, K = ref.conv(x, w, b, state, lengths, True, dy)
+    ref.check(y, want["y"], major["y"], K, "y")
+    assert torch.equal(final[1].isnan(), state[1].isnan()) and torch.equal(final[1].isinf(), state[1].isinf())
+    for k, name in (("x", "dx"), ("weight", "dweight"), ("bias", "dbias"), ("initial_state", "dstate")):
+        ref.check(got[k], want[name], major[name], K, name)
+
+
+def test_the_last_input_meets_no_step_behind_it():
+    """Without SiLU an infinite last input reaches the gradient of the last tap alone."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(16)
+    T, N, D, W = 12, 2, 8, 4
+    lengths = torch.tensor([T, 6], device="cuda")
+    x, w, dy = seq(g, T, N, D, F32), torch.randn(D, W, generator=g, device="cuda").requires_grad_(), seq(g, T, N, D, F32)
+    x[5, 1, 3] = float("inf")
+    got, = torch.autograd.grad(ssm.causal_conv1d(x, w, lengths=lengths, silu=False)[0], w, dy)
+    want, major, K = ref.conv(x, w, None, None, lengths, False, dy)
+    assert got[3, 3].isinf()
+    got[3, 3] = 0.0
+    for r in (want, major):
+        r["dweight"][3, 3] = 0.0
+    ref.check(got, want["dweight"], major["dweight"], K, "dweight")
