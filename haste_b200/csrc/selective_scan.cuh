@@ -61,6 +61,17 @@ __device__ __forceinline__ float2 decay(float2 delta, float2 A) {
   const float2 v = __ffma2_rn(delta, A, make_float2(EXP2_LOW, EXP2_LOW));
   return make_float2(exp2_fast(v.x), exp2_fast(v.y));
 }
+// exp(sum A) h + e: what stands behind a piece whose steps add up to `sum`.  Decays above one (A or delta of the
+// other sign) may have a product beyond float32 where the state that they meet is zero or small: two factors.
+__device__ __forceinline__ float behind(float sum, float A, float h, float e) {
+  const float v = fmaf(sum, A, EXP2_LOW), first = v > 127.f ? 127.f : v;  // (a NaN stays)
+  h *= exp2_fast(first);
+  if (h != 0.f) h *= exp2_fast(v - first);
+  return h + e;
+}
+__device__ __forceinline__ float2 behind(float sum, float2 A, float2 h, float2 e) {
+  return make_float2(behind(sum, A.x, h.x, e.x), behind(sum, A.y, h.y, e.y));
+}
 
 // delta = log(1 + exp(v)) = max(v, 0) + log(1 + e) and its slope, with e = exp(-|v|).  The product
 // -|v| log2(e) is taken in two parts, so that e keeps its bits for large |v|; log(1 + e) / e on [0, 1] is a

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
       reorder(e, order);
       const float sum = a.sums[p * pairs + rown + ch];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) carry[j][i] = __ffma2_rn(decay(both(sum), A2[j][i]), carry[j][i], e[i]);
+      for (int i = 0; i < 2; ++i) carry[j][i] = behind(sum, A2[j][i], carry[j][i], e[i]);
     }
   }
 

@@ -68,9 +68,9 @@ __global__ void __launch_bounds__(THREADS, CH == 2 ? 4 : 5) scan_fwd(Args<T> a) 
     for (int p = 0; p < at.piece; ++p) {
       float2 e[2];
       load_states(a.ends + p * pairs * a.S + row, s0, a.S, e);
-      const float2 sum = both(a.sums[p * pairs + rown + ch]);
+      const float sum = a.sums[p * pairs + rown + ch];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) h[j][i] = __ffma2_rn(decay(sum, A[j][i]), h[j][i], e[i]);
+      for (int i = 0; i < 2; ++i) h[j][i] = behind(sum, A[j][i], h[j][i], e[i]);
     }
   }
 

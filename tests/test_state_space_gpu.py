@@ -724,3 +724,45 @@ def test_the_last_input_meets_no_step_behind_it():
     for r in (want, major):
         r["dweight"][3, 3] = 0.0
     ref.check(got, want["dweight"], major["dweight"], K, "dweight")
+
+
+@pytest.mark.parametrize("S,gate", [(16, True), (5, False)])
+def test_pieces_with_states_that_grow(S, gate):
+    """Decays above one: over a piece their product may leave float32 although no state does.  Nothing
+    comes in before the last steps, no gradient behind the first ones: all results are finite, those
+    of the pieces in between zero."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(17)
+    T, N, D = 900, 1, 64
+    x, z, dy = (torch.randn(T, N, D, generator=g, device="cuda") for _ in range(3))
+    B, C = (torch.randn(T, N, 1, S, generator=g, device="cuda") for _ in range(2))
+    x[:-10] = 0.0
+    dy[10:] = 0.0
+    d = dict(x=x, dt=torch.rand(T, N, D, generator=g, device="cuda") * 0.1 + 0.95, B=B, C=C,
+             A=torch.rand(D, S, generator=g, device="cuda") * 0.5 + 2.0)
+    if gate:
+        d["z"] = z
+    names = leaves(d, list(d))
+    y, final = ssm.selective_scan(**d, softplus=False)
+    got = dict(zip(names, torch.autograd.grad(y, [d[k] for k in names], dy)))
+    want, major, K = ref.scan(x, d["dt"], d["A"], B, C, None, d.get("z"), softplus=False, dy=dy)
+    ref.check(y, want["y"], major["y"], K, "y")
+    ref.check(final, want["final"], major["final"], K, "final")
+    for k in names:
+        ref.check(got[k], want["d" + k], major["d" + k], K, "d" + k)
+
+
+def test_a_small_state_that_grows_through_pieces():
+    """exp(A sum of delta) of a piece beyond float32 (e^110), the state that it meets e^-60."""
+    from haste_b200 import ssm
+    T, N, D, S = 192, 1, 8, 4
+    one = torch.ones(T, N, D, device="cuda")
+    A = torch.full((D, S), 110.0 / 64, device="cuda")  # 64 steps of 1
+    h = torch.full((N, D, S), 1e-26, device="cuda")
+    dt = one.clone()
+    dt[64:] = -0.5  # and back: e^(110 - 60 - 110) in the end
+    bc = torch.ones(T, N, 1, S, device="cuda")
+    y, final = ssm.selective_scan(0 * one, dt, A, bc, bc, initial_state=h, softplus=False)
+    want, major, K = ref.scan(0 * one, dt, A, bc, bc, state=h, softplus=False)
+    ref.check(y, want["y"], major["y"], K, "y")
+    ref.check(final, want["final"], major["final"], K, "final")
