@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) s += m.red[w][k][i];
+      if (t0 + k >= len) s = 0.f;  // (the state that stays may be no number)
       a.part[((((long long)at.ct * a.T_ + t0 + k) * a.rows + n - a.n0) * a.G + at.g) * (2 * SP) + i] = s;
     }
     float skip[V], ds[V], db[V];
@@ -352,6 +353,13 @@ __global__ void __launch_bounds__(THREADS, CH == 1 ? 4 : 3) scan_bwd(Args<T> a) 
     for (int i = 0; i < SL; ++i) {
       const int k = ts + i * ROWS;
       if (!has || t0 + k >= at.last) continue;
+      if (t0 + k >= len) {
+        const float none[V] = {};
+        store<T, V>(a.dx.at(t0 + k, n) + d, none);
+        store<T, V>(a.ddt.at(t0 + k, n) + d, none);
+        if (Gate) store<T, V>(a.dz.at(t0 + k, n) + d, none);
+        continue;
+      }
       float g[V], xv[V], lb[V], da[V], dx[V], ddt[V];
       load<float, V>(&m.dy[k][cs], g);
       unpack<T, V>(x[i], xv);

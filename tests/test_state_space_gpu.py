@@ -766,3 +766,28 @@ def test_a_small_state_that_grows_through_pieces():
     want, major, K = ref.scan(0 * one, dt, A, bc, bc, state=h, softplus=False)
     ref.check(y, want["y"], major["y"], K, "y")
     ref.check(final, want["final"], major["final"], K, "final")
+
+
+@pytest.mark.parametrize("D", [6, 40])
+@pytest.mark.parametrize("gate", [True, False])
+def test_gradients_behind_the_end_are_zero_whatever_the_state(gate, D):
+    """A state that overflowed at the last step: the gradients behind it stay zero, and no other channel
+    notices.  (The channel's own dA takes 0 times that state from the steps behind, as the formula does.)"""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(18)
+    T, N, S = 24, 2, 16
+    d = scan_inputs(g, T, N, D, S, 1, F32, dict(z=gate))
+    lengths = torch.tensor([13, T], device="cuda")
+    d["x"][12, 0, 1] = float("inf")
+    names = leaves(d, list(d))
+    dy = seq(g, T, N, D, F32)
+    y, final = ssm.selective_scan(**d, lengths=lengths)
+    assert final[0, 1].isinf().any() and not y[13:, 0].any()
+    got = dict(zip(names, torch.autograd.grad(y, [d[k] for k in names], dy)))
+    for k in ("x", "dt", "B", "C") + (("z",) if gate else ()):
+        assert not got[k][13:, 0].any(), k
+    d["x"].detach()[12, 0, 1] = 0.0
+    rest = [n for n in range(D) if n != 1]
+    want, major, K = ref.scan(d["x"], d["dt"], d["A"], d["B"], d["C"], d["D"], d.get("z"), d["dt_bias"], None, lengths, dy=dy)
+    ref.check(got["A"][rest], want["dA"][rest], major["dA"][rest], K, "dA")
+    ref.check(got["x"][..., rest], want["dx"][..., rest], major["dx"][..., rest], K, "dx")
