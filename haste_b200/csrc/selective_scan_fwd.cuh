@@ -297,8 +297,9 @@ __global__ void __launch_bounds__(256) scan_step(Args<T> a, int dblocks) {
 
 template <typename T, int Q, int CH, int V>
 void launch_scan(const Args<T>& k, int blocks, cudaStream_t s) {
-  // (the last piece's end is nobody's start)
-  if (k.chunks > 1) scan_fwd<T, Q, CH, V, false, true><<<blocks * (k.chunks - 1), THREADS, 0, s>>>(k);
+  // (the last piece's end is nobody's start; two channels a thread take whole sequences)
+  if constexpr (CH == 1)
+    if (k.chunks > 1) scan_fwd<T, Q, CH, V, false, true><<<blocks * (k.chunks - 1), THREADS, 0, s>>>(k);
   if (k.z.p) scan_fwd<T, Q, CH, V, true, false><<<blocks * k.chunks, THREADS, 0, s>>>(k);
   else scan_fwd<T, Q, CH, V, false, false><<<blocks * k.chunks, THREADS, 0, s>>>(k);
 }
