@@ -17,8 +17,9 @@ namespace {
 
 using namespace ss;
 
-// Steps of one group: 64 bytes of a thread's channels.  The next group is under way while one is computed.
-template <typename T, int V>
+// Steps of one group in the forward pass: 64 bytes where a thread has four channels.  The next group is under way
+// while one is computed.
+template <typename T>
 constexpr int GROUP = sizeof(T) == 4 ? 4 : 8;
 
 template <typename T>
@@ -101,7 +102,7 @@ __device__ __forceinline__ void convolve(const float2 (&w)[W][P], const float2 (
 // Forced elsewhere it costs: fp32 300 x 64 x 1024 34 and 36, three taps 11 and 13.  0: no wish.)
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128, sizeof(T) == 2 && V == 4 && W == 4 ? 5 : 0) conv_fwd(ConvArgs<T> a) {
-  constexpr int G = GROUP<T, V>, P = (V + 1) / 2;
+  constexpr int G = GROUP<T>, P = (V + 1) / 2;
   const int d = ((blockIdx.x % a.dtiles) * blockDim.x + threadIdx.x) * V;
   const int item = blockIdx.x / a.dtiles, n = item % a.N, c = item / a.N;
   if (d >= a.D) return;
@@ -337,7 +338,7 @@ struct Shape {
     const int lanes = ceil_div(a.D, v);
     threads = std::min(128, ceil_div(lanes, 32) * 32);
     dtiles = ceil_div(lanes, threads);
-    // One wave: as many chunks as the resident blocks, of 16 steps at least.  A chunk reads W - 1 steps twice.
+    // One wave: as many chunks as the resident blocks, of about 16 steps at least.  A chunk reads W - 1 steps twice.
     // fp32 T=400 N=64 D=1024, us forward / backward: chunks of 64 steps, 1.2 / 2 waves, 47 / 69; one wave 39 / 63.
     // (Blocks of 256 or 512 threads: 52 / 95, 54 / 200.)  How many blocks of 128 threads an SM holds follows from
     // the registers; with five and three for every variant, against these (us forward / backward): bf16, two taps,

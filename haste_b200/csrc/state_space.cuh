@@ -143,7 +143,9 @@ __device__ __forceinline__ int row_length(const long long* lengths, int n, int T
 }
 
 // sigmoid(v) = 1 / (1 + 2^(-v log2 e)), two approximate instructions (2^-22 relative and one unit in the last
-// place); an overflowing exponential gives zero.  silu(v) = v s and its slope from s = sigmoid(v).
+// place).  The product -v log2 e is rounded once, which puts the exponential, and for negative v the result, off by
+// up to |v| 2^-24 of its value (6e-7 at -10, 3.6e-6 at -60); an overflowing exponential gives zero.
+// silu(v) = v s and its slope from s = sigmoid(v).
 __device__ __forceinline__ float reciprocal(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
