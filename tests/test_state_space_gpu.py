@@ -791,3 +791,15 @@ def test_gradients_behind_the_end_are_zero_whatever_the_state(gate, D):
     want, major, K = ref.scan(d["x"], d["dt"], d["A"], d["B"], d["C"], d["D"], d.get("z"), d["dt_bias"], None, lengths, dy=dy)
     ref.check(got["A"][rest], want["dA"][rest], major["dA"][rest], K, "dA")
     ref.check(got["x"][..., rest], want["dx"][..., rest], major["dx"][..., rest], K, "dx")
+
+
+def test_traced_calls_follow_their_input():
+    """The tracer records the call itself: another input gives that input's results and gradients."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    for call, x in _calls(g):
+        traced = torch.jit.trace(call, x, check_trace=False)
+        other = torch.randn(x.shape, generator=g, device="cuda").requires_grad_()
+        got, want = traced(other), call(other)
+        assert torch.equal(got, want) and not torch.equal(got, call(x))
+        for a, b in zip(torch.autograd.grad(got.sum(), other), torch.autograd.grad(want.sum(), other)):
+            assert torch.equal(a, b)
