@@ -107,7 +107,7 @@ def causal_conv1d(x, weight, bias=None, initial_state=None, lengths=None, silu=T
     """Depthwise causal convolution along time: y_t = act(bias + sum_k weight[:,k] x_{t-(W-1)+k}).
 
     x [T,N,D], weight [D,W] with 2 to 4 taps, bias [D]; `initial_state` [N,W-1,D] holds the inputs
-    before the first (zeros without it).  weight and bias have x's type or float32.
+    before the first (zeros without it).  weight and bias have one type, x's or float32.
     Returns (y, final_state): the last W-1 inputs of each row."""
     if lengths is not None:
         lengths = _lengths(lengths, x)
@@ -138,7 +138,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     y_t = (C_t . h_t + D x_t) silu(z_t), per channel with S states.
 
     x, dt, z [T,N,D], A [D,S] (S up to 128), B, C [T,N,S] or, with G groups of D / G channels,
-    [T,N,G,S]; D, dt_bias [D]; `initial_state` [N,D,S] float32 (zeros without it).  Without
+    [T,N,G,S]; D, dt_bias [D]; x, dt, z, B, C have one type, A, D, dt_bias any (they are taken as float32);
+    `initial_state` [N,D,S] float32 (zeros without it).  Without
     `softplus`, delta = dt + dt_bias.  Returns (y, final_state)."""
     if lengths is not None:
         lengths = _lengths(lengths, x)
@@ -169,8 +170,8 @@ def fused_norm(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1
 
     x, gate, residual [T,N,H] (H up to 8192), the others [H]; each of gate, residual, scale (with a
     residual only) and bias may be absent.  `kind` "rms" divides by the root mean square, "layer" subtracts the mean
-    first.  The residual, and r with it, may be float32 beside narrower x; parameters have x's type
-    or float32.  Returns (y, r), r None without a residual; r is normalised before it is rounded."""
+    first.  The residual, and r with it, may be float32 beside narrower x; the parameters have one
+    type, x's or float32.  Returns (y, r), r None without a residual; r is normalised before it is rounded."""
     if kind not in ("rms", "layer"):
         raise ValueError(f"haste_b200: kind must be 'rms' or 'layer', got {kind!r}")
     layer = kind == "layer"
