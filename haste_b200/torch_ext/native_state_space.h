@@ -52,9 +52,6 @@ void devices(const Tensor& x, at::ArrayRef<Tensor> ts) {
 Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
 OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-// The kernels take any strides but along the last axis.
-Tensor unit_strided(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-
 // [T,N,...], or one step of it, [N,...].
 haste_b200_sequence view(const Tensor& t, bool step = false) {
   if (!t.defined() || !t.numel()) return {nullptr, 0, 0};
@@ -69,6 +66,11 @@ Tensor output(const Tensor& like, std::vector<int64_t> sizes, at::TensorOptions 
   return at::empty(sizes, o);
 }
 Tensor output(const Tensor& like) { return output(like, like.sizes().vec(), like.options()); }
+// The kernels take any strides but along the last axis.  A copy lies like the original, and so do outputs.
+Tensor unit_strided(const Tensor& t) {
+  if (!t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1) return t;
+  return t.dim() < 3 ? t.contiguous() : output(t).copy_(t);
+}
 template <typename T>
 T* data(const Tensor& t) { return t.defined() && t.numel() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 Tensor floats(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kFloat)); }

@@ -803,3 +803,20 @@ def test_traced_calls_follow_their_input():
         assert torch.equal(got, want) and not torch.equal(got, call(x))
         for a, b in zip(torch.autograd.grad(got.sum(), other), torch.autograd.grad(want.sum(), other)):
             assert torch.equal(a, b)
+
+
+def test_outputs_lie_like_batch_first_inputs_of_any_stride():
+    """Batch-first, every second channel: the copy that the kernels read is batch-first too."""
+    from haste_b200 import ssm
+    g = torch.Generator(device="cuda").manual_seed(20)
+    T, N, D, S = 6, 3, 8, 4
+    x = seq(g, T, N, D, F32, batch_first=True, step=2).requires_grad_()
+    w, weight = torch.randn(D, 3, generator=g, device="cuda"), torch.randn(D, generator=g, device="cuda")
+    A, bc = -torch.rand(D, S, generator=g, device="cuda"), seq(g, T, N, 2 * S, F32, batch_first=True, step=2)
+    dense = x.detach().contiguous().requires_grad_()
+    for call in (lambda v: ssm.causal_conv1d(v, w)[0], lambda v: ssm.fused_norm(v, weight, residual=v)[0],
+                 lambda v: ssm.selective_scan(v, v, A, bc[..., :S], bc[..., S:])[0]):
+        y, want = call(x), call(dense)
+        assert torch.equal(y, want) and y.transpose(0, 1).is_contiguous() and want.is_contiguous()
+        for a, b in zip(torch.autograd.grad(y.square().sum(), x), torch.autograd.grad(want.square().sum(), dense)):
+            assert torch.equal(a, b)
