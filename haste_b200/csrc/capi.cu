@@ -18,6 +18,10 @@ long long selective_scan_scratch(const haste_b200_selective_scan& a, bool backwa
 int fused_norm_forward(const haste_b200_fused_norm& a, cudaStream_t s);
 int fused_norm_backward(const haste_b200_fused_norm& a, cudaStream_t s);
 long long fused_norm_scratch(const haste_b200_fused_norm& a);
+int gated_scan_forward(const haste_b200_gated_scan& a, cudaStream_t s);
+int gated_scan_backward(const haste_b200_gated_scan& a, cudaStream_t s);
+long long gated_scan_checkpoints(const haste_b200_gated_scan& a);
+long long gated_scan_scratch(const haste_b200_gated_scan& a, bool backward);
 
 const char* last_error();
 long long launch_count();
@@ -354,6 +358,7 @@ int haste_b200_layer_norm_indrnn_backward(
 HB_STATE_SPACE(causal_conv1d)
 HB_STATE_SPACE(selective_scan)
 HB_STATE_SPACE(fused_norm)
+HB_STATE_SPACE(gated_scan)
 #undef HB_STATE_SPACE
 
 long long haste_b200_causal_conv1d_scratch(const haste_b200_causal_conv1d* args) {
@@ -367,6 +372,13 @@ long long haste_b200_selective_scan_scratch(const haste_b200_selective_scan* arg
 }
 long long haste_b200_fused_norm_scratch(const haste_b200_fused_norm* args) {
   return args ? fused_norm_scratch(*args) : 0;
+}
+
+long long haste_b200_gated_scan_checkpoints(const haste_b200_gated_scan* args) {
+  return args ? gated_scan_checkpoints(*args) : 0;
+}
+long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int backward) {
+  return args ? gated_scan_scratch(*args, backward != 0) : 0;
 }
 
 int haste_b200_gemm(int dtype, int M, int N, int K, const void* a, long long a_rs, long long a_cs,

@@ -575,6 +575,17 @@ def fused_norm_backward(x, weight, bias, gate, residual, scale, eps, layer_norm,
     return _C.native().fused_norm_backward(x, weight, bias, gate, residual, scale, eps, layer_norm, statistics, dy, dr)
 
 
+def gated_scan_forward(x, gate, decay=None, input_gate=None, state=None, lengths=None, training=False):
+    """[y, final_state, checkpoints]: x, gate, input_gate [T,N,D], decay [D], state [N,D]; `checkpoints`
+    (None unless training) is for the backward pass."""
+    return list(_C.native().gated_scan_forward(x, gate, decay, input_gate, state, lengths, training))
+
+
+def gated_scan_backward(x, gate, decay, input_gate, state, lengths, checkpoints, dy, dfinal_state=None):
+    """[dx, dgate, ddecay, dinput_gate, dstate]; None where the tensor is."""
+    return _C.native().gated_scan_backward(x, gate, decay, input_gate, state, lengths, checkpoints, dy, dfinal_state)
+
+
 # ---------------------------------------------------------------- helpers for tests/bench
 def gemm(a, b, out=None, accumulate=False):
     """out (+)= a @ b for 2-D CUDA tensors with arbitrary strides (views allowed)."""

@@ -1,10 +1,11 @@
-"""Operators of a selective state space block, with gradients, and for single tokens.
+"""Operators of state space and gated linear recurrence blocks, with gradients, and for single tokens.
 
     x = ssm.causal_conv1d(x, w, b)[0]              # short causal convolution and SiLU
     y, h = ssm.selective_scan(x, dt, A, B, C, D=D, z=z, dt_bias=dt_bias)
+    y, h = ssm.gated_scan(x, gate, decay=decay, input_gate=i)     # one state a channel, gates as inputs
     y = ssm.fused_norm(y, weight, gate=z)[0]       # norm behind a block, or in front of one
 
-and `causal_conv1d_step` / `selective_scan_step` where tokens come one at a time.  The state that a
+and `causal_conv1d_step` / `selective_scan_step` / `gated_scan_step` where tokens come one at a time.  The state that a
 call returns is what the next one takes, so a prompt may be cut anywhere and followed by steps.
 
 Sequences are [T,N,...] in float32, bfloat16 or float16; a batch-first tensor goes in as a transposed
@@ -20,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _C, ops
 
-__all__ = ["causal_conv1d", "causal_conv1d_step", "selective_scan", "selective_scan_step", "fused_norm"]
+__all__ = ["causal_conv1d", "causal_conv1d_step", "selective_scan", "selective_scan_step", "gated_scan", "gated_scan_step", "fused_norm"]
 
 
 _tracing_state = torch._C._get_tracing_state
@@ -84,6 +85,22 @@ class _SelectiveScan(torch.autograd.Function):
         *inputs, lengths, saved = ctx.saved_tensors
         dy = torch.zeros_like(inputs[0]) if dy is None else dy
         return (None, None, *_pick(ctx, 2, ops.selective_scan_backward(*inputs, lengths, ctx.softplus, saved, dy, dlast)))
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lengths, x, gate, decay, input_gate, state):
+        y, last, saved = ops.gated_scan_forward(x, gate, decay, input_gate, state, lengths, True)
+        ctx.save_for_backward(x, gate, decay, input_gate, state, lengths, saved)
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        *inputs, lengths, saved = ctx.saved_tensors
+        dy = torch.zeros_like(inputs[0]) if dy is None else dy
+        return (None, *_pick(ctx, 1, ops.gated_scan_backward(*inputs, lengths, saved, dy, dlast)))
 
 
 class _FusedNorm(torch.autograd.Function):
@@ -163,6 +180,34 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, sof
                                   None if z is None else z[None], dt_bias, state, softplus=softplus)
         return y[0], state
     return _native().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, softplus, out_state)
+
+
+def gated_scan(x, gate, decay=None, input_gate=None, initial_state=None, lengths=None):
+    """r = sigmoid(gate);  with `decay`: log a = decay r, w = sqrt(1 - a^2);  without: a = r, w = 1 - a;
+    h_t = a_t h_{t-1} + w_t x_t sigmoid(input_gate_t).  Returns (h of every step, final_state).
+
+    x, gate, input_gate [T,N,D] have one type; decay [D] has any and is taken as float32, values above zero count as
+    zero; `initial_state` [N,D] float32 (zeros without it)."""
+    if lengths is not None:
+        lengths = _lengths(lengths, x)
+    decay = _float(decay)
+    if _shown():
+        return _GatedScan.apply(lengths, x, gate, decay, input_gate, initial_state)
+    return _native().gated_scan(x, gate, decay, input_gate, initial_state, lengths)
+
+
+def gated_scan_step(x, gate, state, decay=None, input_gate=None, out_state=None):
+    """One token: x, gate, input_gate [N,D], state [N,D] float32.  Returns (y [N,D], new state); the new state goes
+    into `out_state` where given, which may be `state` itself."""
+    decay = _float(decay)
+    if _shown() or _wants_grad(x, gate, state, decay, input_gate):
+        if out_state is not None:
+            raise ValueError("haste_b200: out_state is for calls without gradients")
+        if x.dim() != 2:
+            raise ValueError(f"haste_b200: x must have 2 dimensions, got {list(x.shape)}")
+        y, state = gated_scan(x[None], gate[None], decay, None if input_gate is None else input_gate[None], state)
+        return y[0], state
+    return _native().gated_scan_step(x, gate, state, decay, input_gate, out_state)
 
 
 def fused_norm(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1e-5, kind="rms"):

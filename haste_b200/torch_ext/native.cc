@@ -43,7 +43,8 @@ bool has_c(int cell) { return cell == LSTM || cell == LN_LSTM; }
   X(layer_norm_indrnn_forward) X(layer_norm_indrnn_backward) X(lstm_forward_iterate)                 \
   X(gru_forward_iterate) X(causal_conv1d_forward) X(causal_conv1d_backward) X(causal_conv1d_scratch)   \
   X(selective_scan_forward) X(selective_scan_backward) X(selective_scan_checkpoints)                 \
-  X(selective_scan_scratch) X(fused_norm_forward) X(fused_norm_backward) X(fused_norm_scratch)
+  X(selective_scan_scratch) X(fused_norm_forward) X(fused_norm_backward) X(fused_norm_scratch)       \
+  X(gated_scan_forward) X(gated_scan_backward) X(gated_scan_checkpoints) X(gated_scan_scratch)
 struct Library {
 #define HB_FIELD(f) decltype(&haste_b200_##f) f = nullptr;
   HB_FUNCTIONS(HB_FIELD)
@@ -494,6 +495,7 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> forward(
 }
 
 #include "native_state_space.h"
+#include "native_gated.h"
 
 }  // namespace
 
@@ -508,4 +510,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("load", &load);
   m.def("forward", &forward, py::call_guard<py::gil_scoped_release>());
   state_space::bind(m);
+  gated::bind(m);
 }

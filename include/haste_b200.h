@@ -400,6 +400,35 @@ int haste_b200_fused_norm_forward(const haste_b200_fused_norm* args, void* strea
 int haste_b200_fused_norm_backward(const haste_b200_fused_norm* args, void* stream);
 long long haste_b200_fused_norm_scratch(const haste_b200_fused_norm* args);
 
+/* ---- Gated linear recurrence ---------------------------------------------- */
+/* r = sigmoid(gate); with decay: log a = min(decay[d], 0) r, w = sqrt(1 - a^2), without: a = r, w = 1 - a;
+ * h_t = a_t h_{t-1} + w_t x_t sigmoid(input_gate_t),  y_t = h_t.  No counterpart in the reference; arguments,
+ * sequences, `lengths` and scratch as in the state space operators above.
+ *   x, gate, input_gate (may be absent), y [T,N,D]   decay [D] (may be NULL), state, final_state [N,D]: float,
+ *   dense; final_state may be the same buffer as state.
+ * checkpoints: what the backward pass starts its pieces from, haste_b200_gated_scan_checkpoints() floats; NULL if
+ * there will be none.
+ * backward: reads checkpoints, dy and dfinal_state; writes dx, dgate, dinput_gate (if input_gate), ddecay (if decay)
+ * and dstate (may be NULL).  scratch: haste_b200_gated_scan_scratch() floats, aligned to 8 bytes. */
+typedef struct {
+  int dtype, T, N, D;
+  haste_b200_sequence x, gate, input_gate, y;
+  const float *decay, *state;
+  float* final_state;
+  const long long* lengths;
+  float* checkpoints;
+  haste_b200_sequence dy, dx, dgate, dinput_gate;
+  const float* dfinal_state;
+  float *ddecay, *dstate;
+  float* scratch;
+} haste_b200_gated_scan;
+int haste_b200_gated_scan_forward(const haste_b200_gated_scan* args, void* stream);
+int haste_b200_gated_scan_backward(const haste_b200_gated_scan* args, void* stream);
+long long haste_b200_gated_scan_checkpoints(const haste_b200_gated_scan* args);
+/* Floats of scratch that the forward (backward != 0: backward) call needs.  The forward call does without
+ * if `scratch` is NULL, at a cost in time where there are few channels. */
+long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int backward);
+
 /* ---- Dense contraction (exposed for tests and benchmarks) --------------- */
 /* C[m,n] (+)= sum_k A(m,k) B(k,n);  A(m,k) at a[m*a_rs + k*a_cs],
  * B(k,n) at b[k*b_rs + n*b_cs], C row-major with leading dimension ldc.
