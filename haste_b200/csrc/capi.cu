@@ -22,6 +22,9 @@ int gated_scan_forward(const haste_b200_gated_scan& a, cudaStream_t s);
 int gated_scan_backward(const haste_b200_gated_scan& a, cudaStream_t s);
 long long gated_scan_checkpoints(const haste_b200_gated_scan& a);
 long long gated_scan_scratch(const haste_b200_gated_scan& a, bool backward);
+int grad_norm(const haste_b200_gradient* g, int count, float* norm, float* scratch, cudaStream_t s);
+int clip_gradients(const haste_b200_gradient* g, int count, float max_norm, float* norm, float* scratch, cudaStream_t s);
+long long grad_norm_scratch(const haste_b200_gradient* g, int count);
 
 const char* last_error();
 long long launch_count();
@@ -379,6 +382,19 @@ long long haste_b200_gated_scan_checkpoints(const haste_b200_gated_scan* args) {
 }
 long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int backward) {
   return args ? gated_scan_scratch(*args, backward != 0) : 0;
+}
+
+int haste_b200_grad_norm(const haste_b200_gradient* gradients, int count, float* norm, float* scratch, void* stream) {
+  HB_TRY(report_timeout());
+  return grad_norm(gradients, count, norm, scratch, (cudaStream_t)stream);
+}
+int haste_b200_clip_gradients(const haste_b200_gradient* gradients, int count, float max_norm, float* norm,
+                              float* scratch, void* stream) {
+  HB_TRY(report_timeout());
+  return clip_gradients(gradients, count, max_norm, norm, scratch, (cudaStream_t)stream);
+}
+long long haste_b200_grad_norm_scratch(const haste_b200_gradient* gradients, int count) {
+  return gradients && count > 0 ? grad_norm_scratch(gradients, count) : 0;
 }
 
 int haste_b200_gemm(int dtype, int M, int N, int K, const void* a, long long a_rs, long long a_cs,

@@ -27,6 +27,8 @@ parallel wrappers, which this mirrors.
 import torch
 import torch.distributed as dist
 
+from .gradients import clip_grad_norm_
+
 __all__ = ["shard", "dropconnect_mask", "broadcast_parameters", "all_reduce_tensors",
            "all_reduce_gradients", "GradientBucket", "attach", "DataParallel"]
 
@@ -231,6 +233,7 @@ class DataParallel:
             dp.zero_grad()
             y = net(shard(x, rank, world)); loss(y).backward()
             dp.finish()                         # gradients summed over the ranks, in p.grad
+            dp.clip_grad_norm_(1.0)             # where wanted: the same norm and factor on every rank
             optimiser.step()
 
     Every rank runs its slice of the batch; the parameter gradients of each layer and
@@ -245,7 +248,7 @@ class DataParallel:
     """
 
     def __init__(self, net, group=None, overlap=True, reduce=True):
-        self.group, self.overlap, self.reduce = group, overlap, reduce
+        self.net, self.group, self.overlap, self.reduce = net, group, overlap, reduce
         self.hooks, self.order = [], []
         for m in net.modules():
             if type(m).__name__ in _CELL_OF_CLASS and hasattr(m, "_dp"):
@@ -281,6 +284,11 @@ class DataParallel:
                     view = view * h.recurrent_scale
                 getattr(h.layer, name).grad = view
         self.order = []
+
+    def clip_grad_norm_(self, max_norm, error_if_nonfinite=False):
+        """Scales the gradients of all of the network's parameters so that their norm is at most `max_norm`, and
+        returns what it was (`gradients.clip_grad_norm_`).  Call after `finish`, when every rank holds the same sums."""
+        return clip_grad_norm_(self.net.parameters(), max_norm, error_if_nonfinite)
 
     def detach(self):
         for h in self.hooks:

@@ -1,6 +1,8 @@
 // Host path of the operators of a gated linear recurrence block.  Part of native.cc.
 #pragma once
 
+#include <algorithm>
+
 namespace gated {
 
 using namespace state_space;
@@ -129,12 +131,89 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ gradients
+// Tensors whose elements fill one range of memory, in any order of axes.
+haste_b200_gradient range_of(const Tensor& t, const char* name) {
+  if (t.layout() != at::kStrided) refuse(std::string(name) + " must be dense tensors, got a sparse one");
+  const int dtype = storage(t);
+  if (!t.is_non_overlapping_and_dense())
+    refuse(std::string(name) + " must fill one range of memory each, got strides over " + shape_of(t));
+  return {ptr(t), ptr(t), (long long)t.numel(), dtype, dtype};
+}
+struct Span {
+  const char *from, *to;
+  int gradient;  // number, or -1 - number of an output
+};
+// What is written must be nobody else's: each output its own gradient's memory, or its own.
+void refuse_overlaps(const std::vector<haste_b200_gradient>& g) {
+  std::vector<Span> spans;
+  spans.reserve(2 * g.size());
+  auto add = [&](const void* p, int64_t bytes, int who) {
+    if (bytes) spans.push_back({static_cast<const char*>(p), static_cast<const char*>(p) + bytes, who});
+  };
+  for (size_t i = 0; i < g.size(); ++i) {
+    add(g[i].data, g[i].numel * (g[i].dtype == HASTE_B200_F32 ? 4 : 2), (int)i);
+    if (g[i].out != g[i].data || g[i].out_dtype != g[i].dtype)
+      add(g[i].out, g[i].numel * (g[i].out_dtype == HASTE_B200_F32 ? 4 : 2), -1 - (int)i);
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  const char* written = nullptr;  // end of the last written span so far, and of the last read one
+  const char* read = nullptr;
+  for (const Span& s : spans) {
+    const bool writes = s.gradient < 0 || g[s.gradient].out == g[s.gradient].data;
+    if ((written && s.from < written) || (writes && read && s.from < read))
+      refuse("gradients overlap in memory with one another or with an output");
+    const char*& end = writes ? written : read;
+    end = std::max(end, s.to);
+  }
+}
+
+// The norm of all gradients (a float32 scalar).  With max_norm they are scaled into `out`, or where they are.
+Tensor clip_gradients(const std::vector<Tensor>& gradients, const c10::optional<double>& max_norm,
+                      const c10::optional<std::vector<Tensor>>& out) {
+  if (gradients.empty()) refuse("there must be a gradient");
+  if (max_norm && !(*max_norm >= 0)) refuse("max_norm must not be negative");
+  if (out && out->size() != gradients.size())
+    refuse("out must hold as many tensors as there are gradients: " + std::to_string(gradients.size()) + ", got " +
+           std::to_string(out->size()));
+  if (gradients.size() > INT32_MAX / 2) refuse("too many gradients");
+  std::vector<haste_b200_gradient> g;
+  g.reserve(gradients.size());
+  for (size_t i = 0; i < gradients.size(); ++i) {
+    g.push_back(range_of(gradients[i], "gradients"));
+    if (!out) continue;
+    const Tensor& o = (*out)[i];
+    if (o.sizes() != gradients[i].sizes()) refuse("out must have the gradients' shapes, got " + shape_of(o) + " for " + shape_of(gradients[i]));
+    const haste_b200_gradient to = range_of(o, "out");
+    if (o.numel() > 1 && o.strides() != gradients[i].strides()) refuse("out must lie in memory like the gradients");
+    g.back().out = const_cast<void*>(to.data);
+    g.back().out_dtype = to.dtype;
+  }
+  devices(gradients[0], gradients);
+  if (out) devices(gradients[0], *out);
+  if (max_norm) {
+    refuse_overlaps(g);
+    for (const Tensor& t : out ? *out : gradients) {
+      TORCH_CHECK(!(t.is_leaf() && t.requires_grad() && at::GradMode::is_enabled()),
+                  "haste_b200: a leaf that requires grad cannot be scaled in place");
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+  }
+  const c10::cuda::CUDAGuard guard(gradients[0].device());
+  Tensor norm = at::empty({}, gradients[0].options().dtype(at::kFloat).requires_grad(false));
+  Tensor scratch = at::empty({std::max<int64_t>(1, lib.grad_norm_scratch(g.data(), (int)g.size()))}, norm.options());
+  if (max_norm) CALL(clip_gradients, g.data(), (int)g.size(), (float)*max_norm, static_cast<float*>(norm.data_ptr()), static_cast<float*>(scratch.data_ptr()), stream());
+  else CALL(grad_norm, g.data(), (int)g.size(), static_cast<float*>(norm.data_ptr()), static_cast<float*>(scratch.data_ptr()), stream());
+  return norm;
+}
+
 void bind(py::module& m) {
   const py::call_guard<py::gil_scoped_release> free;
   m.def("gated_scan", &gated_scan, free);
   m.def("gated_scan_forward", &gated_scan_forward, free);
   m.def("gated_scan_step", &gated_scan_step, free);
   m.def("gated_scan_backward", &gated_scan_backward, free);
+  m.def("clip_gradients", &clip_gradients, free);
 }
 
 }  // namespace gated

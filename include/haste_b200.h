@@ -429,6 +429,25 @@ long long haste_b200_gated_scan_checkpoints(const haste_b200_gated_scan* args);
  * if `scratch` is NULL, at a cost in time where there are few channels. */
 long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int backward);
 
+/* ---- Gradient norm and clipping ------------------------------------------- */
+/* norm = sqrt(sum over all gradients of their squares);  out = data * min(1, max_norm / (norm + 1e-6)), with a factor
+ * of 1 where max_norm is infinite.  No counterpart in the reference.
+ * `gradients` is host memory, read before the call returns; data, out and norm (one float) are on the device.  A
+ * gradient is `numel` elements that lie next to each other; out (of out_dtype) may be data itself, and must otherwise
+ * overlap no gradient and no other out.  A norm that is not finite scales as the formula says: infinite ones to zero
+ * (and infinite values to NaN), a NaN to NaN.  scratch: haste_b200_grad_norm_scratch() floats, aligned to 8 bytes.
+ * The calls allocate nothing, keep nothing and may be captured. */
+typedef struct {
+  const void* data;
+  void* out;
+  long long numel;
+  int dtype, out_dtype;
+} haste_b200_gradient;
+int haste_b200_grad_norm(const haste_b200_gradient* gradients, int count, float* norm, float* scratch, void* stream);
+int haste_b200_clip_gradients(const haste_b200_gradient* gradients, int count, float max_norm, float* norm,
+                              float* scratch, void* stream);
+long long haste_b200_grad_norm_scratch(const haste_b200_gradient* gradients, int count);
+
 /* ---- Dense contraction (exposed for tests and benchmarks) --------------- */
 /* C[m,n] (+)= sum_k A(m,k) B(k,n);  A(m,k) at a[m*a_rs + k*a_cs],
  * B(k,n) at b[k*b_rs + n*b_cs], C row-major with leading dimension ldc.

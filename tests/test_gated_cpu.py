@@ -77,6 +77,29 @@ def test_gated_scan_step_refuses():
         ssm.gated_scan_step(z(2, 4).requires_grad_(), z(2, 4), z(2, 4), out_state=z(2, 4))
 
 
+@pytest.mark.parametrize("args,error,says", [
+    (([z(4, 4)[:, ::2]], 1.0), ValueError, "one range of memory"),
+    (([z(4, dtype=torch.float64)], 1.0), TypeError, "float32, bfloat16 and float16"),
+    (([z(4).to_sparse()], 1.0), ValueError, "sparse"),
+    (([z(4)], -1.0), ValueError, "max_norm"),
+    (([z(4)], 1.0, [z(5)]), ValueError, "shapes"),
+    (([z(4, 5)], 1.0, [z(5, 4).t()]), ValueError, "lie in memory"),
+    (([z(4)], 1.0, [z(4), z(4)]), ValueError, "as many"),
+    (([z(4)], 1.0), RuntimeError, "CUDA tensor"),
+])
+def test_clip_gradients_refuses(args, error, says):
+    from haste_b200 import gradients
+    with pytest.raises(error, match=says):
+        gradients.clip_gradients(*args)
+
+
+def test_no_gradients_have_a_norm_of_zero():
+    import haste_b200
+    from haste_b200 import gradients
+    assert gradients.grad_norm([None]).item() == 0 and gradients.clip_gradients([], 1.0).item() == 0
+    assert haste_b200.clip_grad_norm_(torch.nn.Parameter(z(3)), 1.0).item() == 0
+
+
 def test_entry_points_refuse_bad_blocks():
     """Through the C ABI: arguments are checked before anything touches a device."""
     import ctypes
