@@ -47,6 +47,8 @@ SIGNATURES = {
     "haste_b200_fused_norm_backward": [_p, _p],
     "haste_b200_gated_scan_forward": [_p, _p],
     "haste_b200_gated_scan_backward": [_p, _p],
+    "haste_b200_linear_forward": [_p, _p],
+    "haste_b200_linear_backward": [_p, _p],
     "haste_b200_grad_norm": [_p, _i, _p, _p, _p],
     "haste_b200_clip_gradients": [_p, _i, _f, _p, _p, _p],
     "haste_b200_gemm": [_i] * 4 + [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _i, _p],
@@ -64,7 +66,8 @@ OTHER_SYMBOLS = ["haste_b200_last_error", "haste_b200_version", "haste_b200_laun
                  "haste_b200_sm_budget", "haste_b200_causal_conv1d_scratch",
                  "haste_b200_selective_scan_checkpoints", "haste_b200_selective_scan_scratch",
                  "haste_b200_fused_norm_scratch",
-                 "haste_b200_gated_scan_checkpoints", "haste_b200_gated_scan_scratch", "haste_b200_grad_norm_scratch"]
+                 "haste_b200_gated_scan_checkpoints", "haste_b200_gated_scan_scratch", "haste_b200_grad_norm_scratch",
+                 "haste_b200_linear_scratch"]
 
 _lib = None
 
@@ -89,9 +92,9 @@ def lib():
         L.haste_b200_version.restype = ctypes.c_char_p
         L.haste_b200_launch_count.restype = _ll
         for op in ("causal_conv1d_scratch", "selective_scan_checkpoints", "selective_scan_scratch", "fused_norm_scratch",
-                   "gated_scan_checkpoints", "gated_scan_scratch", "grad_norm_scratch"):
+                   "gated_scan_checkpoints", "gated_scan_scratch", "grad_norm_scratch", "linear_scratch"):
             fn = getattr(L, f"haste_b200_{op}")
-            fn.argtypes = [_p, _i] if op.endswith(("scan_scratch", "grad_norm_scratch")) else [_p]
+            fn.argtypes = [_p, _i] if op.endswith(("scan_scratch", "grad_norm_scratch", "linear_scratch")) else [_p]
             fn.restype = _ll
         _lib = L
     return _lib

@@ -22,6 +22,9 @@ int gated_scan_forward(const haste_b200_gated_scan& a, cudaStream_t s);
 int gated_scan_backward(const haste_b200_gated_scan& a, cudaStream_t s);
 long long gated_scan_checkpoints(const haste_b200_gated_scan& a);
 long long gated_scan_scratch(const haste_b200_gated_scan& a, bool backward);
+int linear_forward(const haste_b200_linear& a, cudaStream_t s);
+int linear_backward(const haste_b200_linear& a, cudaStream_t s);
+long long linear_scratch(const haste_b200_linear& a, bool backward);
 int grad_norm(const haste_b200_gradient* g, int count, float* norm, float* scratch, cudaStream_t s);
 int clip_gradients(const haste_b200_gradient* g, int count, float max_norm, float* norm, float* scratch, cudaStream_t s);
 long long grad_norm_scratch(const haste_b200_gradient* g, int count);
@@ -362,6 +365,7 @@ HB_STATE_SPACE(causal_conv1d)
 HB_STATE_SPACE(selective_scan)
 HB_STATE_SPACE(fused_norm)
 HB_STATE_SPACE(gated_scan)
+HB_STATE_SPACE(linear)
 #undef HB_STATE_SPACE
 
 long long haste_b200_causal_conv1d_scratch(const haste_b200_causal_conv1d* args) {
@@ -384,6 +388,9 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
   return args ? gated_scan_scratch(*args, backward != 0) : 0;
 }
 
+long long haste_b200_linear_scratch(const haste_b200_linear* args, int backward) {
+  return args ? linear_scratch(*args, backward != 0) : 0;
+}
 int haste_b200_grad_norm(const haste_b200_gradient* gradients, int count, float* norm, float* scratch, void* stream) {
   HB_TRY(report_timeout());
   return grad_norm(gradients, count, norm, scratch, (cudaStream_t)stream);

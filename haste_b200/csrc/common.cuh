@@ -121,7 +121,15 @@ struct GemmDesc {
   // The recurrence kernels write gate gradients in this form so that they are split once.
   const void* a_pl = nullptr; long long a_pl_ld = 0, a_pl_stride = 0;
   const void* b_pl = nullptr; long long b_pl_ld = 0, b_pl_stride = 0;
+  // Projections (linear.cu): any size on the tensor cores, fp16 operands multiplied as they are, the caller's scratch
+  // (gemm_scratch() bytes), and what is done to the sums before they are stored (dtype_c: dtype, or fp32).
+  const struct Epilogue* epilogue = nullptr;
+  bool projection = false;
+  void* scratch = nullptr;
 };
+// Bytes of scratch that a projection's contraction needs.
+size_t gemm_scratch(const GemmDesc& g);
+int gemm_sm100(const GemmDesc& g, cudaStream_t stream);
 int gemm(const GemmDesc& g, cudaStream_t stream);
 int gemm_simt(const GemmDesc& g, cudaStream_t stream);
 // Whether a contraction with a_pl / b_pl reads nothing but the planes (its a / b may then be null).

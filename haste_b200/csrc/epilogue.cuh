@@ -1,0 +1,128 @@
+// What a projection does to its sums before it stores them: y = act(sum + bias) + residual, and the slopes of its
+// activations for the backward pass.
+#pragma once
+
+#include "state_space.cuh"
+
+namespace hb {
+
+// Pointers into dense or row-strided matrices [rows, outputs]; null where absent.
+struct Epilogue {
+  const void* bias;      // float or the operands' type
+  const void* residual;  // the output's type
+  long long ld_res;
+  void* pre;             // sum + bias in the operands' type, kept for the backward pass
+  long long ld_pre;
+  int bias_f32, act;
+};
+
+namespace epi {
+
+using namespace ss;
+
+// Accurate: to the last bits of float32 (its sequences); otherwise within 2e-7 of the function's own size, which is
+// nothing to 16 bits, in a third of the instructions.  Infinities come out as the formulas have them: p times zero is a NaN.
+__device__ __forceinline__ float exp2_(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// (1 - e) / (1 + e), e = exp(-2 |v|); near zero, where that cancels, the series up to v^9.
+template <bool Accurate>
+__device__ __forceinline__ float tanh_(float v) {
+  if constexpr (Accurate) return tanhf(v);
+  const float a = fabsf(v), e = exp2_(a * -2.885390081777927f);
+  const float far = copysignf((1.f - e) * reciprocal(1.f + e), v), q = v * v;
+  float p = 62.f / 2835;
+  p = fmaf(p, q, -17.f / 315);
+  p = fmaf(p, q, 2.f / 15);
+  p = fmaf(p, q, -1.f / 3);
+  return a < 0.25f ? fmaf(v * q, p, v) : far;
+}
+// The normal distribution Phi(v) and exp(-v^2 / 2).  Not accurate: the complementary error function by formula 7.1.26 of
+// Abramowitz and Stegun, off by 1.5e-7 at most.
+template <bool Accurate>
+__device__ __forceinline__ float normal(float v, float& bell) {
+  bell = exp2_(v * v * -0.7213475204444817f);
+  if constexpr (Accurate) return 0.5f * erfcf(v * -0.7071067811865476f);
+  const float t = reciprocal(fmaf(fabsf(v), 0.3275911f * 0.7071067811865476f, 1.f));
+  float p = 0.5f * 1.061405429f;
+  p = fmaf(p, t, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
+  const float tail = p * t * bell;
+  return v < 0.f ? tail : 1.f - tail;
+}
+
+template <bool Accurate>
+__device__ __forceinline__ float activate(int act, float p) {
+  switch (act) {
+    case HASTE_B200_RELU: return p < 0.f ? 0.f : p;  // (a NaN stays)
+    case HASTE_B200_SILU: return silu(p);
+    case HASTE_B200_GELU: {
+      float bell;
+      return p * normal<Accurate>(p, bell);
+    }
+    case HASTE_B200_TANH: return tanh_<Accurate>(p);
+    case HASTE_B200_SIGMOID: return sigmoid(p);
+    default: return p;
+  }
+}
+template <bool Accurate>
+__device__ __forceinline__ float slope(int act, float p) {
+  switch (act) {
+    case HASTE_B200_RELU: return p > 0.f ? 1.f : p != p ? p : 0.f;
+    case HASTE_B200_SILU: {
+      const float s = sigmoid(p);
+      return silu_slope(p, s);
+    }
+    case HASTE_B200_GELU: {
+      float bell;
+      const float n = normal<Accurate>(p, bell);
+      return fmaf(p * 0.3989422804014327f, bell, n);
+    }
+    case HASTE_B200_TANH: {
+      const float e = exp2_(fabsf(p) * -2.885390081777927f), r = reciprocal(1.f + e);
+      return 4.f * e * r * r;  // 1 - tanh^2
+    }
+    case HASTE_B200_SIGMOID: {
+      const float e = exp2_(fabsf(p) * -1.4426950408889634f), r = reciprocal(1.f + e);
+      return e * r * r;
+    }
+    default: return 1.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const Epilogue& e, int n) {
+  return e.bias_f32 ? static_cast<const float*>(e.bias)[n] : ld(static_cast<const T*>(e.bias) + n);
+}
+// Element (m, n) of y from its sum.
+template <typename T, typename TO>
+__device__ __forceinline__ void finish(const Epilogue& e, float v, int m, int n, TO* y) {
+  if (e.bias) v += bias_at<T>(e, n);
+  if (e.pre) st(static_cast<T*>(e.pre) + m * e.ld_pre + n, v);
+  v = activate<sizeof(T) == 4>(e.act, v);
+  if (e.residual) v += ld(static_cast<const TO*>(e.residual) + m * e.ld_res + n);
+  st(y, v);
+}
+// Four neighbouring elements, whose rows take accesses of four (`wide`); bias: theirs.
+template <typename T, typename TO>
+__device__ __forceinline__ void finish4(const Epilogue& e, float (&v)[4], const float (&bias)[4], int m, int n, TO* y) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] += bias[j];
+  if (e.pre) store<T, 4>(static_cast<T*>(e.pre) + m * e.ld_pre + n, v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = activate<sizeof(T) == 4>(e.act, v[j]);
+  if (e.residual) {
+    float r[4];
+    load<TO, 4>(static_cast<const TO*>(e.residual) + m * e.ld_res + n, r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += r[j];
+  }
+  store<TO, 4>(y, v);
+}
+
+}  // namespace epi
+}  // namespace hb

@@ -3,7 +3,6 @@
 
 namespace hb {
 
-int gemm_sm100(const GemmDesc& g, cudaStream_t stream);     // gemm_sm100.cu
 int gemm_simt_few(const GemmDesc& g, cudaStream_t stream);  // gemm_simt.cu
 
 // Fewer than 32 rows stay on fp32 FMAs unless they are bf16: bf16 planes are less.  Relative error

@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "cells.cuh"
+#include "epilogue.cuh"
 #include "tcgen05.cuh"
 
 namespace hb {
@@ -59,7 +60,18 @@ struct Params {
   const int* uneven;           // fp16 planes: points to whether bf16 planes have taken their place
   float* partial;              // non-null: write fp32 partial tiles [split][M][partial_ld]
   int partial_ld;              // N rounded up to whole 32-column chunks
+  int half;                    // one product of fp16 operands as they are
   int* err;
+};
+// A contraction that stores its sums as they are, or one that is a projection's, with operands of type T.
+struct Plain {
+  static constexpr bool projection = false;
+};
+template <typename T_>
+struct Projection {
+  static constexpr bool projection = true;
+  typedef T_ T;
+  Epilogue e;
 };
 
 template <int NPROD>
@@ -189,12 +201,44 @@ __device__ __forceinline__ void fill_tile(const float* v, uint8_t* buf) {
   for (int j = 0; j < 8; ++j)
     tile[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
-template <int NPROD, int MODE>
-__device__ __forceinline__ void store_chunk(const Params& p, int sp, int m0, int n0, uint8_t* buf, int ea = 0, int eb = 0) {
+// A projection's tile: bias, activation and residual on the way out.  The activation is chosen where it is used: a branch
+// that all threads take together, next to which four copies of each loop cost small contractions their instructions' fetch.
+template <typename T, typename TO>
+__device__ __forceinline__ void store_projection(const Params& p, const Epilogue& e, const float4* tile, int m0, int n0) {
+  const int rows = min(32, p.M - m0), cols = min(32, p.N - n0), lane = threadIdx.x & 31;
+  TO* dst = static_cast<TO*>(p.c) + m0 * p.ldc + n0;
+  if (p.wide && (cols & 3) == 0) {
+    const int u = lane & 7;
+    if (u * 4 >= cols) return;
+    float bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = e.bias ? epi::bias_at<T>(e, n0 + u * 4 + j) : 0.f;
+#pragma unroll 2
+    for (int r = lane >> 3; r < rows; r += 4) {
+      const float4 x = tile[r * 8 + (u ^ (r & 7))];
+      float v[4] = {x.x, x.y, x.z, x.w};
+      epi::finish4<T, TO>(e, v, bias, m0 + r, n0 + u * 4, dst + r * p.ldc + u * 4);
+    }
+  } else if (lane < cols) {
+    const float* at = reinterpret_cast<const float*>(tile) + (lane & 3);
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r)
+      epi::finish<T, TO>(e, at[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4], m0 + r, n0 + lane, dst + r * p.ldc + lane);
+  }
+}
+template <int NPROD, int MODE, typename EP>
+__device__ __forceinline__ void store_chunk(const Params& p, const EP& ep, int sp, int m0, int n0, uint8_t* buf, int ea = 0,
+                                            int eb = 0) {
   if (m0 >= p.M || n0 >= p.N) return;  // the same for the whole warp
   const float4* tile = reinterpret_cast<const float4*>(buf);
   __syncwarp();
-  if constexpr (NPROD == 1) {
+  if constexpr (EP::projection) {
+    if (p.partial)
+      store_tile<false, NEVER, float>(tile, p.partial + ((long long)sp * p.M + m0) * p.partial_ld + n0, p.partial_ld,
+                                      min(32, p.M - m0), 32, true, false, 0, 0);
+    else if (sizeof(typename EP::T) == 4 || p.c_is_bf16) store_projection<typename EP::T, typename EP::T>(p, ep.e, tile, m0, n0);
+    else store_projection<typename EP::T, float>(p, ep.e, tile, m0, n0);
+  } else if constexpr (NPROD == 1) {
     if (p.partial)  // rows of whole chunks
       store_tile<false, NEVER, float>(tile, p.partial + ((long long)sp * p.M + m0) * p.partial_ld + n0, p.partial_ld,
                                       min(32, p.M - m0), 32, true, false, 0, 0);
@@ -224,8 +268,9 @@ __device__ __forceinline__ void store_chunk(const Params& p, int sp, int m0, int
 template <int NPROD, int MODE>
 constexpr int chunk_of() { return MODE == PLAIN ? Cfg<NPROD>::CHUNK : (MODE == F16_PLANES ? 2 : 1); }
 
-template <int NPROD, int MODE = PLAIN>
-__device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p) {
+template <int NPROD, int MODE = PLAIN, typename EP = Plain>
+__device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p,
+                                          const EP& ep = EP()) {
   using C = Cfg<NPROD>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -311,7 +356,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      constexpr uint32_t type = MODE == F16_PLANES ? 0u : 1u;  // fp16 or bf16 operands
+      const uint32_t type = MODE == F16_PLANES || (NPROD == 1 && p.half) ? 0u : 1u;  // fp16 or bf16 operands
       const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) |
                              ((uint32_t)p.a_mn_major << 15) | ((uint32_t)p.b_mn_major << 16) |
                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -415,7 +460,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
             for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
             __syncwarp();  // the tile before has been read
             fill_tile(v, tile);
-            store_chunk<NPROD, MODE>(p, sp, m0, n0 + ch * 32, tile);
+            store_chunk<NPROD, MODE>(p, ep, sp, m0, n0 + ch * 32, tile);
           }
         }
         tc_fence_before();
@@ -443,7 +488,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c)
             if (c == ch) fill_tile(sum + (C::CHUNK ? c * 32 : 0), tile);
-          store_chunk<NPROD, MODE>(p, sp, m0, n0 + ch * 32, tile, ea, eb);
+          store_chunk<NPROD, MODE>(p, ep, sp, m0, n0 + ch * 32, tile, ea, eb);
         }
       }
     }
@@ -464,6 +509,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ Params p) {
   gemm_tile<NPROD>(map_a, map_b, p);
+}
+template <int NPROD, typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+projection_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ Params p, const __grid_constant__ Projection<T> ep) {
+  gemm_tile<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 // fp16 planes, or the bf16 planes that have taken their place.
 __global__ void __launch_bounds__(THREADS, 1)
@@ -496,8 +547,9 @@ constexpr int PAIR_EPI_WARPS = 8;
 // (Ten warps put three on two of the SM's four sub-partitions, 16384 registers each, so 168
 // registers per thread is the most a 320-thread CTA can have; the epilogue therefore drains the
 // accumulator 16 columns at a time.)
-template <int NPROD, int MODE = PLAIN>
-__device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p) {
+template <int NPROD, int MODE = PLAIN, typename EP = Plain>
+__device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p,
+                                          const EP& ep = EP()) {
   using C = Cfg<NPROD>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -587,7 +639,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (CTA 0 only)
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t type = MODE == F16_PLANES ? 0u : 1u;  // fp16 or bf16 operands
+      const uint32_t type = MODE == F16_PLANES || (NPROD == 1 && p.half) ? 0u : 1u;  // fp16 or bf16 operands
       const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) |
                              ((uint32_t)p.a_mn_major << 15) | ((uint32_t)p.b_mn_major << 16) |
                              ((uint32_t)(PBN >> 3) << 17) | ((uint32_t)(PBM >> 4) << 24);
@@ -686,7 +738,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
             for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
             __syncwarp();  // the tile before has been read
             fill_tile(v, tile);
-            store_chunk<NPROD, MODE>(p, sp, m0, n0 + ch * 32, tile);
+            store_chunk<NPROD, MODE>(p, ep, sp, m0, n0 + ch * 32, tile);
           }
         }
         tc_fence_before();
@@ -703,7 +755,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c)
             if (c == ch) fill_tile(sum + (C::CHUNK ? c * 32 : 0), tile);
-          store_chunk<NPROD, MODE>(p, sp, m0, n0 + ch * 32, tile, ea, eb);
+          store_chunk<NPROD, MODE>(p, ep, sp, m0, n0 + ch * 32, tile, ea, eb);
         }
       }
     }
@@ -727,6 +779,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ Params p) {
   gemm_pair<NPROD>(map_a, map_b, p);
+}
+template <int NPROD, typename T>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+projection_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ Params p, const __grid_constant__ Projection<T> ep) {
+  gemm_pair<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_tcgen05_pair_f16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -1078,6 +1136,21 @@ void launch_reduce(const float* part, int splits, int M, int N, int ld_part, voi
     splitk_reduce_kernel<TC, false><<<blocks, 256, 0, stream>>>(part, splits, stride, M, N, ld_part, (TC*)c, ldc, accumulate);
 }
 
+// The same for a projection, element by element.
+template <typename T, typename TO>
+__global__ void __launch_bounds__(256) projection_reduce_kernel(const float* __restrict__ part, int splits, int M, int N, int ld_part,
+                                                                TO* __restrict__ c, long long ldc, const Epilogue e) {
+  const long long total = (long long)M * N, stride = (long long)M * ld_part;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+    const int m = (int)(i / N), n = (int)(i - (long long)m * N);
+    const float* src = part + (long long)m * ld_part + n;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += src[k * stride];
+    epi::finish<T, TO>(e, s, m, n, c + m * ldc + n);
+  }
+}
+
 // ----------------------------------------------------------------------------
 // Host side
 // ----------------------------------------------------------------------------
@@ -1113,6 +1186,12 @@ int set_kernel_attributes() {
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<1>, attr, pair_smem<1>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<3>, attr, pair_smem<3>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<6>, attr, pair_smem<6>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<1, __nv_bfloat16>, attr, single_smem<1>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<1, __half>, attr, single_smem<1>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<6, float>, attr, single_smem<6>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<1, __nv_bfloat16>, attr, pair_smem<1>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<1, __half>, attr, pair_smem<1>()));
+  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<6, float>, attr, pair_smem<6>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_f16_kernel, attr, max(single_smem<3>(), single_smem<6>())));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_f16_kernel, attr, max(pair_smem<3>(), pair_smem<6>())));
   if (dev >= 0 && dev < kMaxDevices) g_attr_set[dev].store(true, std::memory_order_release);
@@ -1167,6 +1246,7 @@ namespace {
 const char* refusal(const GemmDesc& g) {
   if (!encode_fn()) return "cuTensorMapEncodeTiled not available";
   if (g.K <= 0) return "K == 0";
+  if (g.projection) return nullptr;  // (its operands have unit strides)
   // Small problems are launch-bound either way; keep them on the generic kernel.
   if ((long long)g.M * g.N * g.K < (1LL << 21) || g.M < 8 || g.N < 32)
     return "problem too small for the tensor-core path";
@@ -1183,35 +1263,28 @@ bool f16_planes(const GemmDesc& g) {
   return g.precise && g.dtype == HASTE_B200_F32 && g.dtype_c == HASTE_B200_F32 && !g.accumulate && g.a_cs == 1 &&
          g.b_cs == 1 && g.b_rs != 1 && g.K >= 256 && (double)g.M * g.N * g.K >= 8e9;
 }
-}  // namespace
-
-bool gemm_reads_planes(const GemmDesc& g) { return gemm_path() != HASTE_B200_GEMM_SIMT && !refusal(g); }
-
-int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
-  auto unsupported = [](const char* why) {
-    set_last_error("gemm_sm100: %s", why);
-    return HASTE_B200_ERR_UNSUPPORTED;
-  };
-  if (g.M <= 0 || g.N <= 0) return HASTE_B200_OK;
-  if (const char* why = refusal(g)) return unsupported(why);
+// How a contraction is carried out: kernel, K split, and the scratch for planes of fp32 operands and partial tiles.
+struct Cut {
+  bool f32, a_k, b_k, f16, pair, a_pre, b_pre, a_copy, b_copy, via_partial;
+  int M, N, K, sms, pairs, tiles_m, tiles_n, kb_total, splits, kb_per_split, planes, room, part_ld;
+  long long a_rows, a_cols, b_rows, b_cols, a_ld_src, b_ld_src, a_ld, b_ld;
+  size_t a_plane, b_plane, part_bytes, a_exps, b_exps, words, bytes;
+  explicit Cut(const GemmDesc& g);
+};
+Cut::Cut(const GemmDesc& g) {
   // __half storage takes the split path too: a half splits exactly into two bf16 planes
-  const bool half_src = g.dtype == HASTE_B200_F16;
-  const bool f32 = g.dtype == HASTE_B200_F32 || half_src;
-  const bool a_k = g.a_cs == 1, b_k = g.b_rs == 1;
-
-  const int M = g.M, N = g.N, K = g.K;
-  const bool f16 = f16_planes(g);
-  Operand A, B;
-  A.mn_major = !a_k;
-  B.mn_major = !b_k;
+  f32 = g.dtype == HASTE_B200_F32 || (g.dtype == HASTE_B200_F16 && !g.projection);
+  a_k = g.a_cs == 1;
+  b_k = g.b_rs == 1;
+  M = g.M; N = g.N; K = g.K;
+  f16 = f16_planes(g);
   // extents in (outer rows, inner contiguous) form
-  const long long a_rows = a_k ? M : K, a_cols = a_k ? K : M;
-  const long long b_rows = b_k ? N : K, b_cols = b_k ? K : N;
-  const long long a_ld_src = a_k ? g.a_rs : g.a_cs;
-  const long long b_ld_src = b_k ? g.b_cs : g.b_rs;
+  a_rows = a_k ? M : K; a_cols = a_k ? K : M;
+  b_rows = b_k ? N : K; b_cols = b_k ? K : N;
+  a_ld_src = a_k ? g.a_rs : g.a_cs;
+  b_ld_src = b_k ? g.b_cs : g.b_rs;
 
-  // scratch: planes for fp32 operands, partial tiles for split-K
-  const int sms = sm_count();
+  sms = sm_count();
   // CTA pairs on 256 x 256 tiles where the output is wide enough to fill them and the work is
   // worth the cluster launch and the coarser waves: 4 .. 7 us below 16 G multiply-adds, where only a
   // long K lets the pair's better rate make up for it (us, pair / single: fp32 2000 x 512 x 512 31 / 17,
@@ -1219,13 +1292,14 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
   // second, 22 / 27 for the third).
   const double macs = (double)M * N * K;
   const bool large = macs >= 16e9 || (macs >= 4e9 && K >= 1024);
-  const int pairs = (gemm_path() == HASTE_B200_GEMM_TCGEN05_SINGLE || M < 192 || N < 192 || !large)
-                        ? 0 : max_pairs();
-  const bool pair = pairs > 0;
+  pairs = (gemm_path() == HASTE_B200_GEMM_TCGEN05_SINGLE || M < 192 || N < 192 || !large)
+              ? 0 : max_pairs();
+  pair = pairs > 0;
   const int units = pair ? pairs : sms;
-  const int tiles_m = ceil_div(M, pair ? PBM : BM), tiles_n = ceil_div(N, pair ? PBN : BN);
-  const int kb_total = ceil_div(K, BK);
-  int splits = 1;
+  tiles_m = ceil_div(M, pair ? PBM : BM);
+  tiles_n = ceil_div(N, pair ? PBN : BN);
+  kb_total = ceil_div(K, BK);
+  splits = 1;
   // (With K of 8192 and more also where a second or third wave would be nearly empty: 2048 x 3072 is 96 tiles
   // for 74 pairs; us at K = 64000 one split / three 734 / 601, 2000 x 2600, K = 20000 260 / 222.)
   if (kb_total >= 8 && tiles_m * tiles_n < (kb_total >= 128 ? 4 : 1) * units) {
@@ -1234,7 +1308,7 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
     // + the traffic of the partial tiles (written once, read once by the reduction).
     const int tiles = tiles_m * tiles_n;
     const int max_splits = min(kb_total / 4, 64);
-    const double products = g.dtype == HASTE_B200_BF16 ? 1.0 : (g.precise && !f16 ? 6.0 : 3.0);
+    const double products = !f32 ? 1.0 : (g.precise && !f16 ? 6.0 : 3.0);
     // us per K block and work unit (measured: the single-CTA kernel is bound by its operand
     // loads, the pair kernel by the tensor pipe)
     const double t_kb = pair ? 0.27 * products : (products == 1.0 ? 0.27 : 0.17 * products);
@@ -1248,97 +1322,132 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
       if (t < best) { best = t; splits = sp; }
     }
   }
-  int kb_per_split = ceil_div(kb_total, splits);
+  kb_per_split = ceil_div(kb_total, splits);
   splits = ceil_div(kb_total, kb_per_split);
 
   auto planes_usable = [&](const void* p, long long ld) {
     return f32 && !g.precise && p && (ld % 8) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
   };
-  const bool a_pre = planes_usable(g.a_pl, g.a_pl_ld) && (g.a_pl_stride % 8) == 0;
-  const bool b_pre = planes_usable(g.b_pl, g.b_pl_ld) && (g.b_pl_stride % 8) == 0;
+  a_pre = planes_usable(g.a_pl, g.a_pl_ld) && (g.a_pl_stride % 8) == 0;
+  b_pre = planes_usable(g.b_pl, g.b_pl_ld) && (g.b_pl_stride % 8) == 0;
   // An operand goes through scratch if it has to be split or if TMA cannot address its rows
   // (bf16 with a row or a start that is no multiple of 16 bytes: the copy costs two passes over the
   // operand, the CUDA-core kernel that would take it as it is twenty times the contraction).
-  const bool a_copy = f32 ? !a_pre : (a_ld_src % 8) != 0 || ((uintptr_t)g.a & 15) != 0;
-  const bool b_copy = f32 ? !b_pre : (b_ld_src % 8) != 0 || ((uintptr_t)g.b & 15) != 0;
-  const long long a_ld = a_pre ? g.a_pl_ld : (a_copy ? ((a_cols + 7) & ~7LL) : a_ld_src);
-  const long long b_ld = b_pre ? g.b_pl_ld : (b_copy ? ((b_cols + 7) & ~7LL) : b_ld_src);
-  const int planes = f32 ? (g.precise && !f16 ? 3 : 2) : 1, room = f16 ? 3 : planes;
-  const size_t a_plane = a_copy ? Arena::pad((size_t)a_rows * a_ld * 2) : 0;
-  const size_t b_plane = b_copy ? Arena::pad((size_t)b_rows * b_ld * 2) : 0;
-  const int part_ld = (N + 31) & ~31;
-  const bool via_partial = splits > 1;
-  const size_t part_bytes = via_partial ? Arena::pad((size_t)splits * M * part_ld * 4) : 0;
-  const size_t a_exps = f16 ? Arena::pad((size_t)M * 4) : 0, b_exps = f16 ? Arena::pad((size_t)tiles_n * PBN) : 0;
-  const size_t words = f16 ? Arena::pad((size_t)(8 * sms + 1) * 4) : 0;
-  const size_t bytes = room * (a_plane + b_plane) + part_bytes + a_exps + b_exps + words + 1024;
+  a_copy = f32 ? !a_pre : (a_ld_src % 8) != 0 || ((uintptr_t)g.a & 15) != 0;
+  b_copy = f32 ? !b_pre : (b_ld_src % 8) != 0 || ((uintptr_t)g.b & 15) != 0;
+  a_ld = a_pre ? g.a_pl_ld : (a_copy ? ((a_cols + 7) & ~7LL) : a_ld_src);
+  b_ld = b_pre ? g.b_pl_ld : (b_copy ? ((b_cols + 7) & ~7LL) : b_ld_src);
+  planes = f32 ? (g.precise && !f16 ? 3 : 2) : 1;
+  room = f16 ? 3 : planes;
+  a_plane = a_copy ? Arena::pad((size_t)a_rows * a_ld * 2) : 0;
+  b_plane = b_copy ? Arena::pad((size_t)b_rows * b_ld * 2) : 0;
+  part_ld = (N + 31) & ~31;
+  via_partial = splits > 1;
+  part_bytes = via_partial ? Arena::pad((size_t)splits * M * part_ld * 4) : 0;
+  a_exps = f16 ? Arena::pad((size_t)M * 4) : 0;
+  b_exps = f16 ? Arena::pad((size_t)tiles_n * PBN) : 0;
+  words = f16 ? Arena::pad((size_t)(8 * sms + 1) * 4) : 0;
+  bytes = room * (a_plane + b_plane) + part_bytes + a_exps + b_exps + words + 1024;
+}
+}  // namespace
+
+size_t gemm_scratch(const GemmDesc& g) { return g.M > 0 && g.N > 0 && g.K > 0 ? Cut(g).bytes : 0; }
+
+bool gemm_reads_planes(const GemmDesc& g) { return gemm_path() != HASTE_B200_GEMM_SIMT && !refusal(g); }
+
+int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
+  auto unsupported = [](const char* why) {
+    set_last_error("gemm_sm100: %s", why);
+    return HASTE_B200_ERR_UNSUPPORTED;
+  };
+  if (g.M <= 0 || g.N <= 0) return HASTE_B200_OK;
+  if (const char* why = refusal(g)) return unsupported(why);
+  const Cut c(g);
+  const int M = c.M, N = c.N, K = c.K, splits = c.splits, planes = c.planes;
+  const bool f16 = c.f16, pair = c.pair;
+  Operand A, B;
+  A.mn_major = !c.a_k;
+  B.mn_major = !c.b_k;
   Arena ws;
-  HB_TRY(make_arena(&ws, stream, bytes, /*slot=*/1));
+  if (g.scratch) {
+    ws.base = static_cast<char*>(g.scratch);
+    ws.cap = c.bytes;
+  } else {
+    HB_TRY(make_arena(&ws, stream, c.bytes, /*slot=*/1));
+  }
   int* err = device_error_word();
   if (!err) return unsupported("error word allocation failed");
-  A.base = a_pre ? g.a_pl : g.a;
-  A.plane_stride = a_pre ? g.a_pl_stride : 0;
-  B.base = b_pre ? g.b_pl : g.b;
-  B.plane_stride = b_pre ? g.b_pl_stride : 0;
+  A.base = c.a_pre ? g.a_pl : g.a;
+  A.plane_stride = c.a_pre ? g.a_pl_stride : 0;
+  B.base = c.b_pre ? g.b_pl : g.b;
+  B.plane_stride = c.b_pre ? g.b_pl_stride : 0;
   SplitJob jobs[2];
   int n_jobs = 0;
   auto through_scratch = [&](const void* src, long long ld_src, long long rows, long long cols, size_t plane,
                              long long ld, Operand* o) {
-    __nv_bfloat16* to = ws.take<__nv_bfloat16>(room * plane / 2);
+    __nv_bfloat16* to = ws.take<__nv_bfloat16>(c.room * plane / 2);
     jobs[n_jobs++] = SplitJob{src, ld_src, (int)rows, (int)cols, to, ld, (long long)(plane / 2)};
     o->base = to;
     o->plane_stride = plane / 2;
     return to != nullptr;
   };
-  if (a_copy && !through_scratch(g.a, a_ld_src, a_rows, a_cols, a_plane, a_ld, &A)) return unsupported("scratch arena");
-  if (b_copy && !through_scratch(g.b, b_ld_src, b_rows, b_cols, b_plane, b_ld, &B)) return unsupported("scratch arena");
+  if (c.a_copy && !through_scratch(g.a, c.a_ld_src, c.a_rows, c.a_cols, c.a_plane, c.a_ld, &A)) return unsupported("scratch arena");
+  if (c.b_copy && !through_scratch(g.b, c.b_ld_src, c.b_rows, c.b_cols, c.b_plane, c.b_ld, &B)) return unsupported("scratch arena");
   int* a_exp = nullptr;
   signed char* b_exp = nullptr;
   const int* uneven = nullptr;
   if (f16) {
-    a_exp = ws.take<int>(a_exps / 4);
-    b_exp = ws.take<signed char>(b_exps);
-    int* w = ws.take<int>(words / 4);
+    a_exp = ws.take<int>(c.a_exps / 4);
+    b_exp = ws.take<signed char>(c.b_exps);
+    int* w = ws.take<int>(c.words / 4);
     if (!a_exp || !b_exp || !w) return unsupported("scratch arena");
     HB_TRY(launch_split_f16(jobs, a_exp, b_exp, w, &uneven, stream));
   } else if (n_jobs) {
-    HB_TRY(launch_split(jobs, n_jobs, g.dtype, planes, stream));
+    // (a copy of whole 16-bit words: a half goes through as a bf16 does, a NaN stays a NaN)
+    HB_TRY(launch_split(jobs, n_jobs, c.f32 ? g.dtype : HASTE_B200_BF16, planes, stream));
   }
-  A.ld = a_ld;
-  B.ld = b_ld;
+  A.ld = c.a_ld;
+  B.ld = c.b_ld;
   float* partial = nullptr;
-  if (via_partial) {
-    partial = ws.take<float>(part_bytes / 4);
+  if (c.via_partial) {
+    partial = ws.take<float>(c.part_bytes / 4);
     if (!partial) return unsupported("scratch arena");
   }
 
   Params p;
   p.M = M; p.N = N; p.K = K;
   p.a_mn_major = A.mn_major; p.b_mn_major = B.mn_major;
-  p.tiles_m = tiles_m; p.tiles_n = tiles_n; p.splits = splits;
-  p.kb_per_split = kb_per_split; p.kb_total = kb_total;
+  p.tiles_m = c.tiles_m; p.tiles_n = c.tiles_n; p.splits = splits;
+  p.kb_per_split = c.kb_per_split; p.kb_total = c.kb_total;
   p.c_is_bf16 = g.dtype_c == HASTE_B200_BF16 ? 1 : (g.dtype_c == HASTE_B200_F16 ? 2 : 0);
   p.accumulate = g.accumulate;
   p.c = g.c; p.ldc = g.ldc;
   p.wide = (g.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(g.c) & (4 * dtype_size(g.dtype_c) - 1)) == 0;
+  if (g.epilogue) {
+    const Epilogue& e = *g.epilogue;
+    const size_t in = dtype_size(g.dtype), out = dtype_size(g.dtype_c);
+    p.wide = p.wide && e.ld_res % 4 == 0 && reinterpret_cast<uintptr_t>(e.residual) % (4 * out) == 0 && e.ld_pre % 4 == 0 &&
+             reinterpret_cast<uintptr_t>(e.pre) % (4 * in) == 0;
+  }
   p.a_exp = a_exp; p.b_exp = b_exp;
   p.uneven = uneven;
   p.partial = partial;
-  p.partial_ld = part_ld;
+  p.partial_ld = c.part_ld;
+  p.half = g.dtype == HASTE_B200_F16 && !c.f32;
   p.err = err;
 
   HB_TRY(set_kernel_attributes());
   // K-major: inner = K, box 64 (k) x 128 rows.  MN-major: inner = M/N, box 64 x 64 (k).
   CUtensorMap m_a, m_b, bf_a, bf_b;
   auto maps = [&](CUtensorMap* a, CUtensorMap* b, int n) {
-    return make_map(a, A.base, a_cols, a_rows, A.ld, A.plane_stride, n, 64, A.mn_major ? 64 : BM) &&
-           make_map(b, B.base, b_cols, b_rows, B.ld, B.plane_stride, n, 64, B.mn_major ? 64 : BN);
+    return make_map(a, A.base, c.a_cols, c.a_rows, A.ld, A.plane_stride, n, 64, A.mn_major ? 64 : BM) &&
+           make_map(b, B.base, c.b_cols, c.b_rows, B.ld, B.plane_stride, n, 64, B.mn_major ? 64 : BN);
   };
   if (!maps(&m_a, &m_b, planes) || (f16 && !maps(&bf_a, &bf_b, 3)))
     return unsupported("tensor map encoding rejected the operand");
   if (pair) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * min(pairs, tiles_m * tiles_n * splits));
+    cfg.gridDim = dim3(2 * min(c.pairs, c.tiles_m * c.tiles_n * splits));
     cfg.blockDim = dim3(PAIR_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1348,7 +1457,15 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (f16) {
+    if (g.epilogue) {
+      cfg.dynamicSmemBytes = planes == 3 ? pair_smem<6>() : pair_smem<1>();
+      if (g.dtype == HASTE_B200_F32)
+        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<6, float>, m_a, m_b, p, Projection<float>{*g.epilogue}));
+      else if (g.dtype == HASTE_B200_BF16)
+        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<1, __nv_bfloat16>, m_a, m_b, p, Projection<__nv_bfloat16>{*g.epilogue}));
+      else
+        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<1, __half>, m_a, m_b, p, Projection<__half>{*g.epilogue}));
+    } else if (f16) {
       cfg.dynamicSmemBytes = max(pair_smem<3>(), pair_smem<6>());
       HB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tcgen05_pair_f16_kernel, m_a, m_b, bf_a, bf_b, p));
     } else if (planes == 3) {
@@ -1362,8 +1479,14 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
       HB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tcgen05_pair_kernel<1>, m_a, m_b, p));
     }
   } else {
-    const int grid = min(sms, tiles_m * tiles_n * splits);
-    if (f16)
+    const int grid = min(c.sms, c.tiles_m * c.tiles_n * splits);
+    if (g.epilogue && g.dtype == HASTE_B200_F32)
+      projection_kernel<6, float><<<grid, THREADS, single_smem<6>(), stream>>>(m_a, m_b, p, Projection<float>{*g.epilogue});
+    else if (g.epilogue && g.dtype == HASTE_B200_BF16)
+      projection_kernel<1, __nv_bfloat16><<<grid, THREADS, single_smem<1>(), stream>>>(m_a, m_b, p, Projection<__nv_bfloat16>{*g.epilogue});
+    else if (g.epilogue)
+      projection_kernel<1, __half><<<grid, THREADS, single_smem<1>(), stream>>>(m_a, m_b, p, Projection<__half>{*g.epilogue});
+    else if (f16)
       gemm_tcgen05_f16_kernel<<<grid, THREADS, max(single_smem<3>(), single_smem<6>()), stream>>>(m_a, m_b, bf_a, bf_b, p);
     else if (planes == 3)
       gemm_tcgen05_kernel<6><<<grid, THREADS, single_smem<6>(), stream>>>(m_a, m_b, p);
@@ -1374,11 +1497,25 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
   }
   HB_LAUNCH_OK();
   count_launch(1);
-  if (via_partial) {
+  if (c.via_partial) {
+    if (g.epilogue) {
+      const int blocks = (int)min(((long long)M * N + 255) / 256, 8LL * c.sms);
+#define HB_REDUCE(T, TO) \
+  projection_reduce_kernel<T, TO><<<blocks, 256, 0, stream>>>(partial, splits, M, N, c.part_ld, (TO*)g.c, g.ldc, *g.epilogue)
+      if (g.dtype == HASTE_B200_F32) HB_REDUCE(float, float);
+      else if (g.dtype == HASTE_B200_BF16 && g.dtype_c == HASTE_B200_BF16) HB_REDUCE(__nv_bfloat16, __nv_bfloat16);
+      else if (g.dtype == HASTE_B200_BF16) HB_REDUCE(__nv_bfloat16, float);
+      else if (g.dtype_c == HASTE_B200_F16) HB_REDUCE(__half, __half);
+      else HB_REDUCE(__half, float);
+#undef HB_REDUCE
+      HB_LAUNCH_OK();
+      count_launch(1);
+      return HASTE_B200_OK;
+    }
     auto reduce = g.dtype_c == HASTE_B200_BF16  ? launch_reduce<__nv_bfloat16>
                   : g.dtype_c == HASTE_B200_F16 ? launch_reduce<__half>
                                                 : launch_reduce<float>;
-    reduce(partial, splits, M, N, part_ld, g.c, g.ldc, g.accumulate, 16 * sms, stream);
+    reduce(partial, splits, M, N, c.part_ld, g.c, g.ldc, g.accumulate, 16 * c.sms, stream);
     HB_LAUNCH_OK();
     count_launch(1);
   }

@@ -59,6 +59,13 @@ int* g_errw = nullptr;
 
 int* device_error_word() {
   std::call_once(g_errw_once, [] {
+    // (another thread's or this one's capture of a stream does not forbid this allocation, which no stream sees)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    struct Back {
+      cudaStreamCaptureMode* mode;
+      ~Back() { cudaThreadExchangeStreamCaptureMode(mode); }
+    } back{&mode};
     void* p = nullptr;
     if (cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
       g_errw = static_cast<int*>(p);

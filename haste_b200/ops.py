@@ -586,6 +586,20 @@ def gated_scan_backward(x, gate, decay, input_gate, state, lengths, checkpoints,
     return _C.native().gated_scan_backward(x, gate, decay, input_gate, state, lengths, checkpoints, dy, dfinal_state)
 
 
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4, "sigmoid": 5}
+
+
+def fused_linear_forward(x, weight, bias=None, activation=None, residual=None, training=False):
+    """[y, sums]: x [...,C], weight [H,C], bias [H], residual [...,H]; `sums` (None unless training with an
+    activation) is for the backward pass."""
+    return list(_C.native().fused_linear_forward(x, weight, bias, ACTIVATIONS[activation], residual, training))
+
+
+def fused_linear_backward(x, weight, bias, activation, sums, dy):
+    """[dx, dweight, dbias]; the last is None where the bias is.  The residual's gradient is dy."""
+    return list(_C.native().fused_linear_backward(x, weight, bias, ACTIVATIONS[activation], sums, dy, True, True, True))
+
+
 # ---------------------------------------------------------------- helpers for tests/bench
 def gemm(a, b, out=None, accumulate=False):
     """out (+)= a @ b for 2-D CUDA tensors with arbitrary strides (views allowed)."""

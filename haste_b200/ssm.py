@@ -4,6 +4,7 @@
     y, h = ssm.selective_scan(x, dt, A, B, C, D=D, z=z, dt_bias=dt_bias)
     y, h = ssm.gated_scan(x, gate, decay=decay, input_gate=i)     # one state a channel, gates as inputs
     y = ssm.fused_norm(y, weight, gate=z)[0]       # norm behind a block, or in front of one
+    r = ssm.fused_linear(y, w, b, activation="silu", residual=r)  # projection into a block, or back
 
 and `causal_conv1d_step` / `selective_scan_step` / `gated_scan_step` where tokens come one at a time.  The state that a
 call returns is what the next one takes, so a prompt may be cut anywhere and followed by steps.
@@ -21,7 +22,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _C, ops
 
-__all__ = ["causal_conv1d", "causal_conv1d_step", "selective_scan", "selective_scan_step", "gated_scan", "gated_scan_step", "fused_norm"]
+__all__ = ["causal_conv1d", "causal_conv1d_step", "selective_scan", "selective_scan_step", "gated_scan", "gated_scan_step", "fused_norm",
+           "fused_linear"]
 
 
 _tracing_state = torch._C._get_tracing_state
@@ -118,6 +120,21 @@ class _FusedNorm(torch.autograd.Function):
         *inputs, stats = ctx.saved_tensors
         dy = torch.zeros_like(inputs[0]) if dy is None else dy
         return (None, None, *_pick(ctx, 2, ops.fused_norm_backward(*inputs, *ctx.how, stats, dy, dr)))
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, activation, x, weight, bias, residual):
+        y, sums = ops.fused_linear_forward(x, weight, bias, activation, residual, True)
+        ctx.save_for_backward(x, weight, bias, sums)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, sums = ctx.saved_tensors
+        return (None, *_pick(ctx, 1, [*ops.fused_linear_backward(x, weight, bias, ctx.activation, sums, dy), dy]))
 
 
 def causal_conv1d(x, weight, bias=None, initial_state=None, lengths=None, silu=True):
@@ -223,3 +240,17 @@ def fused_norm(x, weight, bias=None, gate=None, residual=None, scale=None, eps=1
     if _shown():
         return _FusedNorm.apply(eps, layer, x, weight, bias, gate, residual, scale)
     return _native().fused_norm(x, weight, bias, gate, residual, scale, eps, layer)
+
+
+def fused_linear(x, weight, bias=None, activation=None, residual=None):
+    """act(x weight^T + bias) + residual, in one pass over the product.
+
+    x [...,C], weight [H,C] (as torch.nn.Linear has it) in x's type, bias [H] in that type or float32, residual [...,H]
+    in that type or float32, which is then the result's.  `activation` is None, "relu", "silu", "gelu" (x times the
+    normal distribution), "tanh" or "sigmoid".  Sums are float32; float32 inputs are multiplied to float32's rounding.
+    Rows may lie at any distance, and time-major views of batch-first tensors are read as they lie."""
+    if activation not in ops.ACTIVATIONS:
+        raise ValueError(f"haste_b200: activation must be one of {list(ops.ACTIVATIONS)}, got {activation!r}")
+    if _shown():
+        return _FusedLinear.apply(activation, x, weight, bias, residual)
+    return _native().fused_linear(x, weight, bias, ops.ACTIVATIONS[activation], residual)

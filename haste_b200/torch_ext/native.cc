@@ -45,7 +45,7 @@ bool has_c(int cell) { return cell == LSTM || cell == LN_LSTM; }
   X(selective_scan_forward) X(selective_scan_backward) X(selective_scan_checkpoints)                 \
   X(selective_scan_scratch) X(fused_norm_forward) X(fused_norm_backward) X(fused_norm_scratch)       \
   X(gated_scan_forward) X(gated_scan_backward) X(gated_scan_checkpoints) X(gated_scan_scratch)            \
-  X(grad_norm) X(clip_gradients) X(grad_norm_scratch)
+  X(linear_forward) X(linear_backward) X(linear_scratch) X(grad_norm) X(clip_gradients) X(grad_norm_scratch)
 struct Library {
 #define HB_FIELD(f) decltype(&haste_b200_##f) f = nullptr;
   HB_FUNCTIONS(HB_FIELD)

@@ -131,6 +131,187 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ fused_linear
+// The rows of [...,C] in one order: that of the leading axes, or of the first two swapped (a batch-first tensor seen
+// time-major), whichever lies in memory with one distance from row to row.
+bool one_distance(const Tensor& t, int64_t* ld) {
+  const int64_t C = t.size(-1);
+  *ld = C;
+  int64_t next = -1;  // rows that the axes so far hold, times their distance
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (next < 0) *ld = t.stride(i);
+    else if (t.stride(i) != next) return false;
+    next = t.stride(i) * t.size(i);
+  }
+  return *ld >= C;  // (not repeated or overlapping ones)
+}
+struct Matrix {
+  Tensor t;
+  int64_t ld;
+};
+Matrix matrix(Tensor t, bool swapped) {
+  if (swapped) t = t.transpose(0, 1);
+  int64_t ld;
+  if ((t.size(-1) > 1 && t.stride(-1) != 1) || !one_distance(t, &ld)) {
+    t = t.contiguous();
+    ld = t.size(-1);
+  }
+  return {t, ld};
+}
+
+struct Linear {
+  haste_b200_linear a{};
+  Tensor weight, bias;
+  Matrix x;
+  bool swapped = false;
+  std::vector<int64_t> sizes;  // of y, in x's order
+  Linear(const Tensor& x_, const Tensor& weight_, const OptTensor& bias_, int64_t activation) {
+    if (x_.dim() < 1) refuse("x must have a dimension at least, got " + shape_of(x_));
+    dims(weight_, "weight", 2);
+    const int64_t C = x_.size(-1), H = weight_.size(0);
+    a.dtype = a.out_dtype = a.param_dtype = storage(x_);
+    if (C < 1 || H < 1 || C >= 1 << 20 || H >= 1 << 20) refuse("weight must have 1 to 2^20 - 1 rows and columns, got " + shape_of(weight_));
+    shape(weight_, "weight", {H, C});
+    type(weight_, "weight", x_.scalar_type());
+    bias = given(bias_);
+    if (bias.defined()) {
+      shape(bias, "bias", {H});
+      type(bias, "bias", x_.scalar_type(), at::kFloat);
+      if (bias.scalar_type() == at::kFloat) a.param_dtype = HASTE_B200_F32;
+    }
+    const int64_t M = x_.numel() / C;
+    if (M > 1 << 30) refuse("too many rows: " + shape_of(x_));
+    devices(x_, {weight_, bias});
+    int64_t ld;
+    if (x_.dim() == 3 && x_.numel() && (C == 1 || x_.stride(-1) == 1) && !one_distance(x_, &ld))
+      swapped = one_distance(x_.transpose(0, 1), &ld);
+    x = matrix(x_, swapped);
+    weight = weight_.contiguous();
+    bias = contiguous(bias);
+    a.activation = (int)activation;
+    a.M = (int)M; a.C = (int)C; a.H = (int)H;
+    a.x = ptr(x.t); a.x_ld = x.ld;
+    a.weight = ptr(weight); a.bias = ptr(bias);
+    sizes = x.t.sizes().vec();
+    sizes.back() = H;
+  }
+  Tensor back(const Tensor& t) const { return swapped ? t.transpose(0, 1) : t; }
+  // A tensor of y's shape, in x's order.
+  Matrix like_y(const Tensor& t, const char* name) {
+    std::vector<int64_t> want = sizes;
+    if (swapped) std::swap(want[0], want[1]);
+    if (t.sizes() != at::IntArrayRef(want)) refuse(std::string(name) + " must have y's shape, got " + shape_of(t));
+    return matrix(t, swapped);
+  }
+};
+struct Scratch {
+  Tensor t;
+  Scratch(const Tensor& x, long long bytes) : t(bytes ? at::empty({bytes}, x.options().dtype(at::kByte)) : Tensor()) {}
+  void* get() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
+// (y, p or None): p, the sums with bias in x's type, [M,H] in x's order of rows, where a backward pass will need it.
+std::tuple<Tensor, OptTensor> fused_linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t activation,
+                                                   const OptTensor& residual, bool keep) {
+  Linear c(x, weight, bias, activation);
+  at::ScalarType out = x.scalar_type();
+  Matrix r;
+  if (residual) {
+    type(*residual, "residual", x.scalar_type(), at::kFloat);
+    devices(x, {*residual});
+    r = c.like_y(*residual, "residual");
+    out = residual->scalar_type();
+    c.a.residual = ptr(r.t);
+    c.a.residual_ld = r.ld;
+    if (out == at::kFloat) c.a.out_dtype = HASTE_B200_F32;
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty(c.sizes, x.options().dtype(out)), pre;
+  c.a.y = ptr(y);
+  c.a.y_ld = c.a.H;
+  if (keep && activation) {
+    pre = at::empty({c.a.M, c.a.H}, x.options());
+    c.a.pre = ptr(pre);
+  }
+  const Scratch scratch(x, lib.linear_scratch(&c.a, 0));
+  c.a.scratch = scratch.get();
+  CALL(linear_forward, &c.a, stream());
+  return {c.back(y), maybe(pre)};
+}
+
+// Gradients of x, weight and bias, those that are wanted.
+std::tuple<OptTensor, OptTensor, OptTensor> fused_linear_backward(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                                                                  int64_t activation, const OptTensor& pre_, const Tensor& dy_,
+                                                                  bool want_x, bool want_weight, bool want_bias) {
+  Linear c(x, weight, bias, activation);
+  type(dy_, "dy", x.scalar_type(), at::kFloat);
+  if (dy_.scalar_type() == at::kFloat) c.a.out_dtype = HASTE_B200_F32;
+  Tensor pre = given(pre_);
+  if (activation) {
+    if (!pre.defined()) refuse("an activation's backward pass needs the sums that the forward pass kept");
+    shape(pre, "pre", {c.a.M, c.a.H});
+    type(pre, "pre", x.scalar_type());
+    pre = pre.contiguous();
+  }
+  devices(x, {dy_, pre});
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Matrix dy = c.like_y(dy_, "dy");
+  c.a.pre = ptr(pre);
+  c.a.dy = ptr(dy.t);
+  c.a.dy_ld = dy.ld;
+  Tensor dx, dw, db;
+  if (want_x) {
+    dx = at::empty(c.x.t.sizes(), x.options());
+    c.a.dx = ptr(dx);
+    c.a.dx_ld = c.a.C;
+  }
+  if (want_weight) {
+    dw = at::empty_like(c.weight);
+    c.a.dweight = ptr(dw);
+  }
+  if (want_bias && c.bias.defined()) {
+    db = at::empty_like(c.bias);
+    c.a.dbias = ptr(db);
+  }
+  const Scratch scratch(x, lib.linear_scratch(&c.a, 1));
+  c.a.scratch = scratch.get();
+  CALL(linear_backward, &c.a, stream());
+  return {dx.defined() ? OptTensor(c.back(dx)) : OptTensor(), maybe(dw), maybe(db)};
+}
+
+struct LinearNode : public torch::autograd::Function<LinearNode> {
+  static variable_list forward(AutogradContext* ctx, int64_t activation, Tensor x, Tensor weight, OptTensor bias, OptTensor residual) {
+    auto [y, pre] = fused_linear_forward(x, weight, bias, activation, residual, true);
+    ctx->save_for_backward({x, weight, given(bias), given(pre)});
+    ctx->saved_data["activation"] = activation;
+    auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    ctx->saved_data["wants"] = (int64_t)(wants(x) | wants(weight) << 1 | wants(given(bias)) << 2 | wants(given(residual)) << 3);
+    ctx->set_materialize_grads(false);
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    return guarded("fused_linear", [&]() -> variable_list {
+      variable_list out(5);
+      if (!grad[0].defined()) return out;
+      const variable_list v = ctx->get_saved_variables();
+      const int64_t wants = ctx->saved_data["wants"].toInt();
+      if (wants & 7) {
+        auto [dx, dw, db] = fused_linear_backward(v[0], v[1], maybe(v[2]), ctx->saved_data["activation"].toInt(), maybe(v[3]), grad[0],
+                                                  wants & 1, wants & 2, wants & 4);
+        out[1] = given(dx); out[2] = given(dw); out[3] = given(db);
+      }
+      if (wants & 8) out[4] = grad[0];
+      return out;
+    });
+  }
+};
+
+Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t activation, const OptTensor& residual) {
+  if (!wants_grad({x, weight, bias, residual})) return std::get<0>(fused_linear_forward(x, weight, bias, activation, residual, false));
+  return LinearNode::apply(activation, x, weight, bias, residual)[0];
+}
+
 // ------------------------------------------------------------------ gradients
 // Tensors whose elements fill one range of memory, in any order of axes.
 haste_b200_gradient range_of(const Tensor& t, const char* name) {
@@ -213,6 +394,9 @@ void bind(py::module& m) {
   m.def("gated_scan_forward", &gated_scan_forward, free);
   m.def("gated_scan_step", &gated_scan_step, free);
   m.def("gated_scan_backward", &gated_scan_backward, free);
+  m.def("fused_linear", &fused_linear, free);
+  m.def("fused_linear_forward", &fused_linear_forward, free);
+  m.def("fused_linear_backward", &fused_linear_backward, free);
   m.def("clip_gradients", &clip_gradients, free);
 }
 

@@ -429,6 +429,43 @@ long long haste_b200_gated_scan_checkpoints(const haste_b200_gated_scan* args);
  * if `scratch` is NULL, at a cost in time where there are few channels. */
 long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int backward);
 
+/* ---- Projections ---------------------------------------------------------- */
+/* y[m,h] = act(sum_c x[m,c] weight[h,c] + bias[h]) + residual[m,h], on the tensor cores, sums in fp32 (fp32 operands:
+ * accurate to fp32 rounding).  No counterpart in the reference, whose layers project inside.
+ *   x [M,C], residual, y [M,H]: rows x_ld, residual_ld, y_ld elements apart, elements of a row next to each other
+ *   weight [H,C] dense, dtype; C and H are 1 to 2^20 - 1, M is at most 2^30   bias [H] param_dtype (F32 or dtype; may be NULL)
+ *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y.
+ *   pre [M,H] dense, dtype: the sums with bias, written for the backward pass; NULL if there will be none, or if
+ *   activation is HASTE_B200_IDENTITY.
+ * backward: dy [M,H] out_dtype, rows dy_ld apart; writes dx [M,C] (rows dx_ld apart; may be NULL), dweight [H,C] (may be
+ * NULL) in dtype and dbias [H] in param_dtype (may be NULL).  The residual's gradient is dy.
+ * scratch: haste_b200_linear_scratch() bytes, aligned to 256, asked for with all other members set (backward: dx,
+ * dweight, dbias not NULL if they will be written).  The calls keep nothing and may be captured. */
+#define HASTE_B200_IDENTITY 0
+#define HASTE_B200_RELU 1
+#define HASTE_B200_SILU 2
+#define HASTE_B200_GELU 3 /* x Phi(x), the normal distribution's own */
+#define HASTE_B200_TANH 4
+#define HASTE_B200_SIGMOID 5
+typedef struct {
+  int dtype, param_dtype, out_dtype, activation;
+  int M, C, H;
+  const void *x, *weight, *bias, *residual;
+  long long x_ld, residual_ld;
+  void* y;
+  long long y_ld;
+  void* pre;
+  const void* dy;
+  long long dy_ld;
+  void* dx;
+  long long dx_ld;
+  void *dweight, *dbias;
+  void* scratch;
+} haste_b200_linear;
+int haste_b200_linear_forward(const haste_b200_linear* args, void* stream);
+int haste_b200_linear_backward(const haste_b200_linear* args, void* stream);
+long long haste_b200_linear_scratch(const haste_b200_linear* args, int backward);
+
 /* ---- Gradient norm and clipping ------------------------------------------- */
 /* norm = sqrt(sum over all gradients of their squares);  out = data * min(1, max_norm / (norm + 1e-6)), with a factor
  * of 1 where max_norm is infinite.  No counterpart in the reference.

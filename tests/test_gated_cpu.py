@@ -77,6 +77,25 @@ def test_gated_scan_step_refuses():
         ssm.gated_scan_step(z(2, 4).requires_grad_(), z(2, 4), z(2, 4), out_state=z(2, 4))
 
 
+@pytest.mark.parametrize("change,error,says", [
+    (dict(x=torch.tensor(1.0)), ValueError, "a dimension at least"),
+    (dict(x=z(5, 2, 4, dtype=torch.float64)), TypeError, "float32, bfloat16 and float16"),
+    (dict(weight=z(6)), ValueError, "2 dimensions"),
+    (dict(weight=z(6, 5)), ValueError, "weight must be"),
+    (dict(weight=z(0, 4)), ValueError, "weight must have"),
+    (dict(x=z(5, 2, 0), weight=z(6, 0)), ValueError, "weight must have"),
+    (dict(weight=z(6, 4, dtype=torch.bfloat16)), TypeError, "weight must be"),
+    (dict(bias=z(4)), ValueError, "bias must be"),
+    (dict(bias=z(6, dtype=torch.float16)), TypeError, "bias must be"),
+    (dict(activation="swish"), ValueError, "activation must be one of"),
+    (dict(), RuntimeError, "CUDA tensor"),
+])
+def test_fused_linear_refuses(change, error, says):
+    from haste_b200 import ssm
+    with pytest.raises(error, match=says):
+        ssm.fused_linear(**(dict(x=z(5, 2, 4), weight=z(6, 4), bias=z(6)) | change))
+
+
 @pytest.mark.parametrize("args,error,says", [
     (([z(4, 4)[:, ::2]], 1.0), ValueError, "one range of memory"),
     (([z(4, dtype=torch.float64)], 1.0), TypeError, "float32, bfloat16 and float16"),
@@ -105,7 +124,7 @@ def test_entry_points_refuse_bad_blocks():
     import ctypes
     from haste_b200 import _C
     L = _C.lib()
-    for name in ("gated_scan_forward", "gated_scan_backward"):
+    for name in ("gated_scan_forward", "gated_scan_backward", "linear_forward", "linear_backward"):
         call = getattr(L, f"haste_b200_{name}")
         assert call(None, None) == 1
         assert b"null pointer" in L.haste_b200_last_error()
