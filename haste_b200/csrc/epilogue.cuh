@@ -55,42 +55,52 @@ __device__ __forceinline__ float normal(float v, float& bell) {
   return v < 0.f ? tail : 1.f - tail;
 }
 
-template <bool Accurate>
-__device__ __forceinline__ float activate(int act, float p) {
-  switch (act) {
-    case HASTE_B200_RELU: return p < 0.f ? 0.f : p;  // (a NaN stays)
-    case HASTE_B200_SILU: return silu(p);
-    case HASTE_B200_GELU: {
-      float bell;
-      return p * normal<Accurate>(p, bell);
-    }
-    case HASTE_B200_TANH: return tanh_<Accurate>(p);
-    case HASTE_B200_SIGMOID: return sigmoid(p);
-    default: return p;
+template <bool Accurate, int Act>
+__device__ __forceinline__ float activate(float p) {
+  if constexpr (Act == HASTE_B200_RELU) return p < 0.f ? 0.f : p;  // (a NaN stays)
+  if constexpr (Act == HASTE_B200_SILU) return silu(p);
+  if constexpr (Act == HASTE_B200_GELU) {
+    float bell;
+    return p * normal<Accurate>(p, bell);
   }
+  if constexpr (Act == HASTE_B200_TANH) return tanh_<Accurate>(p);
+  if constexpr (Act == HASTE_B200_SIGMOID) return sigmoid(p);
+  return p;
 }
-template <bool Accurate>
-__device__ __forceinline__ float slope(int act, float p) {
+template <bool Accurate, int Act>
+__device__ __forceinline__ float slope(float p) {
+  if constexpr (Act == HASTE_B200_RELU) return p > 0.f ? 1.f : p != p ? p : 0.f;
+  if constexpr (Act == HASTE_B200_SILU) return silu_slope(p, sigmoid(p));
+  if constexpr (Act == HASTE_B200_GELU) {
+    float bell;
+    const float n = normal<Accurate>(p, bell);
+    return fmaf(p * 0.3989422804014327f, bell, n);
+  }
+  if constexpr (Act == HASTE_B200_TANH) {
+    const float e = exp2_(fabsf(p) * -2.885390081777927f), r = reciprocal(1.f + e);
+    return 4.f * e * r * r;  // 1 - tanh^2
+  }
+  if constexpr (Act == HASTE_B200_SIGMOID) {
+    const float e = exp2_(fabsf(p) * -1.4426950408889634f), r = reciprocal(1.f + e);
+    return e * r * r;
+  }
+  return 1.f;
+}
+// f with the activation as a compile-time number: chosen once for all elements that f walks (chosen for each, next to
+// the others' code, a pass waits for its instructions: bf16 64000 x 2048 slopes 260 us).
+template <int A>
+struct Act {
+  static constexpr int value = A;
+};
+template <typename F>
+__host__ __device__ __forceinline__ void with_activation(int act, const F& f) {
   switch (act) {
-    case HASTE_B200_RELU: return p > 0.f ? 1.f : p != p ? p : 0.f;
-    case HASTE_B200_SILU: {
-      const float s = sigmoid(p);
-      return silu_slope(p, s);
-    }
-    case HASTE_B200_GELU: {
-      float bell;
-      const float n = normal<Accurate>(p, bell);
-      return fmaf(p * 0.3989422804014327f, bell, n);
-    }
-    case HASTE_B200_TANH: {
-      const float e = exp2_(fabsf(p) * -2.885390081777927f), r = reciprocal(1.f + e);
-      return 4.f * e * r * r;  // 1 - tanh^2
-    }
-    case HASTE_B200_SIGMOID: {
-      const float e = exp2_(fabsf(p) * -1.4426950408889634f), r = reciprocal(1.f + e);
-      return e * r * r;
-    }
-    default: return 1.f;
+    case HASTE_B200_RELU: f(Act<HASTE_B200_RELU>()); break;
+    case HASTE_B200_SILU: f(Act<HASTE_B200_SILU>()); break;
+    case HASTE_B200_GELU: f(Act<HASTE_B200_GELU>()); break;
+    case HASTE_B200_TANH: f(Act<HASTE_B200_TANH>()); break;
+    case HASTE_B200_SIGMOID: f(Act<HASTE_B200_SIGMOID>()); break;
+    default: f(Act<HASTE_B200_IDENTITY>());
   }
 }
 
@@ -103,7 +113,7 @@ template <typename T, typename TO>
 __device__ __forceinline__ void finish(const Epilogue& e, float v, int m, int n, TO* y) {
   if (e.bias) v += bias_at<T>(e, n);
   if (e.pre) st(static_cast<T*>(e.pre) + m * e.ld_pre + n, v);
-  v = activate<sizeof(T) == 4>(e.act, v);
+  with_activation(e.act, [&](auto act) { v = activate<sizeof(T) == 4, decltype(act)::value>(v); });
   if (e.residual) v += ld(static_cast<const TO*>(e.residual) + m * e.ld_res + n);
   st(y, v);
 }
@@ -113,8 +123,10 @@ __device__ __forceinline__ void finish4(const Epilogue& e, float (&v)[4], const 
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] += bias[j];
   if (e.pre) store<T, 4>(static_cast<T*>(e.pre) + m * e.ld_pre + n, v);
+  with_activation(e.act, [&](auto act) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = activate<sizeof(T) == 4>(e.act, v[j]);
+    for (int j = 0; j < 4; ++j) v[j] = activate<sizeof(T) == 4, decltype(act)::value>(v[j]);
+  });
   if (e.residual) {
     float r[4];
     load<TO, 4>(static_cast<const TO*>(e.residual) + m * e.ld_res + n, r);

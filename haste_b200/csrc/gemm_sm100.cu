@@ -65,13 +65,16 @@ struct Params {
 };
 // A contraction that stores its sums as they are, or one that is a projection's, with operands of type T.
 struct Plain {
-  static constexpr bool projection = false;
+  static constexpr bool projection = false, tiles = false;
 };
-template <typename T_>
+template <typename T_, typename TO_>
 struct Projection {
-  static constexpr bool projection = true;
+  static constexpr bool projection = true, tiles = sizeof(T_) == 2;
   typedef T_ T;
+  typedef TO_ TO;
+  CUtensorMap y, pre;  // for whole-tile stores
   Epilogue e;
+  int whole;  // y, what is kept and the residual take them
 };
 
 template <int NPROD>
@@ -226,6 +229,105 @@ __device__ __forceinline__ void store_projection(const Params& p, const Epilogue
       epi::finish<T, TO>(e, at[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4], m0 + r, n0 + lane, dst + r * p.ldc + lane);
   }
 }
+// Sixteen-bit operands: a warp's 32 rows of the tile, in steps of 128 bytes of y.  Lane r holds row r of the sums, so bias and
+// activation happen in the registers that tensor memory is read into; y (and p, what the backward pass reads) goes as
+// 16-byte words into a tile of shared memory that a bulk store takes out, and the residual comes in by the same tile: rows
+// by eight lanes from memory, words of its own row to each lane.  buf: 4 KB for y, 4 KB for p.
+// (With the sums themselves through shared memory, and loads and stores of four elements behind it, the epilogue bounded
+// the product: bf16 64000 x 2048, K = 1024 with SiLU 401 us, with p 428.)
+template <typename EP>
+__device__ __forceinline__ void project_tile(const Params& p, const EP& ep, uint32_t taddr, int m0, int n0, uint8_t* buf) {
+  typedef typename EP::T T;
+  typedef typename EP::TO TO;
+  constexpr int CW = 128 / sizeof(TO), V = 16 / sizeof(TO);  // columns of a step, of a 16-byte word of y
+  const Epilogue& e = ep.e;
+  const int lane = threadIdx.x & 31;
+  uint4* tile = reinterpret_cast<uint4*>(buf);
+  uint4* kept = tile + 256;
+  uint4 res[8];
+  auto fetch = [&](int n) {  // rows i * 4 + lane / 8, word lane % 8
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), c = n + (lane & 7) * V;
+      res[i] = make_uint4(0, 0, 0, 0);
+      if (m0 + r < p.M && c < p.N)
+        res[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const TO*>(e.residual) + (long long)(m0 + r) * e.ld_res + c));
+    }
+  };
+  if (e.residual) fetch(n0);
+#pragma unroll 1
+  for (int n = n0; n < min(n0 + BN, p.N); n += CW) {
+    if (lane == 0) tma_stores_read();
+    __syncwarp();  // the tiles before have been read
+    if (e.residual) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        tile[r * 8 + ((lane & 7) ^ (r & 7))] = res[i];
+      }
+      __syncwarp();
+      if (n + CW < n0 + BN) fetch(n + CW);
+    }
+#pragma unroll
+    for (int h = 0; h < CW / 32; ++h) {
+      uint32_t r[32];
+      float v[32];
+      tc_ld32(taddr + (n - n0) + h * 32, r);
+      if (e.bias) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {  // (N is a multiple of eight)
+          float b[8] = {};
+          const int c = n + h * 32 + j;
+          if (c < p.N) {
+            if (e.bias_f32) ss::load<float, 8>(static_cast<const float*>(e.bias) + c, b);
+            else ss::load<T, 8>(static_cast<const T*>(e.bias) + c, b);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[j + k] = b[k];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      }
+      tc_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+      if (e.pre) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint4 word;
+          ss::store<T, 8>(reinterpret_cast<T*>(&word), reinterpret_cast<const float(&)[8]>(v[w * 8]));
+          if (sizeof(TO) == 2) kept[lane * 8 + ((h * 4 + w) ^ (lane & 7))] = word;
+          else if (m0 + lane < p.M && n + w * 8 < p.N)  // (half a line a row)
+            *reinterpret_cast<uint4*>(static_cast<T*>(e.pre) + (long long)(m0 + lane) * e.ld_pre + n + w * 8) = word;
+        }
+      }
+      epi::with_activation(e.act, [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = epi::activate<false, decltype(act)::value>(v[j]);
+      });
+#pragma unroll
+      for (int w = 0; w < 32 / V; ++w) {
+        uint4* word = &tile[lane * 8 + ((h * 4 + w) ^ (lane & 7))];
+        float(&y)[V] = reinterpret_cast<float(&)[V]>(v[w * V]);
+        if (e.residual) {
+          float q[V];
+          ss::load<TO, V>(reinterpret_cast<const TO*>(word), q);
+#pragma unroll
+          for (int k = 0; k < V; ++k) y[k] += q[k];
+        }
+        ss::store<TO, V>(reinterpret_cast<TO*>(word), y);
+      }
+    }
+    fence_async();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&ep.y, smem_u32(tile), n, m0, 0);
+      if (sizeof(TO) == 2 && e.pre) tma_store_3d(&ep.pre, smem_u32(kept), n, m0, 0);
+    }
+  }
+}
+
 template <int NPROD, int MODE, typename EP>
 __device__ __forceinline__ void store_chunk(const Params& p, const EP& ep, int sp, int m0, int n0, uint8_t* buf, int ea = 0,
                                             int eb = 0) {
@@ -236,8 +338,7 @@ __device__ __forceinline__ void store_chunk(const Params& p, const EP& ep, int s
     if (p.partial)
       store_tile<false, NEVER, float>(tile, p.partial + ((long long)sp * p.M + m0) * p.partial_ld + n0, p.partial_ld,
                                       min(32, p.M - m0), 32, true, false, 0, 0);
-    else if (sizeof(typename EP::T) == 4 || p.c_is_bf16) store_projection<typename EP::T, typename EP::T>(p, ep.e, tile, m0, n0);
-    else store_projection<typename EP::T, float>(p, ep.e, tile, m0, n0);
+    else store_projection<typename EP::T, typename EP::TO>(p, ep.e, tile, m0, n0);
   } else if constexpr (NPROD == 1) {
     if (p.partial)  // rows of whole chunks
       store_tile<false, NEVER, float>(tile, p.partial + ((long long)sp * p.M + m0) * p.partial_ld + n0, p.partial_ld,
@@ -268,28 +369,37 @@ __device__ __forceinline__ void store_chunk(const Params& p, const EP& ep, int s
 template <int NPROD, int MODE>
 constexpr int chunk_of() { return MODE == PLAIN ? Cfg<NPROD>::CHUNK : (MODE == F16_PLANES ? 2 : 1); }
 
+// Shared memory: the ring, a tile per epilogue warp (two where whole tiles are stored, which on pairs takes a stage), barriers.
+template <int NPROD, typename EP, bool PAIR>
+struct Room {
+  static constexpr int STAGES = PAIR && EP::tiles ? Cfg<NPROD>::STAGES - 1 : Cfg<NPROD>::STAGES;
+  static constexpr int TILE = EP::tiles ? 2 * EPI_TILE : EPI_TILE, WARPS = PAIR ? 8 : 4;
+  static constexpr int BARS = STAGES * Cfg<NPROD>::STAGE_BYTES + WARPS * TILE, SMEM = BARS + 256 + 1024 /*align*/;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
 template <int NPROD, int MODE = PLAIN, typename EP = Plain>
 __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p,
                                           const EP& ep = EP()) {
   using C = Cfg<NPROD>;
+  using R = Room<NPROD, EP, false>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(aligned + C::STAGES * C::STAGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aligned + R::BARS);
   // barrier slots: full[STAGES], empty[STAGES], acc_full[NACC], acc_empty[NACC]
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
-  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
-  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + NACC + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * NACC);
+  auto empty_bar = [&](int s) { return bar0 + 8u * (R::STAGES + s); };
+  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * R::STAGES + a); };
+  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * R::STAGES + NACC + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * R::STAGES + 2 * NACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int chunk = chunk_of<NPROD, MODE>();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < R::STAGES; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
@@ -349,7 +459,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
               tma_load_3d(db, mb, full_bar(stage), k0, n0, pl);
             }
           }
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+          if (++stage == R::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -405,7 +515,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
               }
             }
             tc_commit(empty_bar(stage));  // frees the stage once these MMAs have read it
-            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            if (++stage == R::STAGES) { stage = 0; phase ^= 1u; }
           }
           if (ok) tc_commit(accf_bar(acc));  // this chunk of the accumulation is complete
         }
@@ -414,7 +524,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quad = warp & 3;  // tensor-memory lane quadrant this warp may read
-    uint8_t* tile = aligned + C::STAGES * C::STAGE_BYTES + 256 + (warp - 2) * EPI_TILE;
+    uint8_t* tile = aligned + R::STAGES * C::STAGE_BYTES + (warp - 2) * R::TILE;
     uint32_t acc_phase = 0;  // one parity bit per accumulator
     int cidx = 0;
     bool ok = true;
@@ -450,8 +560,14 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
             for (int j = 0; j < 32; ++j) sum[(C::CHUNK ? ch * 32 : 0) + j] += __uint_as_float(r[j]);
           }
         } else {
+          bool stored = false;
+          if constexpr (EP::tiles)
+            if (ep.whole && !p.partial) {
+              if (m0 < p.M) project_tile(p, ep, taddr, m0, n0, tile);
+              stored = true;
+            }
 #pragma unroll 1
-          for (int ch = 0; ch < BN / 32 && m0 < p.M && n0 + ch * 32 < p.N; ++ch) {
+          for (int ch = 0; ch < BN / 32 && !stored && m0 < p.M && n0 + ch * 32 < p.N; ++ch) {
             uint32_t r[32];
             tc_ld32(taddr + ch * 32, r);
             tc_wait_ld();
@@ -494,6 +610,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
     }
   }
 
+  if (EP::tiles && warp >= 2 && lane == 0) tma_stores_done();
   // Drain: every role arrives here, also after a time-out, so tensor memory is released.
   tc_fence_before();
   __syncthreads();
@@ -510,10 +627,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     const __grid_constant__ Params p) {
   gemm_tile<NPROD>(map_a, map_b, p);
 }
-template <int NPROD, typename T>
+template <int NPROD, typename T, typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
 projection_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                  const __grid_constant__ Params p, const __grid_constant__ Projection<T> ep) {
+                  const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
   gemm_tile<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 // fp16 planes, or the bf16 planes that have taken their place.
@@ -551,17 +668,18 @@ template <int NPROD, int MODE = PLAIN, typename EP = Plain>
 __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtensorMap& map_b, const Params& p,
                                           const EP& ep = EP()) {
   using C = Cfg<NPROD>;
+  using R = Room<NPROD, EP, true>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(aligned + C::STAGES * C::STAGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aligned + R::BARS);
   // barrier slots: full[STAGES], empty[STAGES], acc_full[2], acc_empty[2]
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
-  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
-  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + PAIR_NACC + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * PAIR_NACC);
+  auto empty_bar = [&](int s) { return bar0 + 8u * (R::STAGES + s); };
+  auto accf_bar = [&](int a) { return bar0 + 8u * (2 * R::STAGES + a); };
+  auto acce_bar = [&](int a) { return bar0 + 8u * (2 * R::STAGES + PAIR_NACC + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * R::STAGES + 2 * PAIR_NACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -570,7 +688,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
   constexpr int chunk = chunk_of<NPROD, MODE>();
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
+    for (int s = 0; s < R::STAGES; ++s) {
       mbar_init(full_bar(s), 1);   // CTA 0's producer; the bytes of both CTAs' loads
       mbar_init(empty_bar(s), 1);  // one commit
     }
@@ -632,7 +750,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
               tma_load_3d_pair(db, &map_b, fb, k0, n0, pl);
             }
           }
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+          if (++stage == R::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -683,7 +801,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
               }
             }
             tc_commit_pair(empty_bar(stage), 3);  // frees the stage in both CTAs
-            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            if (++stage == R::STAGES) { stage = 0; phase ^= 1u; }
           }
           if (ok) tc_commit_pair(accf_bar(acc), 3);  // this chunk is complete in both CTAs
         }
@@ -692,7 +810,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
     const int quad = warp & 3;         // tensor-memory lane quadrant this warp may read
-    uint8_t* tile = aligned + C::STAGES * C::STAGE_BYTES + 256 + (warp - 2) * EPI_TILE;
+    uint8_t* tile = aligned + R::STAGES * C::STAGE_BYTES + (warp - 2) * R::TILE;
     const int half = (warp - 2) >> 2;  // which 128 columns of the accumulator
     uint32_t acc_phase = 0;  // one parity bit per accumulator
     int cidx = 0;
@@ -728,8 +846,14 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
             for (int j = 0; j < 16; ++j) sum[(C::CHUNK ? ch * 16 : 0) + j] += __uint_as_float(r[j]);
           }
         } else {
+          bool stored = false;
+          if constexpr (EP::tiles)
+            if (ep.whole && !p.partial) {
+              if (m0 < p.M) project_tile(p, ep, taddr, m0, n0, tile);
+              stored = true;
+            }
 #pragma unroll 1
-          for (int ch = 0; ch < BN / 32 && m0 < p.M && n0 + ch * 32 < p.N; ++ch) {
+          for (int ch = 0; ch < BN / 32 && !stored && m0 < p.M && n0 + ch * 32 < p.N; ++ch) {
             uint32_t r[32];
             tc_ld32(taddr + ch * 32, r);
             tc_wait_ld();
@@ -763,6 +887,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
 
   // Drain: every role of both CTAs arrives here, also after a time-out.  Neither CTA may leave
   // while the other's MMAs can still read its shared memory or signal its barriers.
+  if (EP::tiles && warp >= 2 && lane == 0) tma_stores_done();
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -780,10 +905,10 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                          const __grid_constant__ Params p) {
   gemm_pair<NPROD>(map_a, map_b, p);
 }
-template <int NPROD, typename T>
+template <int NPROD, typename T, typename TO>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 projection_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                       const __grid_constant__ Params p, const __grid_constant__ Projection<T> ep) {
+                       const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
   gemm_pair<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
@@ -1169,10 +1294,15 @@ std::atomic<bool> g_attr_set[kMaxDevices];
 std::atomic<int> g_max_pairs[kMaxDevices];  // 0: not asked yet, -1: no clusters, else the count
 
 template <int NPROD>
-constexpr int single_smem() { return Cfg<NPROD>::SMEM + 4 * EPI_TILE; }
+constexpr int single_smem() { return Room<NPROD, Plain, false>::SMEM; }
 template <int NPROD>
-constexpr int pair_smem() { return Cfg<NPROD>::SMEM + PAIR_EPI_WARPS * EPI_TILE; }
-static_assert(pair_smem<1>() <= 232448 && pair_smem<3>() <= 232448 && pair_smem<6>() <= 232448, "shared memory per CTA");
+constexpr int pair_smem() { return Room<NPROD, Plain, true>::SMEM; }
+template <int NPROD, typename T, typename TO>
+cudaError_t allow_projection() {
+  const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  const cudaError_t e = cudaFuncSetAttribute(projection_kernel<NPROD, T, TO>, attr, Room<NPROD, Projection<T, TO>, false>::SMEM);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(projection_pair_kernel<NPROD, T, TO>, attr, Room<NPROD, Projection<T, TO>, true>::SMEM);
+}
 
 int set_kernel_attributes() {
   int dev = 0;
@@ -1186,12 +1316,11 @@ int set_kernel_attributes() {
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<1>, attr, pair_smem<1>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<3>, attr, pair_smem<3>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<6>, attr, pair_smem<6>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<1, __nv_bfloat16>, attr, single_smem<1>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<1, __half>, attr, single_smem<1>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_kernel<6, float>, attr, single_smem<6>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<1, __nv_bfloat16>, attr, pair_smem<1>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<1, __half>, attr, pair_smem<1>()));
-  HB_CUDA_OK(cudaFuncSetAttribute(projection_pair_kernel<6, float>, attr, pair_smem<6>()));
+  HB_CUDA_OK((allow_projection<1, __nv_bfloat16, __nv_bfloat16>()));
+  HB_CUDA_OK((allow_projection<1, __nv_bfloat16, float>()));
+  HB_CUDA_OK((allow_projection<1, __half, __half>()));
+  HB_CUDA_OK((allow_projection<1, __half, float>()));
+  HB_CUDA_OK((allow_projection<6, float, float>()));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_f16_kernel, attr, max(single_smem<3>(), single_smem<6>())));
   HB_CUDA_OK(cudaFuncSetAttribute(gemm_tcgen05_pair_f16_kernel, attr, max(pair_smem<3>(), pair_smem<6>())));
   if (dev >= 0 && dev < kMaxDevices) g_attr_set[dev].store(true, std::memory_order_release);
@@ -1351,6 +1480,49 @@ Cut::Cut(const GemmDesc& g) {
 }
 }  // namespace
 
+namespace {
+template <int NPROD, typename T, typename TO>
+int launch_projection(const GemmDesc& g, const Cut& c, const CUtensorMap& m_a, const CUtensorMap& m_b, const Params& p, cudaStream_t stream) {
+  Projection<T, TO> ep = {};
+  const Epilogue& e = *g.epilogue;
+  ep.e = e;
+  if (ep.tiles && !c.via_partial) {
+    auto lies = [](const void* q, long long ld, size_t size) { return !q || ((uintptr_t)q % 16 == 0 && ld * size % 16 == 0); };
+    ep.whole = c.N % 8 == 0 && lies(g.c, g.ldc, sizeof(TO)) && lies(e.residual, e.ld_res, sizeof(TO)) && lies(e.pre, e.ld_pre, sizeof(T)) &&
+               lies(e.bias, 8, 2) && make_store_map(&ep.y, g.c, sizeof(TO), c.N, c.M, g.ldc) &&
+               (!e.pre || make_store_map(&ep.pre, e.pre, sizeof(T), c.N, c.M, e.ld_pre));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.stream = stream;
+  const int items = c.tiles_m * c.tiles_n * c.splits;
+  if (c.pair) {
+    cfg.gridDim = dim3(2 * min(c.pairs, items));
+    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.dynamicSmemBytes = Room<NPROD, Projection<T, TO>, true>::SMEM;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<NPROD, T, TO>, m_a, m_b, p, ep));
+  } else {
+    cfg.gridDim = dim3(min(c.sms, items));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Room<NPROD, Projection<T, TO>, false>::SMEM;
+    HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_kernel<NPROD, T, TO>, m_a, m_b, p, ep));
+  }
+  count_launch(1);
+  if (!c.via_partial) return HASTE_B200_OK;
+  const int blocks = (int)min(((long long)c.M * c.N + 255) / 256, 8LL * c.sms);
+  projection_reduce_kernel<T, TO><<<blocks, 256, 0, stream>>>(p.partial, c.splits, c.M, c.N, c.part_ld, (TO*)g.c, g.ldc, e);
+  HB_LAUNCH_OK();
+  count_launch(1);
+  return HASTE_B200_OK;
+}
+}  // namespace
+
 size_t gemm_scratch(const GemmDesc& g) { return g.M > 0 && g.N > 0 && g.K > 0 ? Cut(g).bytes : 0; }
 
 bool gemm_reads_planes(const GemmDesc& g) { return gemm_path() != HASTE_B200_GEMM_SIMT && !refusal(g); }
@@ -1445,6 +1617,14 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
   };
   if (!maps(&m_a, &m_b, planes) || (f16 && !maps(&bf_a, &bf_b, 3)))
     return unsupported("tensor map encoding rejected the operand");
+  if (g.epilogue) {
+    if (g.dtype == HASTE_B200_F32) HB_TRY((launch_projection<6, float, float>(g, c, m_a, m_b, p, stream)));
+    else if (g.dtype == HASTE_B200_BF16 && g.dtype_c == HASTE_B200_F32) HB_TRY((launch_projection<1, __nv_bfloat16, float>(g, c, m_a, m_b, p, stream)));
+    else if (g.dtype == HASTE_B200_BF16) HB_TRY((launch_projection<1, __nv_bfloat16, __nv_bfloat16>(g, c, m_a, m_b, p, stream)));
+    else if (g.dtype_c == HASTE_B200_F32) HB_TRY((launch_projection<1, __half, float>(g, c, m_a, m_b, p, stream)));
+    else HB_TRY((launch_projection<1, __half, __half>(g, c, m_a, m_b, p, stream)));
+    return HASTE_B200_OK;
+  }
   if (pair) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * min(c.pairs, c.tiles_m * c.tiles_n * splits));
@@ -1457,15 +1637,7 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (g.epilogue) {
-      cfg.dynamicSmemBytes = planes == 3 ? pair_smem<6>() : pair_smem<1>();
-      if (g.dtype == HASTE_B200_F32)
-        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<6, float>, m_a, m_b, p, Projection<float>{*g.epilogue}));
-      else if (g.dtype == HASTE_B200_BF16)
-        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<1, __nv_bfloat16>, m_a, m_b, p, Projection<__nv_bfloat16>{*g.epilogue}));
-      else
-        HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_pair_kernel<1, __half>, m_a, m_b, p, Projection<__half>{*g.epilogue}));
-    } else if (f16) {
+    if (f16) {
       cfg.dynamicSmemBytes = max(pair_smem<3>(), pair_smem<6>());
       HB_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tcgen05_pair_f16_kernel, m_a, m_b, bf_a, bf_b, p));
     } else if (planes == 3) {
@@ -1480,13 +1652,7 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
     }
   } else {
     const int grid = min(c.sms, c.tiles_m * c.tiles_n * splits);
-    if (g.epilogue && g.dtype == HASTE_B200_F32)
-      projection_kernel<6, float><<<grid, THREADS, single_smem<6>(), stream>>>(m_a, m_b, p, Projection<float>{*g.epilogue});
-    else if (g.epilogue && g.dtype == HASTE_B200_BF16)
-      projection_kernel<1, __nv_bfloat16><<<grid, THREADS, single_smem<1>(), stream>>>(m_a, m_b, p, Projection<__nv_bfloat16>{*g.epilogue});
-    else if (g.epilogue)
-      projection_kernel<1, __half><<<grid, THREADS, single_smem<1>(), stream>>>(m_a, m_b, p, Projection<__half>{*g.epilogue});
-    else if (f16)
+    if (f16)
       gemm_tcgen05_f16_kernel<<<grid, THREADS, max(single_smem<3>(), single_smem<6>()), stream>>>(m_a, m_b, bf_a, bf_b, p);
     else if (planes == 3)
       gemm_tcgen05_kernel<6><<<grid, THREADS, single_smem<6>(), stream>>>(m_a, m_b, p);
@@ -1498,20 +1664,6 @@ int gemm_sm100(const GemmDesc& g, cudaStream_t stream) {
   HB_LAUNCH_OK();
   count_launch(1);
   if (c.via_partial) {
-    if (g.epilogue) {
-      const int blocks = (int)min(((long long)M * N + 255) / 256, 8LL * c.sms);
-#define HB_REDUCE(T, TO) \
-  projection_reduce_kernel<T, TO><<<blocks, 256, 0, stream>>>(partial, splits, M, N, c.part_ld, (TO*)g.c, g.ldc, *g.epilogue)
-      if (g.dtype == HASTE_B200_F32) HB_REDUCE(float, float);
-      else if (g.dtype == HASTE_B200_BF16 && g.dtype_c == HASTE_B200_BF16) HB_REDUCE(__nv_bfloat16, __nv_bfloat16);
-      else if (g.dtype == HASTE_B200_BF16) HB_REDUCE(__nv_bfloat16, float);
-      else if (g.dtype_c == HASTE_B200_F16) HB_REDUCE(__half, __half);
-      else HB_REDUCE(__half, float);
-#undef HB_REDUCE
-      HB_LAUNCH_OK();
-      count_launch(1);
-      return HASTE_B200_OK;
-    }
     auto reduce = g.dtype_c == HASTE_B200_BF16  ? launch_reduce<__nv_bfloat16>
                   : g.dtype_c == HASTE_B200_F16 ? launch_reduce<__half>
                                                 : launch_reduce<float>;

@@ -20,9 +20,10 @@ using namespace ss;
 constexpr int THREADS = 256, ROWS = THREADS / 32;
 
 // A block takes 32 lanes of V columns and every chunks-th row in eights: a warp a row, four rows ahead.
-template <typename T, typename TO, int V>
-__global__ void __launch_bounds__(THREADS) slope_kernel(const T* pre, const TO* dy, long long dy_ld, T* dp, int act, int M, int H,
+template <typename T, typename TO, int V, int Act>
+__global__ void __launch_bounds__(THREADS) slope_kernel(const T* pre, const TO* dy, long long dy_ld, T* dp, int M, int H,
                                                         float* part) {
+  constexpr bool act = Act != HASTE_B200_IDENTITY;
   __shared__ float sums[ROWS][32][V + 1];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int n = (blockIdx.x * 32 + lane) * V;
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(THREADS) slope_kernel(const T* pre, const TO* 
       if (act) {
         unpack<T, V>(p[i], q);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= epi::slope<sizeof(T) == 4>(act, q[j]);
+        for (int j = 0; j < V; ++j) v[j] *= epi::slope<sizeof(T) == 4, Act>(q[j]);
       }
       if (!ok || m >= M) continue;
       if (dp) store<T, V>(dp + m * H + n, v);
@@ -82,8 +83,10 @@ bool direct(const haste_b200_linear& a) { return a.activation == HASTE_B200_IDEN
 template <typename T, typename TO, int V>
 int launch_slope(const haste_b200_linear& a, T* dp, float* part, int* chunks, cudaStream_t s) {
   *chunks = chunks_of(a.M, a.H, V);
-  slope_kernel<T, TO, V><<<dim3(ceil_div(a.H, 32 * V), *chunks), THREADS, 0, s>>>(
-      static_cast<const T*>(a.pre), static_cast<const TO*>(a.dy), a.dy_ld, dp, a.activation, a.M, a.H, part);
+  epi::with_activation(a.activation, [&](auto act) {
+    slope_kernel<T, TO, V, decltype(act)::value><<<dim3(ceil_div(a.H, 32 * V), *chunks), THREADS, 0, s>>>(
+        static_cast<const T*>(a.pre), static_cast<const TO*>(a.dy), a.dy_ld, dp, a.M, a.H, part);
+  });
   HB_LAUNCH_OK();
   count_launch(1);
   return HASTE_B200_OK;

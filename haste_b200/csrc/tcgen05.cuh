@@ -215,6 +215,18 @@ __device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t desc_
       : "memory");
 }
 
+// ---- tile stores: shared memory -> a tensor map's tile, clipped at its bounds ----------------
+// One thread issues, after every writer's fence_async() and a barrier among them; it waits before the tile is written
+// again (reads) and before it leaves (all).
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
+               "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- host side: tensor maps -------------------------------------------------------------
 inline PFN_cuTensorMapEncodeTiled encode_fn() {
   static PFN_cuTensorMapEncodeTiled fn = nullptr;
@@ -244,6 +256,17 @@ inline bool make_map(CUtensorMap* map, const void* ptr, long long inner, long lo
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+// A matrix of `rows` x `cols` elements of `bytes` (2 or 4) for stores of tiles of 128 bytes x 32 rows, 128-byte swizzle.
+inline bool make_store_map(CUtensorMap* map, void* ptr, int bytes, long long cols, long long rows, long long ld) {
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * bytes, (cuuint64_t)(ld * rows) * bytes};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / bytes), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return encode_fn()(map, bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides,
+                     box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc
