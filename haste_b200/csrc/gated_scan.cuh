@@ -25,7 +25,11 @@ namespace gated {
 using namespace ss;
 
 constexpr int THREADS = 256, SEG = THREADS / 32;  // a warp walks one of the tile's segments
-constexpr int FWD_L = 8, BWD_L = 4;               // steps of a segment
+#ifndef HB_FWD_L
+#define HB_FWD_L 8
+#define HB_FWD_B 2
+#endif
+constexpr int FWD_L = HB_FWD_L, BWD_L = 4, FWD_BLOCKS = HB_FWD_B;               // steps of a segment
 constexpr int FWD_TT = SEG * FWD_L, BWD_TT = SEG * BWD_L;
 constexpr int CKPT = BWD_TT;                      // steps between the states left for the backward pass
 
@@ -60,6 +64,8 @@ struct Place {
   }
 };
 
+// Two neighbouring channels go through each instruction (V of one: the second is idle).
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -70,191 +76,235 @@ __device__ __forceinline__ float rsqrt_fast(float v) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+__device__ __forceinline__ float sqrt_fast(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float at_most(float v, float most) {  // (a NaN stays)
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+  return r;
+}
+__device__ __forceinline__ float at_least(float v, float least) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(least));
+  return r;
+}
+template <int V, typename F>
+__device__ __forceinline__ float2 each(float2 v, const F& f) {
+  return make_float2(f(v.x), V == 2 ? f(v.y) : 0.f);
+}
+template <typename T, int V>
+__device__ __forceinline__ float2 pair_of(const Raw<T, V>& r) {
+  float v[V];
+  unpack<T, V>(r, v);
+  return make_float2(v[0], v[V - 1]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pair(T* p, float2 v) {
+  const float w[2] = {v.x, v.y};
+  store<T, V>(p, reinterpret_cast<const float(&)[V]>(w));
+}
+template <int V>
+__device__ __forceinline__ float2 load_floats(const float* p) {
+  return make_float2(p[0], V == 2 ? p[V - 1] : 0.f);
+}
+template <int V>
+__device__ __forceinline__ void store_floats(float* p, float2 v) {
+  p[0] = v.x;
+  if (V == 2) p[V - 1] = v.y;
+}
 constexpr float LOG2E = 1.4426950408889634f;
 
-// sigmoid(v), sigmoid(-v) and their product, each to its own last bits.
-struct Gate {
-  float r, rest, slope;
-  __device__ __forceinline__ explicit Gate(float v) {
-    const float e = exp2_fast(fabsf(v) * -LOG2E), big = reciprocal(1.f + e), small = e * big;
-    const bool up = v > 0.f;
-    r = up ? big : small;
-    rest = up ? small : big;
-    slope = small * big;
+// r = sigmoid(v) and 1 - r, each to its own last bits; exponentials above 2^125 are held there, so that 1 - r, which is
+// their product with r, stays one.
+template <int V>
+__device__ __forceinline__ void sigmoids(float2 v, float2& r, float2& rest) {
+  const float2 e = each<V>(__fmul2_rn(v, both(-LOG2E)), [](float x) { return at_most(exp2_fast(x), 0x1p125f); });
+  r = each<V>(__fadd2_rn(e, both(1.f)), [](float x) { return reciprocal(x); });
+  rest = __fmul2_rn(e, r);
+}
+template <int V>
+__device__ __forceinline__ float2 sigmoids(float2 v) {
+  const float2 e = each<V>(__fmul2_rn(v, both(-LOG2E)), [](float x) { return exp2_fast(x); });
+  return each<V>(__fadd2_rn(e, both(1.f)), [](float x) { return reciprocal(x); });
+}
+// 2^l for l <= 0 less one, n, and a = 1 + n.  A decay lies next to one, where the special function unit's results are low by
+// 2.4e-8 on average; a state that keeps 1 / (1 - a) steps would add that up.  So n is computed to its own last bits (the
+// exponential's series, where a is above 0.7; `far`: some of the block's channels may go below), and a rounded
+// once, to either side.
+template <int V>
+__device__ __forceinline__ void decays(float2 l, bool far, float2& a, float2& n) {
+  constexpr float c[] = {1.5252733804059840e-05f, 1.5403530393381608e-04f, 1.3333558146428441e-03f, 9.6181291076284772e-03f,
+                         5.5504108664821576e-02f, 2.4022650695910069e-01f, 6.9314718055994529e-01f};  // ln(2)^k / k!
+  float2 p = both(c[0]);
+#pragma unroll
+  for (int k = 1; k < 7; ++k) p = __ffma2_rn(p, l, both(c[k]));
+  n = __fmul2_rn(p, l);
+  a = __fadd2_rn(n, both(1.f));
+  if (far) {
+    const float2 e = each<V>(l, [](float x) { return exp2_fast(x); });
+    const bool x = l.x < -0.505f, y = l.y < -0.505f;
+    a = make_float2(x ? e.x : a.x, y ? e.y : a.y);
+    n = make_float2(x ? e.x - 1.f : n.x, y ? e.y - 1.f : n.y);
   }
-};
+}
+// Without decay: a = r, rounded once to either side where it is near one.
+__device__ __forceinline__ float2 kept(float2 r, float2 rest) {
+  const float2 a = __ffma2_rn(rest, both(-1.f), both(1.f));
+  return make_float2(r.x > 0.5f ? a.x : r.x, r.y > 0.5f ? a.y : r.y);
+}
 
-// What a step does to the state.  A decay lies next to one, where the special function unit's results are low by
-// 2.4e-8 on average; a state that keeps 1 / (1 - a) steps would add that up.  So 1 - a is computed to its own last
-// bits (the exponential's series, where a is above 0.7), and a, its difference from one, is rounded once, to either side.
-template <bool Decay>
-struct Step {
-  float a, w, over;  // over: 1 / w, 0 where w is
-  __device__ __forceinline__ Step(const Gate& g, float decay) {
-    if constexpr (Decay) {
-      const float l = decay * g.r;
-      float p = 1.f / 5040;
-      p = fmaf(p, l, 1.f / 720);
-      p = fmaf(p, l, 1.f / 120);
-      p = fmaf(p, l, 1.f / 24);
-      p = fmaf(p, l, 1.f / 6);
-      p = fmaf(p, l, 0.5f);
-      p = fmaf(p, l, 1.f);
-      const bool slow = l > -0.35f;
-      const float far = exp2_fast(l * LOG2E), m = slow ? -l * p : 1.f - far;
-      a = slow ? 1.f - m : far;
-      const float v = fmaf(m, a, m);  // 1 - a^2
-      over = v >= 1.1754944e-38f ? rsqrt_fast(v) : v * 0.f;  // (a NaN stays)
-      w = v * over;
-    } else {
-      a = g.r > 0.5f ? 1.f - g.rest : g.r;
-      w = g.rest;
-      over = 0.f;
-    }
+// A channel's decay in units of log(2): values above zero count as zero, so that no state grows.
+template <bool Decay, int V>
+__device__ __forceinline__ float2 decay_of(const float* decay, int d) {
+  if (!Decay) return both(0.f);
+  return each<V>(load_floats<V>(decay + d), [](float v) { return at_most(v, 0.f) * LOG2E; });
+}
+__device__ __forceinline__ bool goes_far(float2 decay) { return __any_sync(0xffffffffu, decay.x < -0.5f || decay.y < -0.5f); }
+
+// A load that needs no predicate.
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
+  Raw<T, V> r;
+  constexpr int B = sizeof(T) * V;
+  if constexpr (B == 2) {
+    unsigned short w;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(w) : "l"(p));
+    r.w[0] = w;
+  } else if constexpr (B == 4) {
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
+  } else {
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
   }
-};
-
-// A channel's decay: values above zero count as zero, so that no state grows.
-template <bool Decay>
-__device__ __forceinline__ float decay_of(const float* decay, int d, bool ok) {
-  if (!Decay || !ok) return 0.f;
-  const float v = decay[d];
-  return v > 0.f ? 0.f : v;
+  return r;
+}
+// The steps of a segment, in front of `stop` where not all of a tile is.
+template <int L, typename T, int V>
+__device__ __forceinline__ void fetch_steps(Raw<T, V> (&r)[L], const Seq<const T>& q, int t, int n, int d, int stop, bool whole) {
+  const T* p = q.at(t, n) + d;
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) r[j] = load_raw<T, V>(p + (long long)j * q.t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < L; ++j) r[j] = load_if<T, V>(t + j < stop, p + (long long)j * q.t);
+  }
 }
 
 // ------------------------------------------------------------------ forward
-// A block takes 32 words of neighbouring channels (two channels of 16 bits, one of 32) and tiles of 64 steps, eight to a
-// warp.  A warp folds its steps into (product of decays, what they add to a state of zero), the warps' pairs meet in
-// shared memory, each warp folds those in front of its own into the tile's starting state, and walks its steps again
-// from registers.  One barrier a tile: pairs and the state behind the tile have two buffers.  The next tile's words are
-// under way from when the present ones have been used.
+// A block takes 64 neighbouring channels, two a lane (32, one a lane, where rows do not start on whole pairs), and tiles of
+// FWD_L steps to each of its eight warps.  A warp folds its steps into (product of decays, what they add to a state of
+// zero), the warps' pairs meet in shared memory, each warp folds those in front of its own into the tile's starting state,
+// and walks its steps again from registers.  One barrier a tile: pairs and the state behind the tile have two buffers.
+// The next tile's words are under way from when the present ones have been used.
 //
 // Few channels leave most of the GPU idle, so their sequences are cut into pieces and read twice (the second time from
 // L2): first (Ends) each piece but the last leaves its pair, then each piece starts from those in front of it.
 template <typename T, int V, bool Decay, bool In, bool Ends>
-__global__ void __launch_bounds__(THREADS, 2) gated_fwd(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
   constexpr int L = FWD_L, TT = FWD_TT;
-  __shared__ float2 pairs[2][SEG][V][32];
-  __shared__ float behind[2][V][32];
+  __shared__ float4 pairs[2][SEG][32];
+  __shared__ float2 behind[2][32];
   const Place<V> at(a);
   const int lane = threadIdx.x % 32, seg = threadIdx.x / 32;
-  const int d = at.ok ? at.d : 0;
+  const int d = at.ok ? at.d : a.D - V;  // (lanes without channels repeat the last ones)
   const long long rows = (long long)a.N * a.D, row = (long long)at.n * a.D + d;
-  float decay[V], start[V], total[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    decay[v] = decay_of<Decay>(a.decay, d + v, at.ok);
-    start[v] = !Ends && at.ok && a.state ? a.state[row + v] : 0.f;
-    total[v] = 1.f;
-  }
+  const float2 decay = decay_of<Decay, V>(a.decay, d);
+  const bool far = goes_far(decay);
+  float2 start = !Ends && a.state ? load_floats<V>(a.state + row) : both(0.f), total = both(1.f);
   if (!Ends)
 #pragma unroll 4
-    for (int p = 0; p < at.piece; ++p)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 e = a.ends[p * rows + row + v];
-        start[v] = fmaf(e.x, start[v], e.y);
-      }
-
+    for (int p = 0; p < at.piece; ++p) {
+      const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
+      start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
+    }
   const int stop = min(at.last, at.len);  // tiles from here on are behind the row's end
   Raw<T, V> xn[L], gn[L], in[L];
   auto fetch = [&](int t0) {
-#pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const int t = t0 + seg * L + j;
-      const bool ok = at.ok && t < stop;
-      xn[j] = load_if<T, V>(ok, a.x.at(t, at.n) + d);
-      gn[j] = load_if<T, V>(ok, a.gate.at(t, at.n) + d);
-      if (In) in[j] = load_if<T, V>(ok, a.inner.at(t, at.n) + d);
-    }
+    const bool whole = t0 + TT <= stop;
+    fetch_steps<L, T, V>(xn, a.x, t0 + seg * L, at.n, d, stop, whole);
+    fetch_steps<L, T, V>(gn, a.gate, t0 + seg * L, at.n, d, stop, whole);
+    if (In) fetch_steps<L, T, V>(in, a.inner, t0 + seg * L, at.n, d, stop, whole);
   };
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = start[v];
-  fetch(at.first);
+  float2 h = start;
+  if (at.first < stop) fetch(at.first);
   int k = 0;
   for (int t0 = at.first; t0 < stop; t0 += TT, ++k) {
-    float s[L][V], b[L][V];
+    const int ts = t0 + seg * L;
+    float2 s[L], b[L], p, e;
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float x[V], g[V], i[V];
-      unpack<T, V>(xn[j], x);
-      unpack<T, V>(gn[j], g);
-      if (In) unpack<T, V>(in[j], i);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Step<Decay> step(Gate(g[v]), decay[v]);
-        s[j][v] = step.a;
-        b[j][v] = step.w * (In ? x[v] * sigmoid(i[v]) : x[v]);
+      float2 w;
+      if constexpr (Decay) {
+        float2 n;
+        decays<V>(__fmul2_rn(decay, sigmoids<V>(pair_of<T, V>(gn[j]))), far, s[j], n);
+        w = each<V>(__ffma2_rn(n, s[j], n), [](float x) { return sqrt_fast(-x); });  // 1 - a^2 = -n (1 + a)
+      } else {
+        float2 r;
+        sigmoids<V>(pair_of<T, V>(gn[j]), r, w);
+        s[j] = kept(r, w);
       }
+      b[j] = __fmul2_rn(w, pair_of<T, V>(xn[j]));
+      if (In) b[j] = __fmul2_rn(b[j], sigmoids<V>(pair_of<T, V>(in[j])));
     }
     if (t0 + TT > stop)
 #pragma unroll
       for (int j = 0; j < L; ++j)
-        if (t0 + seg * L + j >= stop)
-#pragma unroll
-          for (int v = 0; v < V; ++v) s[j][v] = 1.f, b[j][v] = 0.f;
+        if (ts + j >= stop) s[j] = both(1.f), b[j] = both(0.f);
     if (t0 + TT < stop) fetch(t0 + TT);
+    p = s[0];
+    e = b[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float p = s[0][v], e = b[0][v];
-#pragma unroll
-      for (int j = 1; j < L; ++j) {
-        e = fmaf(s[j][v], e, b[j][v]);
-        p *= s[j][v];
-      }
-      pairs[k & 1][seg][v][lane] = make_float2(p, e);
+    for (int j = 1; j < L; ++j) {
+      e = __ffma2_rn(s[j], e, b[j]);
+      p = __fmul2_rn(p, s[j]);
     }
+    pairs[k & 1][seg][lane] = make_float4(p.x, p.y, e.x, e.y);
     __syncthreads();
     if constexpr (Ends) {
       if (seg == 0)
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int q = 0; q < SEG; ++q) {
-            const float2 e = pairs[k & 1][q][v][lane];
-            h[v] = fmaf(e.x, h[v], e.y);
-            total[v] *= e.x;
-          }
+        for (int q = 0; q < SEG; ++q) {
+          const float4 w = pairs[k & 1][q][lane];
+          h = __ffma2_rn(make_float2(w.x, w.y), h, make_float2(w.z, w.w));
+          total = __fmul2_rn(total, make_float2(w.x, w.y));
+        }
     } else {
+      h = k ? behind[(k - 1) & 1][lane] : start;
+      for (int q = 0; q < seg; ++q) {
+        const float4 w = pairs[k & 1][q][lane];
+        h = __ffma2_rn(make_float2(w.x, w.y), h, make_float2(w.z, w.w));
+      }
+      if (a.checkpoints && seg * L % CKPT == 0 && at.ok && ts < at.last) store_floats<V>(a.checkpoints + ts / CKPT * rows + row, h);
+      T* y = a.y.at(ts, at.n) + d;
+      if (t0 + TT <= stop) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        h[v] = k ? behind[(k - 1) & 1][v][lane] : start[v];
-        for (int q = 0; q < seg; ++q) {
-          const float2 e = pairs[k & 1][q][v][lane];
-          h[v] = fmaf(e.x, h[v], e.y);
+        for (int j = 0; j < L; ++j) {
+          h = __ffma2_rn(s[j], h, b[j]);
+          if (at.ok) store_pair<T, V>(y + (long long)j * a.y.t, h);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          h = __ffma2_rn(s[j], h, b[j]);
+          if (at.ok && ts + j < at.last) store_pair<T, V>(y + (long long)j * a.y.t, ts + j < stop ? h : both(0.f));
         }
       }
-      const int ts = t0 + seg * L;
-      if (a.checkpoints && seg * L % CKPT == 0 && at.ok && ts < at.last)
-#pragma unroll
-        for (int v = 0; v < V; ++v) a.checkpoints[ts / CKPT * rows + row + v] = h[v];
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float y[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          h[v] = fmaf(s[j][v], h[v], b[j][v]);
-          y[v] = ts + j < stop ? h[v] : 0.f;
-        }
-        if (at.ok && ts + j < at.last) store<T, V>(a.y.at(ts + j, at.n) + d, y);
-      }
-      if (seg == SEG - 1)
-#pragma unroll
-        for (int v = 0; v < V; ++v) behind[k & 1][v][lane] = h[v];
+      if (seg == SEG - 1) behind[k & 1][lane] = h;
     }
   }
   if (!at.ok) return;
   if constexpr (Ends) {
-    if (seg == 0)
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.ends[at.piece * rows + row + v] = make_float2(total[v], h[v]);
+    if (seg == 0) {
+      float2* e = a.ends + at.piece * rows + row;
+      e[0] = make_float2(total.x, h.x);
+      if (V == 2) e[V - 1] = make_float2(total.y, h.y);
+    }
   } else {
-    const float none[V] = {};
-    for (int t = at.first + k * TT + seg; t < at.last; t += SEG) store<T, V>(a.y.at(t, at.n) + d, none);
-    if (a.final_state && at.piece == a.pieces - 1 && seg == SEG - 1)
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.final_state[row + v] = h[v];
+    for (int t = at.first + k * TT + seg; t < at.last; t += SEG) store_pair<T, V>(a.y.at(t, at.n) + d, both(0.f));
+    if (a.final_state && at.piece == a.pieces - 1 && seg == SEG - 1) store_floats<V>(a.final_state + row, h);
   }
 }
 
@@ -269,20 +319,22 @@ __global__ void __launch_bounds__(256) gated_step(Args<T> a) {
   const Raw<T, V> xr = load_if<T, V>(live, a.x.at(0, n) + d), gr = load_if<T, V>(live, a.gate.at(0, n) + d),
                   ir = load_if<T, V>(live && a.inner.p, a.inner.at(0, n) + d);
   const long long row = (long long)n * a.D + d;
-  float h[V], x[V], g[V], in[V], y[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = a.state ? a.state[row + v] : 0.f;
-  unpack<T, V>(xr, x);
-  unpack<T, V>(gr, g);
-  unpack<T, V>(ir, in);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const Step<Decay> step(Gate(g[v]), decay_of<Decay>(a.decay, d + v, true));
-    if (live) h[v] = fmaf(step.a, h[v], step.w * (a.inner.p ? x[v] * sigmoid(in[v]) : x[v]));
-    y[v] = live ? h[v] : 0.f;
-    if (a.final_state) a.final_state[row + v] = h[v];
+  float2 h = a.state ? load_floats<V>(a.state + row) : both(0.f), w, s;
+  const float2 decay = decay_of<Decay, V>(a.decay, d);
+  if constexpr (Decay) {
+    float2 m;
+    decays<V>(__fmul2_rn(decay, sigmoids<V>(pair_of<T, V>(gr))), true, s, m);
+    w = each<V>(__ffma2_rn(m, s, m), [](float x) { return sqrt_fast(-x); });
+  } else {
+    float2 r;
+    sigmoids<V>(pair_of<T, V>(gr), r, w);
+    s = kept(r, w);
   }
-  store<T, V>(a.y.at(0, n) + d, y);
+  float2 b = __fmul2_rn(w, pair_of<T, V>(xr));
+  if (a.inner.p) b = __fmul2_rn(b, sigmoids<V>(pair_of<T, V>(ir)));
+  if (live) h = __ffma2_rn(s, h, b);
+  if (a.final_state) store_floats<V>(a.final_state + row, h);
+  store_pair<T, V>(a.y.at(0, n) + d, live ? h : both(0.f));
 }
 
 // ------------------------------------------------------------------ backward
@@ -293,190 +345,174 @@ __global__ void __launch_bounds__(256) gated_step(Args<T> a) {
 template <typename T, int V, bool Decay, bool In, bool Ends>
 __global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
   constexpr int L = BWD_L, TT = BWD_TT;
-  __shared__ float2 pairs[2][SEG][V][32];
-  __shared__ float backs[2][SEG][V][32];
-  __shared__ float before[2][V][32];
+  __shared__ float4 pairs[2][SEG][32];
+  __shared__ float2 backs[2][SEG][32];
+  __shared__ float2 before[2][32];
   const Place<V> at(a);
   const int lane = threadIdx.x % 32, seg = threadIdx.x / 32;
-  const int d = at.ok ? at.d : 0;
+  const int d = at.ok ? at.d : a.D - V;
   const long long rows = (long long)a.N * a.D, row = (long long)at.n * a.D + d;
-  float decay[V], start[V], total[V], mu[V], sum[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    decay[v] = decay_of<Decay>(a.decay, d + v, at.ok);
-    start[v] = !Ends && at.ok && a.dfinal ? a.dfinal[row + v] : 0.f;
-    total[v] = 1.f;
-    sum[v] = 0.f;
-  }
+  const float2 decay = decay_of<Decay, V>(a.decay, d);
+  const bool far = goes_far(decay);
+  // (dlog_a / ddecay is r; in units of log(2) it is r too, and dlog_a has no units of its own)
+  const float2 natural = __fmul2_rn(decay, both(0.6931471805599453f));
+  // (a channel whose decay is zero adds nothing to its state: w, whose slope has no value there, counts as constant)
+  const float2 moves = make_float2(decay.x != 0.f ? -1.f : 0.f, decay.y != 0.f ? -1.f : 0.f);
+  float2 start = !Ends && a.dfinal ? load_floats<V>(a.dfinal + row) : both(0.f), total = both(1.f), sum = both(0.f);
   if (!Ends)
 #pragma unroll 4
-    for (int p = a.pieces - 1; p > at.piece; --p)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 e = a.ends[p * rows + row + v];
-        start[v] = fmaf(e.x, start[v], e.y);
-      }
-#pragma unroll
-  for (int v = 0; v < V; ++v) mu[v] = start[v];
+    for (int p = a.pieces - 1; p > at.piece; --p) {
+      const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
+      start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
+    }
+  float2 mu = start;
 
   const int stop = min(at.last, at.len);
   const int tiles = stop > at.first ? (stop - at.first + TT - 1) / TT : 0;
   Raw<T, V> xn[L], gn[L], in[L], yn[L];
-  float hn[V];
+  float2 hn = both(0.f);
   auto fetch = [&](int t0) {
-#pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const int t = t0 + seg * L + j;
-      const bool ok = at.ok && t < stop;
-      if (!Ends) xn[j] = load_if<T, V>(ok, a.x.at(t, at.n) + d);
-      gn[j] = load_if<T, V>(ok, a.gate.at(t, at.n) + d);
-      if (In && !Ends) in[j] = load_if<T, V>(ok, a.inner.at(t, at.n) + d);
-      yn[j] = load_if<T, V>(ok, a.dy.at(t, at.n) + d);
-    }
-    if (!Ends)
-#pragma unroll
-      for (int v = 0; v < V; ++v) hn[v] = at.ok ? a.checkpoints[t0 / CKPT * rows + row + v] : 0.f;
+    const bool whole = t0 + TT <= stop;
+    fetch_steps<L, T, V>(gn, a.gate, t0 + seg * L, at.n, d, stop, whole);
+    fetch_steps<L, T, V>(yn, a.dy, t0 + seg * L, at.n, d, stop, whole);
+    if (Ends) return;
+    fetch_steps<L, T, V>(xn, a.x, t0 + seg * L, at.n, d, stop, whole);
+    if (In) fetch_steps<L, T, V>(in, a.inner, t0 + seg * L, at.n, d, stop, whole);
+    hn = load_floats<V>(a.checkpoints + t0 / CKPT * rows + row);
   };
   if (tiles) fetch(at.first + (tiles - 1) * TT);
   if constexpr (!Ends) {
-    const float none[V] = {};
     if (at.ok)
       for (int t = at.first + tiles * TT + seg; t < at.last; t += SEG) {
-        store<T, V>(a.dx.at(t, at.n) + d, none);
-        store<T, V>(a.dgate.at(t, at.n) + d, none);
-        if (In) store<T, V>(a.dinner.at(t, at.n) + d, none);
+        store_pair<T, V>(a.dx.at(t, at.n) + d, both(0.f));
+        store_pair<T, V>(a.dgate.at(t, at.n) + d, both(0.f));
+        if (In) store_pair<T, V>(a.dinner.at(t, at.n) + d, both(0.f));
       }
   }
   for (int k = 0; k < tiles; ++k) {
     const int t0 = at.first + (tiles - 1 - k) * TT, ts = t0 + seg * L;
     const bool whole = t0 + TT <= stop;
-    float x[L][V], s[L][V], dy[L][V], i[L][V], islope[L][V], w[L][V], over[L][V], r[L][V], slope[L][V], h[V];
+    // b: what a step adds to the state; wi: w sigmoid(i); c: -u a / w (without decay -u); r, rest: the gate's sigmoid and
+    // (with decay) decay (1 - r); irest: 1 - sigmoid(i)
+    float2 s[L], b[L], wi[L], c[L], r[L], rest[L], irest[L], dy[L], h;
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float g[V];
-      unpack<T, V>(gn[j], g);
-      unpack<T, V>(yn[j], dy[j]);
-      if (!Ends) unpack<T, V>(xn[j], x[j]);
-      if (In && !Ends) unpack<T, V>(in[j], i[j]);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Gate gate(g[v]);
-        const Step<Decay> step(gate, decay[v]);
-        s[j][v] = step.a;
-        w[j][v] = step.w;
-        over[j][v] = step.over;
-        r[j][v] = gate.r;
-        slope[j][v] = gate.slope;
-        if (In && !Ends) {
-          const Gate inner(i[j][v]);
-          i[j][v] = inner.r;
-          islope[j][v] = inner.slope;
-        } else {
-          i[j][v] = 1.f;
-          islope[j][v] = 0.f;
-        }
+      float2 w;
+      dy[j] = pair_of<T, V>(yn[j]);
+      if constexpr (Decay) {
+        float2 n;
+        sigmoids<V>(pair_of<T, V>(gn[j]), r[j], rest[j]);
+        decays<V>(__fmul2_rn(decay, r[j]), far, s[j], n);
+        if (Ends) continue;
+        const float2 v = __ffma2_rn(n, s[j], n);  // a^2 - 1
+        const float2 over = each<V>(v, [](float x) { return rsqrt_fast(at_least(-x, 0x1p-126f)); });
+        w = __fmul2_rn(__fmul2_rn(v, both(-1.f)), over);
+        c[j] = __fmul2_rn(__fmul2_rn(s[j], moves), over);
+        rest[j] = __fmul2_rn(rest[j], natural);
+      } else {
+        sigmoids<V>(pair_of<T, V>(gn[j]), r[j], w);
+        s[j] = kept(r[j], w);
+        if (Ends) continue;
+        c[j] = both(-1.f);
+        rest[j] = w;
       }
+      const float2 x = pair_of<T, V>(xn[j]);
+      float2 u = x;
+      wi[j] = w;
+      if (In) {
+        float2 i;
+        sigmoids<V>(pair_of<T, V>(in[j]), i, irest[j]);
+        u = __fmul2_rn(x, i);
+        wi[j] = __fmul2_rn(w, i);
+      }
+      b[j] = __fmul2_rn(w, u);
+      c[j] = __fmul2_rn(c[j], u);
     }
     if (!whole)
 #pragma unroll
       for (int j = 0; j < L; ++j)
-        if (ts + j >= stop)
-#pragma unroll
-          for (int v = 0; v < V; ++v) s[j][v] = 1.f, w[j][v] = 0.f;  // (x and dy are zeros)
-    if (!Ends)
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = hn[v];
+        if (ts + j >= stop) s[j] = both(1.f), b[j] = both(0.f);  // (dy is zero)
+    if (!Ends) h = hn;
     if (k + 1 < tiles) fetch(t0 - TT);
+    float2 p = s[0], e = both(0.f), m = both(0.f);
+    if (!Ends) e = b[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float p = 1.f, e = 0.f, m = 0.f;
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        if (!Ends) e = fmaf(s[j][v], e, w[j][v] * (x[j][v] * i[j][v]));
-        p *= s[j][v];
-        m = s[L - 1 - j][v] * (dy[L - 1 - j][v] + m);
-      }
-      pairs[k & 1][seg][v][lane] = make_float2(p, e);
-      backs[k & 1][seg][v][lane] = m;
+    for (int j = 1; j < L; ++j) {
+      if (!Ends) e = __ffma2_rn(s[j], e, b[j]);
+      p = __fmul2_rn(p, s[j]);
     }
+#pragma unroll
+    for (int j = L - 1; j >= 0; --j) m = __fmul2_rn(s[j], __fadd2_rn(dy[j], m));
+    pairs[k & 1][seg][lane] = make_float4(p.x, p.y, e.x, e.y);
+    backs[k & 1][seg][lane] = m;
     __syncthreads();
     if constexpr (Ends) {
       if (seg == 0)
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int q = SEG - 1; q >= 0; --q) {
-            const float p = pairs[k & 1][q][v][lane].x;
-            mu[v] = fmaf(p, mu[v], backs[k & 1][q][v][lane]);
-            total[v] *= p;
-          }
+        for (int q = SEG - 1; q >= 0; --q) {
+          const float4 w = pairs[k & 1][q][lane];
+          mu = __ffma2_rn(make_float2(w.x, w.y), mu, backs[k & 1][q][lane]);
+          total = __fmul2_rn(total, make_float2(w.x, w.y));
+        }
     } else {
-      float hs[L][V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        for (int q = 0; q < seg; ++q) {
-          const float2 e = pairs[k & 1][q][v][lane];
-          h[v] = fmaf(e.x, h[v], e.y);
-        }
-        mu[v] = k ? before[(k - 1) & 1][v][lane] : start[v];
-        for (int q = SEG - 1; q > seg; --q) mu[v] = fmaf(pairs[k & 1][q][v][lane].x, mu[v], backs[k & 1][q][v][lane]);
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-          hs[j][v] = h[v];
-          h[v] = fmaf(s[j][v], h[v], w[j][v] * (x[j][v] * i[j][v]));
-        }
+      for (int q = 0; q < seg; ++q) {
+        const float4 w = pairs[k & 1][q][lane];
+        h = __ffma2_rn(make_float2(w.x, w.y), h, make_float2(w.z, w.w));
       }
+      mu = k ? before[(k - 1) & 1][lane] : start;
+      for (int q = SEG - 1; q > seg; --q) {
+        const float4 w = pairs[k & 1][q][lane];
+        mu = __ffma2_rn(make_float2(w.x, w.y), mu, backs[k & 1][q][lane]);
+      }
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        c[j] = __fadd2_rn(c[j], h);  // h_{t-1} - u a / w
+        h = __ffma2_rn(s[j], h, b[j]);
+      }
+      T *px = a.dx.at(ts, at.n) + d, *pg = a.dgate.at(ts, at.n) + d, *pi = In ? a.dinner.at(ts, at.n) + d : nullptr;
 #pragma unroll
       for (int j = L - 1; j >= 0; --j) {
-        float dx[V], dg[V], di[V];
-        const bool live = ts + j < stop;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float lam = dy[j][v] + mu[v], u = x[j][v] * i[j][v], lw = lam * w[j][v];
-          if (Decay) {
-            const float dl = lam * (s[j][v] * (hs[j][v] - u * (s[j][v] * over[j][v])));
-            dg[v] = dl * (decay[v] * slope[j][v]);
-            sum[v] = live ? fmaf(dl, r[j][v], sum[v]) : sum[v];
-          } else {
-            dg[v] = lam * (hs[j][v] - u) * slope[j][v];
-          }
-          dx[v] = lw * i[j][v];
-          di[v] = lw * x[j][v] * islope[j][v];
-          mu[v] = s[j][v] * lam;
-          if (!live) dx[v] = dg[v] = di[v] = 0.f;
+        const bool live = whole || ts + j < stop;
+        const float2 lam = __fadd2_rn(dy[j], mu);
+        mu = __fmul2_rn(lam, s[j]);
+        float2 dx = __fmul2_rn(lam, wi[j]), dg, di;
+        if (Decay) {
+          const float2 by_decay = __fmul2_rn(__fmul2_rn(mu, c[j]), r[j]);
+          dg = __fmul2_rn(by_decay, rest[j]);
+          sum = __fadd2_rn(sum, live ? by_decay : both(0.f));
+        } else {
+          dg = __fmul2_rn(__fmul2_rn(mu, c[j]), rest[j]);
         }
-        if (at.ok && ts + j < at.last) {
-          store<T, V>(a.dx.at(ts + j, at.n) + d, dx);
-          store<T, V>(a.dgate.at(ts + j, at.n) + d, dg);
-          if (In) store<T, V>(a.dinner.at(ts + j, at.n) + d, di);
+        if (In) di = __fmul2_rn(__fmul2_rn(lam, b[j]), irest[j]);
+        if (!live) dx = dg = di = both(0.f);
+        if (at.ok && (whole || ts + j < at.last)) {
+          store_pair<T, V>(px + (long long)j * a.dx.t, dx);
+          store_pair<T, V>(pg + (long long)j * a.dgate.t, dg);
+          if (In) store_pair<T, V>(pi + (long long)j * a.dinner.t, di);
         }
       }
-      if (seg == 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) before[k & 1][v][lane] = mu[v];
+      if (seg == 0) before[k & 1][lane] = mu;
     }
   }
   if constexpr (Ends) {
-    if (seg == 0 && at.ok)
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.ends[at.piece * rows + row + v] = make_float2(total[v], mu[v]);
+    if (seg == 0 && at.ok) {
+      float2* e = a.ends + at.piece * rows + row;
+      e[0] = make_float2(total.x, mu.x);
+      if (V == 2) e[V - 1] = make_float2(total.y, mu.y);
+    }
   } else {
-    if (a.dstate && at.piece == 0 && seg == 0 && at.ok)
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.dstate[row + v] = mu[v];
+    if (a.dstate && at.piece == 0 && seg == 0 && at.ok) store_floats<V>(a.dstate + row, mu);
     if constexpr (Decay) {
       __syncthreads();  // the last tile's numbers have been read
-#pragma unroll
-      for (int v = 0; v < V; ++v) backs[0][seg][v][lane] = sum[v];
+      backs[0][seg][lane] = sum;
       __syncthreads();
-      if (seg == 0 && at.ok)
+      if (seg == 0 && at.ok) {
+        float2 s = backs[0][0][lane];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float s = backs[0][0][v][lane];
-#pragma unroll
-          for (int q = 1; q < SEG; ++q) s += backs[0][q][v][lane];
-          a.part[at.piece * rows + row + v] = a.decay[d + v] > 0.f ? 0.f : s;
-        }
+        for (int q = 1; q < SEG; ++q) s = __fadd2_rn(s, backs[0][q][lane]);
+        const float2 raw = load_floats<V>(a.decay + d);
+        store_floats<V>(a.part + at.piece * rows + row, make_float2(raw.x > 0.f ? 0.f : s.x, raw.y > 0.f ? 0.f : s.y));
+      }
     }
   }
 }
@@ -489,7 +525,7 @@ inline int pieces_of(const haste_b200_gated_scan& a, int V, int tile) {
   const long long most = a.T / (2 * tile), want = (4LL * sm_count() + blocks - 1) / blocks;
   return (int)std::max(1LL, std::min(most, want));
 }
-// (Scratch is asked for before the pointers are there: whole words are one channel a lane or two, so the most of both.)
+// (Scratch is asked for before the pointers are there, which decide on one channel a lane or two: the most of both.)
 inline int most_pieces(const haste_b200_gated_scan& a, int tile) {
   return std::max(pieces_of(a, 1, tile), pieces_of(a, 2, tile));
 }
@@ -510,10 +546,10 @@ Args<T> pack(const haste_b200_gated_scan& a, int V) {
   return k;
 }
 template <typename T>
-bool words(const haste_b200_gated_scan& a) {
-  if (sizeof(T) == 4 || a.D % 2) return false;
+bool in_pairs(const haste_b200_gated_scan& a) {
+  if (a.D % 2) return false;
   for (const haste_b200_sequence* q : {&a.x, &a.gate, &a.input_gate, &a.y, &a.dy, &a.dx, &a.dgate, &a.dinput_gate})
-    if (!aligned(*q, sizeof(T), 4)) return false;
+    if (!aligned(*q, sizeof(T), 2 * sizeof(T))) return false;
   return true;
 }
 
@@ -597,8 +633,7 @@ int run_gates(const haste_b200_gated_scan& a, bool backward, cudaStream_t s) {
 // One definition per storage type, each in a file of its own.
 template <typename T>
 int run(const haste_b200_gated_scan& a, bool backward, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2)
-    if (words<T>(a)) return run_gates<T, 2>(a, backward, s);
+  if (in_pairs<T>(a)) return run_gates<T, 2>(a, backward, s);
   return run_gates<T, 1>(a, backward, s);
 }
 

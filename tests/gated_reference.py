@@ -61,8 +61,9 @@ def gated_scan(x, gate, decay=None, input_gate=None, state=None, lengths=None, d
         w = torch.sqrt(m * (1 + a))
         ew = 0.5 * (torch.where(m > 0, dm / m, 0.0) + da / (1 + a) + 2 * U) + 4 * U
         over = torch.where(w > 0, 1 / w, 0.0)
-        # An exponential below 2^-126 is flushed to zero, and with it w = sqrt(-2 decay r) to first order: all of w is lost.
-        lost = torch.where(r < 2.0 ** -125, w, 0.0)
+        # Where r is below 2^-125 it may come out as zero or as that: w = sqrt(-2 decay r) to first order is off by the most
+        # that it is there.
+        lost = torch.where(r < 2.0 ** -124, torch.sqrt(-2 * dec * 2.0 ** -124), 0.0)
     else:
         lost = 0.0
         a, w = r, rest
@@ -76,8 +77,9 @@ def gated_scan(x, gate, decay=None, input_gate=None, state=None, lengths=None, d
     u, eu = x * i, (ki + 1) * U
     b = torch.where(live, w * u, 0.0)
     eb = ew + eu + U
-    lost = torch.where(live, lost * u.abs(), 0.0)
-    a, da = torch.where(live, a, 1.0), torch.where(live, da, 0.0)
+    # a sigmoid below 2^-125 may come out as zero or as that: both factors of a step are off by as much
+    lost = torch.where(live, lost * u.abs() + 2.0 ** -124 * x.abs(), 0.0)
+    a, da = torch.where(live, a, 1.0), torch.where(live, da + 2.0 ** -125, 0.0)
     three = torch.where(live, 3 * U, 0.0)
     h = torch.zeros(N, D, dtype=torch.float64) if state is None else state
     E, H = torch.zeros_like(h), h.abs()
