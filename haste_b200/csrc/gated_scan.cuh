@@ -24,12 +24,9 @@ namespace gated {
 
 using namespace ss;
 
-constexpr int THREADS = 256, SEG = THREADS / 32;  // a warp walks one of the tile's segments
-#ifndef HB_FWD_L
-#define HB_FWD_L 8
-#define HB_FWD_B 2
-#endif
-constexpr int FWD_L = HB_FWD_L, BWD_L = 4, FWD_BLOCKS = HB_FWD_B;               // steps of a segment
+constexpr int THREADS = 128, SEG = THREADS / 32;  // a warp walks one of the tile's segments
+constexpr int FWD_L = 4, BWD_L = 4;               // steps of a segment
+constexpr int FWD_BLOCKS = 7, BWD_BLOCKS = 4;     // of an SM, as registers allow
 constexpr int FWD_TT = SEG * FWD_L, BWD_TT = SEG * BWD_L;
 constexpr int CKPT = BWD_TT;                      // steps between the states left for the backward pass
 
@@ -86,11 +83,6 @@ __device__ __forceinline__ float at_most(float v, float most) {  // (a NaN stays
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
   return r;
 }
-__device__ __forceinline__ float at_least(float v, float least) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(least));
-  return r;
-}
 template <int V, typename F>
 __device__ __forceinline__ float2 each(float2 v, const F& f) {
   return make_float2(f(v.x), V == 2 ? f(v.y) : 0.f);
@@ -117,32 +109,48 @@ __device__ __forceinline__ void store_floats(float* p, float2 v) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
+// (Where a factor is a number, the two channels take an instruction each: the number is part of it, where an instruction for
+// two wants it in registers.)
+
 // r = sigmoid(v) and 1 - r, each to its own last bits; exponentials above 2^125 are held there, so that 1 - r, which is
 // their product with r, stays one.
 template <int V>
 __device__ __forceinline__ void sigmoids(float2 v, float2& r, float2& rest) {
-  const float2 e = each<V>(__fmul2_rn(v, both(-LOG2E)), [](float x) { return at_most(exp2_fast(x), 0x1p125f); });
-  r = each<V>(__fadd2_rn(e, both(1.f)), [](float x) { return reciprocal(x); });
+  const float2 e = each<V>(v, [](float x) { return at_most(exp2_fast(x * -LOG2E), 0x1p125f); });
+  r = each<V>(e, [](float x) { return reciprocal(x + 1.f); });
   rest = __fmul2_rn(e, r);
 }
 template <int V>
 __device__ __forceinline__ float2 sigmoids(float2 v) {
-  const float2 e = each<V>(__fmul2_rn(v, both(-LOG2E)), [](float x) { return exp2_fast(x); });
-  return each<V>(__fadd2_rn(e, both(1.f)), [](float x) { return reciprocal(x); });
+  return each<V>(v, [](float x) { return sigmoid(x); });
 }
-// 2^l for l <= 0 less one, n, and a = 1 + n.  A decay lies next to one, where the special function unit's results are low by
-// 2.4e-8 on average; a state that keeps 1 / (1 - a) steps would add that up.  So n is computed to its own last bits (the
-// exponential's series, where a is above 0.7; `far`: some of the block's channels may go below), and a rounded
-// once, to either side.
-template <int V>
-__device__ __forceinline__ void decays(float2 l, bool far, float2& a, float2& n) {
+// 2^l - 1 for l from -0.505 to 0: the exponential's series.
+__device__ __forceinline__ constexpr float series(int k) {  // ln(2)^(7 - k) / (7 - k)!
   constexpr float c[] = {1.5252733804059840e-05f, 1.5403530393381608e-04f, 1.3333558146428441e-03f, 9.6181291076284772e-03f,
-                         5.5504108664821576e-02f, 2.4022650695910069e-01f, 6.9314718055994529e-01f};  // ln(2)^k / k!
-  float2 p = both(c[0]);
+                         5.5504108664821576e-02f, 2.4022650695910069e-01f, 6.9314718055994529e-01f};
+  return c[k];
+}
+__device__ __forceinline__ float exp2_less_one(float l) {
+  float p = series(0);
 #pragma unroll
-  for (int k = 1; k < 7; ++k) p = __ffma2_rn(p, l, both(c[k]));
-  n = __fmul2_rn(p, l);
-  a = __fadd2_rn(n, both(1.f));
+  for (int k = 1; k < 7; ++k) p = fmaf(p, l, series(k));
+  return p * l;
+}
+// a = 2^l for l <= 0, and a - 1.  A decay lies next to one, where the special function unit's results are low by
+// 2.4e-8 on average; a state that keeps 1 / (1 - a) steps would add that up.  So a - 1 is computed to its own last bits
+// (where a is above 0.7; `far`: some of the block's channels may go below), and a rounded once, to either side.
+// Packed: the series' numbers lie in registers, of which the forward pass has enough.
+template <int V, bool Packed>
+__device__ __forceinline__ void decays(float2 l, bool far, float2& a, float2& n) {
+  if constexpr (Packed) {
+    float2 p = both(series(0));
+#pragma unroll
+    for (int k = 1; k < 7; ++k) p = __ffma2_rn(p, l, both(series(k)));
+    n = __fmul2_rn(p, l);
+  } else {
+    n = each<V>(l, [](float x) { return exp2_less_one(x); });
+  }
+  a = make_float2(n.x + 1.f, n.y + 1.f);
   if (far) {
     const float2 e = each<V>(l, [](float x) { return exp2_fast(x); });
     const bool x = l.x < -0.505f, y = l.y < -0.505f;
@@ -152,8 +160,7 @@ __device__ __forceinline__ void decays(float2 l, bool far, float2& a, float2& n)
 }
 // Without decay: a = r, rounded once to either side where it is near one.
 __device__ __forceinline__ float2 kept(float2 r, float2 rest) {
-  const float2 a = __ffma2_rn(rest, both(-1.f), both(1.f));
-  return make_float2(r.x > 0.5f ? a.x : r.x, r.y > 0.5f ? a.y : r.y);
+  return make_float2(r.x > 0.5f ? 1.f - rest.x : r.x, r.y > 0.5f ? 1.f - rest.y : r.y);
 }
 
 // A channel's decay in units of log(2): values above zero count as zero, so that no state grows.
@@ -164,6 +171,16 @@ __device__ __forceinline__ float2 decay_of(const float* decay, int d) {
 }
 __device__ __forceinline__ bool goes_far(float2 decay) { return __any_sync(0xffffffffu, decay.x < -0.5f || decay.y < -0.5f); }
 
+// A thread's place in a sequence, which it walks tile by tile: one addition each, where an address anew is two products.
+template <typename T>
+struct Walk {
+  T* p;
+  long long by;
+  int t;
+  __device__ __forceinline__ Walk(const Seq<T>& q, int first, int n, int d, int steps) : p(q.at(first, n) + d), by((long long)steps * q.t), t(q.t) {}
+  __device__ __forceinline__ void next() { p += by; }
+  __device__ __forceinline__ T* at(int j) const { return p + (long long)j * t; }
+};
 // A load that needs no predicate.
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
@@ -180,25 +197,28 @@ __device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
   }
   return r;
 }
-// The steps of a segment, in front of `stop` where not all of a tile is.
-template <int L, typename T, int V>
-__device__ __forceinline__ void fetch_steps(Raw<T, V> (&r)[L], const Seq<const T>& q, int t, int n, int d, int stop, bool whole) {
-  const T* p = q.at(t, n) + d;
+// The steps of a segment, `left` of which exist where not all of the tile's do.
+template <int L, int V, typename T, typename U>
+__device__ __forceinline__ void fetch_steps(Raw<T, V> (&r)[L], Walk<U>& q, int left, bool whole) {
   if (whole) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) r[j] = load_raw<T, V>(p + (long long)j * q.t);
+    for (int j = 0; j < L; ++j) r[j] = load_raw<T, V>(q.at(j));
   } else {
 #pragma unroll
-    for (int j = 0; j < L; ++j) r[j] = load_if<T, V>(t + j < stop, p + (long long)j * q.t);
+    for (int j = 0; j < L; ++j) r[j] = load_if<T, V>(j < left, q.at(j));
   }
+  q.next();
 }
 
 // ------------------------------------------------------------------ forward
 // A block takes 64 neighbouring channels, two a lane (32, one a lane, where rows do not start on whole pairs), and tiles of
-// FWD_L steps to each of its eight warps.  A warp folds its steps into (product of decays, what they add to a state of
+// four steps to each of its four warps.  A warp folds its steps into (product of decays, what they add to a state of
 // zero), the warps' pairs meet in shared memory, each warp folds those in front of its own into the tile's starting state,
 // and walks its steps again from registers.  One barrier a tile: pairs and the state behind the tile have two buffers.
 // The next tile's words are under way from when the present ones have been used.
+// bf16 1000 x 64 x 1024 with both gates: 129 us, 4.1 TB/s; with the sigmoids, series and root left out 99 us, which is what
+// the accesses and barriers take.  Eight steps a warp and blocks of 256 threads 135 us (fewer instructions, but 3.5 blocks
+// an SM to share out); words copied to shared memory tiles ahead 142; one reciprocal for both gates 129.
 //
 // Few channels leave most of the GPU idle, so their sequences are cut into pieces and read twice (the second time from
 // L2): first (Ends) each piece but the last leaves its pair, then each piece starts from those in front of it.
@@ -215,18 +235,22 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
   const bool far = goes_far(decay);
   float2 start = !Ends && a.state ? load_floats<V>(a.state + row) : both(0.f), total = both(1.f);
   if (!Ends)
-#pragma unroll 4
+#pragma unroll 8
     for (int p = 0; p < at.piece; ++p) {
       const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
       start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
     }
   const int stop = min(at.last, at.len);  // tiles from here on are behind the row's end
+  const int ts0 = at.first + seg * L;
+  Walk<const T> px(a.x, ts0, at.n, d, TT), pg(a.gate, ts0, at.n, d, TT), pi(In ? a.inner : a.x, ts0, at.n, d, TT);
+  Walk<T> py(a.y, Ends ? 0 : ts0, at.n, d, TT);
   Raw<T, V> xn[L], gn[L], in[L];
   auto fetch = [&](int t0) {
     const bool whole = t0 + TT <= stop;
-    fetch_steps<L, T, V>(xn, a.x, t0 + seg * L, at.n, d, stop, whole);
-    fetch_steps<L, T, V>(gn, a.gate, t0 + seg * L, at.n, d, stop, whole);
-    if (In) fetch_steps<L, T, V>(in, a.inner, t0 + seg * L, at.n, d, stop, whole);
+    const int left = stop - t0 - seg * L;
+    fetch_steps<L>(xn, px, left, whole);
+    fetch_steps<L>(gn, pg, left, whole);
+    if (In) fetch_steps<L>(in, pi, left, whole);
   };
   float2 h = start;
   if (at.first < stop) fetch(at.first);
@@ -236,14 +260,15 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
     float2 s[L], b[L], p, e;
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float2 w;
+      float2 w, r, rest;
+      if constexpr (Decay) r = sigmoids<V>(pair_of<T, V>(gn[j]));
+      else sigmoids<V>(pair_of<T, V>(gn[j]), r, rest);
       if constexpr (Decay) {
         float2 n;
-        decays<V>(__fmul2_rn(decay, sigmoids<V>(pair_of<T, V>(gn[j]))), far, s[j], n);
+        decays<V, true>(__fmul2_rn(decay, r), far, s[j], n);
         w = each<V>(__ffma2_rn(n, s[j], n), [](float x) { return sqrt_fast(-x); });  // 1 - a^2 = -n (1 + a)
       } else {
-        float2 r;
-        sigmoids<V>(pair_of<T, V>(gn[j]), r, w);
+        w = rest;
         s[j] = kept(r, w);
       }
       b[j] = __fmul2_rn(w, pair_of<T, V>(xn[j]));
@@ -278,20 +303,20 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
         h = __ffma2_rn(make_float2(w.x, w.y), h, make_float2(w.z, w.w));
       }
       if (a.checkpoints && seg * L % CKPT == 0 && at.ok && ts < at.last) store_floats<V>(a.checkpoints + ts / CKPT * rows + row, h);
-      T* y = a.y.at(ts, at.n) + d;
       if (t0 + TT <= stop) {
 #pragma unroll
         for (int j = 0; j < L; ++j) {
           h = __ffma2_rn(s[j], h, b[j]);
-          if (at.ok) store_pair<T, V>(y + (long long)j * a.y.t, h);
+          if (at.ok) store_pair<T, V>(py.at(j), h);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < L; ++j) {
           h = __ffma2_rn(s[j], h, b[j]);
-          if (at.ok && ts + j < at.last) store_pair<T, V>(y + (long long)j * a.y.t, ts + j < stop ? h : both(0.f));
+          if (at.ok && ts + j < at.last) store_pair<T, V>(py.at(j), ts + j < stop ? h : both(0.f));
         }
       }
+      py.next();
       if (seg == SEG - 1) behind[k & 1][lane] = h;
     }
   }
@@ -323,7 +348,7 @@ __global__ void __launch_bounds__(256) gated_step(Args<T> a) {
   const float2 decay = decay_of<Decay, V>(a.decay, d);
   if constexpr (Decay) {
     float2 m;
-    decays<V>(__fmul2_rn(decay, sigmoids<V>(pair_of<T, V>(gr))), true, s, m);
+    decays<V, false>(__fmul2_rn(decay, sigmoids<V>(pair_of<T, V>(gr))), true, s, m);
     w = each<V>(__ffma2_rn(m, s, m), [](float x) { return sqrt_fast(-x); });
   } else {
     float2 r;
@@ -342,8 +367,10 @@ __global__ void __launch_bounds__(256) gated_step(Args<T> a) {
 // the one that the forward pass left in front of it; a segment is a pair for the states, and for the adjoint
 // mu = a lam, which runs the other way, the same product and a third number.
 // Ends: pieces but the first leave (product, mu that they give to one of zero behind them).
+// bf16 1000 x 64 x 1024 with both gates: 233 us, 3.9 TB/s, bound by what 16 warps an SM issue next to each other (0.6 of the
+// slots): a step's numbers fill 128 registers a thread.  Five blocks an SM spill (629 us), blocks of 256 threads 242.
 template <typename T, int V, bool Decay, bool In, bool Ends>
-__global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
+__global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
   constexpr int L = BWD_L, TT = BWD_TT;
   __shared__ float4 pairs[2][SEG][32];
   __shared__ float2 backs[2][SEG][32];
@@ -357,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
   // (dlog_a / ddecay is r; in units of log(2) it is r too, and dlog_a has no units of its own)
   const float2 natural = __fmul2_rn(decay, both(0.6931471805599453f));
   // (a channel whose decay is zero adds nothing to its state: w, whose slope has no value there, counts as constant)
-  const float2 moves = make_float2(decay.x != 0.f ? -1.f : 0.f, decay.y != 0.f ? -1.f : 0.f);
+  const float2 moves = make_float2(decay.x != 0.f ? 1.f : 0.f, decay.y != 0.f ? 1.f : 0.f);
   float2 start = !Ends && a.dfinal ? load_floats<V>(a.dfinal + row) : both(0.f), total = both(1.f), sum = both(0.f);
   if (!Ends)
-#pragma unroll 4
+#pragma unroll 8
     for (int p = a.pieces - 1; p > at.piece; --p) {
       const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
       start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
@@ -369,16 +396,24 @@ __global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
 
   const int stop = min(at.last, at.len);
   const int tiles = stop > at.first ? (stop - at.first + TT - 1) / TT : 0;
+  const int ts0 = at.first + max(tiles - 1, 0) * TT + seg * L;
+  Walk<const T> pg(a.gate, ts0, at.n, d, -TT), py(a.dy, ts0, at.n, d, -TT), px(a.x, ts0, at.n, d, -TT),
+      pi(In ? a.inner : a.x, ts0, at.n, d, -TT);
+  Walk<T> qx(a.dx, Ends ? 0 : ts0, at.n, d, -TT), qg(a.dgate, Ends ? 0 : ts0, at.n, d, -TT),
+      qi(In ? a.dinner : a.dx, Ends ? 0 : ts0, at.n, d, -TT);
+  const float* ph = a.checkpoints + (ts0 - seg * L) / CKPT * rows + row;
   Raw<T, V> xn[L], gn[L], in[L], yn[L];
   float2 hn = both(0.f);
   auto fetch = [&](int t0) {
     const bool whole = t0 + TT <= stop;
-    fetch_steps<L, T, V>(gn, a.gate, t0 + seg * L, at.n, d, stop, whole);
-    fetch_steps<L, T, V>(yn, a.dy, t0 + seg * L, at.n, d, stop, whole);
+    const int left = stop - t0 - seg * L;
+    fetch_steps<L>(gn, pg, left, whole);
+    fetch_steps<L>(yn, py, left, whole);
     if (Ends) return;
-    fetch_steps<L, T, V>(xn, a.x, t0 + seg * L, at.n, d, stop, whole);
-    if (In) fetch_steps<L, T, V>(in, a.inner, t0 + seg * L, at.n, d, stop, whole);
-    hn = load_floats<V>(a.checkpoints + t0 / CKPT * rows + row);
+    fetch_steps<L>(xn, px, left, whole);
+    if (In) fetch_steps<L>(in, pi, left, whole);
+    hn = load_floats<V>(ph);
+    ph -= rows;
   };
   if (tiles) fetch(at.first + (tiles - 1) * TT);
   if constexpr (!Ends) {
@@ -397,30 +432,29 @@ __global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
     float2 s[L], b[L], wi[L], c[L], r[L], rest[L], irest[L], dy[L], h;
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float2 w;
+      float2 w, i;
       dy[j] = pair_of<T, V>(yn[j]);
+      sigmoids<V>(pair_of<T, V>(gn[j]), r[j], rest[j]);
       if constexpr (Decay) {
         float2 n;
-        sigmoids<V>(pair_of<T, V>(gn[j]), r[j], rest[j]);
-        decays<V>(__fmul2_rn(decay, r[j]), far, s[j], n);
+        decays<V, false>(__fmul2_rn(decay, r[j]), far, s[j], n);
         if (Ends) continue;
         const float2 v = __ffma2_rn(n, s[j], n);  // a^2 - 1
-        const float2 over = each<V>(v, [](float x) { return rsqrt_fast(at_least(-x, 0x1p-126f)); });
-        w = __fmul2_rn(__fmul2_rn(v, both(-1.f)), over);
+        // (1 / w with 1e-30 added to w^2, so that it stays finite where w is zero)
+        const float2 over = each<V>(v, [](float x) { return -rsqrt_fast(1e-30f - x); });
+        w = __fmul2_rn(v, over);
         c[j] = __fmul2_rn(__fmul2_rn(s[j], moves), over);
         rest[j] = __fmul2_rn(rest[j], natural);
       } else {
-        sigmoids<V>(pair_of<T, V>(gn[j]), r[j], w);
+        w = rest[j];
         s[j] = kept(r[j], w);
         if (Ends) continue;
         c[j] = both(-1.f);
-        rest[j] = w;
       }
       const float2 x = pair_of<T, V>(xn[j]);
       float2 u = x;
       wi[j] = w;
       if (In) {
-        float2 i;
         sigmoids<V>(pair_of<T, V>(in[j]), i, irest[j]);
         u = __fmul2_rn(x, i);
         wi[j] = __fmul2_rn(w, i);
@@ -469,28 +503,33 @@ __global__ void __launch_bounds__(THREADS, 2) gated_bwd(Args<T> a) {
         c[j] = __fadd2_rn(c[j], h);  // h_{t-1} - u a / w
         h = __ffma2_rn(s[j], h, b[j]);
       }
-      T *px = a.dx.at(ts, at.n) + d, *pg = a.dgate.at(ts, at.n) + d, *pi = In ? a.dinner.at(ts, at.n) + d : nullptr;
+      auto gradients = [&](auto every) {  // every: all of the tile's steps are in front of the row's end
 #pragma unroll
-      for (int j = L - 1; j >= 0; --j) {
-        const bool live = whole || ts + j < stop;
-        const float2 lam = __fadd2_rn(dy[j], mu);
-        mu = __fmul2_rn(lam, s[j]);
-        float2 dx = __fmul2_rn(lam, wi[j]), dg, di;
-        if (Decay) {
-          const float2 by_decay = __fmul2_rn(__fmul2_rn(mu, c[j]), r[j]);
-          dg = __fmul2_rn(by_decay, rest[j]);
-          sum = __fadd2_rn(sum, live ? by_decay : both(0.f));
-        } else {
-          dg = __fmul2_rn(__fmul2_rn(mu, c[j]), rest[j]);
+        for (int j = L - 1; j >= 0; --j) {
+          const float2 lam = __fadd2_rn(dy[j], mu);
+          mu = __fmul2_rn(lam, s[j]);
+          float2 dx = __fmul2_rn(lam, wi[j]), dg, di = both(0.f), by_decay = both(0.f);
+          if (Decay) {
+            by_decay = __fmul2_rn(__fmul2_rn(mu, c[j]), r[j]);
+            dg = __fmul2_rn(by_decay, rest[j]);
+          } else {
+            dg = __fmul2_rn(__fmul2_rn(mu, c[j]), rest[j]);
+          }
+          if (In) di = __fmul2_rn(__fmul2_rn(lam, b[j]), irest[j]);
+          if (!every.value && ts + j >= stop) dx = dg = di = by_decay = both(0.f);
+          if (Decay) sum = __fadd2_rn(sum, by_decay);
+          if (at.ok && (every.value || ts + j < at.last)) {
+            store_pair<T, V>(qx.at(j), dx);
+            store_pair<T, V>(qg.at(j), dg);
+            if (In) store_pair<T, V>(qi.at(j), di);
+          }
         }
-        if (In) di = __fmul2_rn(__fmul2_rn(lam, b[j]), irest[j]);
-        if (!live) dx = dg = di = both(0.f);
-        if (at.ok && (whole || ts + j < at.last)) {
-          store_pair<T, V>(px + (long long)j * a.dx.t, dx);
-          store_pair<T, V>(pg + (long long)j * a.dgate.t, dg);
-          if (In) store_pair<T, V>(pi + (long long)j * a.dinner.t, di);
-        }
-      }
+      };
+      if (whole) gradients(std::true_type());
+      else gradients(std::false_type());
+      qx.next();
+      qg.next();
+      if (In) qi.next();
       if (seg == 0) before[k & 1][lane] = mu;
     }
   }

@@ -238,8 +238,11 @@ def test_more_elements_than_32_bits_count():
     y, final = ssm.gated_scan(x, gate)
     y2, final2 = ssm.gated_scan(x[-256:], gate[-256:])
     # 0.047^64 is far below a rounding.  The two calls' tiles start at other steps, so sums are associated in another order:
-    # three roundings a step of terms that add up to less than 1 / (1 - 0.05), in either
-    assert torch.equal(y[-192:], y2[-192:]) and (final - final2).abs().max() < 2 * 3 * 1.06 * ref.U
+    # three roundings a step of terms that add up to less than 1 / (1 - 0.05), in either, and each y is rounded by itself
+    apart = 2 * 3 * 1.06 * ref.U
+    assert (final - final2).abs().max() < apart
+    a, b = y[-192:].float(), y2[-192:].float()
+    assert ((a - b).abs() <= torch.finfo(BF16).eps * a.abs() + apart).all() and (a != b).float().mean() < 1e-4
 
 
 def test_second_derivatives_and_tracing():
