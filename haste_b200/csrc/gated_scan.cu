@@ -48,7 +48,7 @@ int gated_scan_backward(const haste_b200_gated_scan& a, cudaStream_t s) { return
 
 long long gated_scan_scratch(const haste_b200_gated_scan& a, bool backward) {
   if (a.T < 0 || a.N <= 0 || a.D <= 0) return 0;
-  const int pieces = gated::most_pieces(a, backward ? gated::BWD_TT : gated::FWD_TT);
+  const int pieces = gated::most_pieces(a, backward);
   const long long rows = (long long)a.N * a.D, ends = pieces > 1 ? 2 * pieces * rows : 0;
   return ends + (backward && a.decay ? pieces * rows : 0);
 }

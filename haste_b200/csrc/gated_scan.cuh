@@ -210,6 +210,32 @@ __device__ __forceinline__ void fetch_steps(Raw<T, V> (&r)[L], Walk<U>& q, int l
   q.next();
 }
 
+// Waits for the launch in front (which this one may have overtaken so far), and lets the next one come.
+__device__ __forceinline__ void after_launch_in_front() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// What comes into a piece from those in front of it (backward: behind it): `count` pairs (product, addend), `step` apart, the
+// nearest last, folded by the block's warps a quarter each, many loads at a time.
+template <int V>
+__device__ __forceinline__ float2 fold_pieces(const float2* first, int count, long long step, float2 start, float4 (&shared)[SEG][32]) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, each = (count + SEG - 1) / SEG;
+  float2 p = both(1.f), e = both(0.f);
+#pragma unroll 8
+  for (int i = warp * each; i < min(count, (warp + 1) * each); ++i) {
+    const float2 *q = first + i * step, x = q[0], y = V == 2 ? q[V - 1] : both(0.f);
+    e = __ffma2_rn(make_float2(x.x, y.x), e, make_float2(x.y, y.y));
+    p = __fmul2_rn(p, make_float2(x.x, y.x));
+  }
+  shared[warp][lane] = make_float4(p.x, p.y, e.x, e.y);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SEG; ++w) {
+    const float4 q = shared[w][lane];
+    start = __ffma2_rn(make_float2(q.x, q.y), start, make_float2(q.z, q.w));
+  }
+  return start;
+}
+
 // ------------------------------------------------------------------ forward
 // A block takes 64 neighbouring channels, two a lane (32, one a lane, where rows do not start on whole pairs), and tiles of
 // four steps to each of its four warps.  A warp folds its steps into (product of decays, what they add to a state of
@@ -234,12 +260,6 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
   const float2 decay = decay_of<Decay, V>(a.decay, d);
   const bool far = goes_far(decay);
   float2 start = !Ends && a.state ? load_floats<V>(a.state + row) : both(0.f), total = both(1.f);
-  if (!Ends)
-#pragma unroll 8
-    for (int p = 0; p < at.piece; ++p) {
-      const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
-      start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
-    }
   const int stop = min(at.last, at.len);  // tiles from here on are behind the row's end
   const int ts0 = at.first + seg * L;
   Walk<const T> px(a.x, ts0, at.n, d, TT), pg(a.gate, ts0, at.n, d, TT), pi(In ? a.inner : a.x, ts0, at.n, d, TT);
@@ -252,8 +272,15 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
     fetch_steps<L>(gn, pg, left, whole);
     if (In) fetch_steps<L>(in, pi, left, whole);
   };
-  float2 h = start;
   if (at.first < stop) fetch(at.first);
+  if (Ends) {
+    let_next_launch_come();
+  } else if (a.pieces > 1) {
+    after_launch_in_front();
+    // (the first tile's pairs go into the other buffer)
+    start = fold_pieces<V>(a.ends + row, at.piece, rows, start, pairs[1]);
+  }
+  float2 h = start;
   int k = 0;
   for (int t0 = at.first; t0 < stop; t0 += TT, ++k) {
     const int ts = t0 + seg * L;
@@ -386,13 +413,6 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
   // (a channel whose decay is zero adds nothing to its state: w, whose slope has no value there, counts as constant)
   const float2 moves = make_float2(decay.x != 0.f ? 1.f : 0.f, decay.y != 0.f ? 1.f : 0.f);
   float2 start = !Ends && a.dfinal ? load_floats<V>(a.dfinal + row) : both(0.f), total = both(1.f), sum = both(0.f);
-  if (!Ends)
-#pragma unroll 8
-    for (int p = a.pieces - 1; p > at.piece; --p) {
-      const float2 *e = a.ends + p * rows + row, x = e[0], y = V == 2 ? e[V - 1] : both(0.f);
-      start = __ffma2_rn(make_float2(x.x, y.x), start, make_float2(x.y, y.y));
-    }
-  float2 mu = start;
 
   const int stop = min(at.last, at.len);
   const int tiles = stop > at.first ? (stop - at.first + TT - 1) / TT : 0;
@@ -416,6 +436,13 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
     ph -= rows;
   };
   if (tiles) fetch(at.first + (tiles - 1) * TT);
+  if (Ends) {
+    let_next_launch_come();
+  } else if (a.pieces > 1) {
+    after_launch_in_front();
+    start = fold_pieces<V>(a.ends + (a.pieces - 1) * rows + row, a.pieces - 1 - at.piece, -rows, start, pairs[1]);
+  }
+  float2 mu = start;
   if constexpr (!Ends) {
     if (at.ok)
       for (int t = at.first + tiles * TT + seg; t < at.last; t += SEG) {
@@ -557,16 +584,20 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
 }
 
 // ------------------------------------------------------------------ host side
-// Pieces of the sequence: none while the channels make two blocks an SM, else as many as make four, of two tiles at least.
-inline int pieces_of(const haste_b200_gated_scan& a, int V, int tile) {
-  const long long blocks = (long long)a.N * ceil_div(a.D, 32 * V);
-  if (blocks >= 2LL * sm_count()) return 1;
-  const long long most = a.T / (2 * tile), want = (4LL * sm_count() + blocks - 1) / blocks;
-  return (int)std::max(1LL, std::min(most, want));
+// Pieces of the sequence: none while the channels make blocks enough (two an SM; backward, which keeps four on an SM where
+// the forward pass keeps seven, one and a half), else as many as make seven an SM, of a tile at least (four an SM: bf16
+// 1000 x 8 x 1024 47 us, backward 62).  us, whole / in
+// pieces, both gates, bf16 1000 x N x 1024: N = 8 forward 70 / 39, backward 86 / 51; 16 78 / 66, 96 / 100; 32 92 / 111, 128 / 172.
+// fp32 2000 x 1 x 1024 162 / 20, 221 / 29; bf16 100 x 8 x 1024 14 / 12, 18 / 17.
+inline int pieces_of(const haste_b200_gated_scan& a, int V, bool backward) {
+  const long long blocks = (long long)a.N * ceil_div(a.D, 32 * V), sms = sm_count();
+  const int tile = backward ? BWD_TT : FWD_TT;
+  if (blocks * 2 >= sms * (backward ? 3 : 4) || a.T < 4 * tile) return 1;
+  return (int)std::min((long long)(a.T / tile), (7 * sms + blocks - 1) / blocks);
 }
 // (Scratch is asked for before the pointers are there, which decide on one channel a lane or two: the most of both.)
-inline int most_pieces(const haste_b200_gated_scan& a, int tile) {
-  return std::max(pieces_of(a, 1, tile), pieces_of(a, 2, tile));
+inline int most_pieces(const haste_b200_gated_scan& a, bool backward) {
+  return std::max(pieces_of(a, 1, backward), pieces_of(a, 2, backward));
 }
 
 template <typename T>
@@ -592,12 +623,29 @@ bool in_pairs(const haste_b200_gated_scan& a) {
   return true;
 }
 
+// A launch that may begin while the one in front of it ends; it waits for that itself.
+template <typename K, typename A>
+int launch_behind(K kernel, long long blocks, const A& args, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  HB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args));
+  count_launch(1);
+  return HASTE_B200_OK;
+}
+
 template <typename T, int V, bool Decay, bool In>
 int run_forward(const haste_b200_gated_scan& a, cudaStream_t s) {
   Args<T> k = pack<T>(a, V);
   // (every piece reads the initial state, so a final state in its place takes whole sequences)
   const bool cut = a.scratch && !(a.state && a.final_state == a.state);
-  const int pieces = cut ? pieces_of(a, V, FWD_TT) : 1;
+  const int pieces = cut ? pieces_of(a, V, false) : 1;
   if (pieces > 1) {
     k.piece = ceil_div(ceil_div(a.T, pieces), FWD_TT) * FWD_TT;
     k.pieces = ceil_div(a.T, k.piece);
@@ -609,8 +657,9 @@ int run_forward(const haste_b200_gated_scan& a, cudaStream_t s) {
     gated_fwd<T, V, Decay, In, true><<<(int)(blocks * (k.pieces - 1)), THREADS, 0, s>>>(k);
     HB_LAUNCH_OK();
     count_launch(1);
+    return launch_behind(gated_fwd<T, V, Decay, In, false>, blocks * k.pieces, k, s);
   }
-  gated_fwd<T, V, Decay, In, false><<<(int)(blocks * k.pieces), THREADS, 0, s>>>(k);
+  gated_fwd<T, V, Decay, In, false><<<(int)blocks, THREADS, 0, s>>>(k);
   HB_LAUNCH_OK();
   count_launch(1);
   return HASTE_B200_OK;
@@ -618,7 +667,7 @@ int run_forward(const haste_b200_gated_scan& a, cudaStream_t s) {
 template <typename T, int V, bool Decay, bool In>
 int run_backward(const haste_b200_gated_scan& a, cudaStream_t s) {
   Args<T> k = pack<T>(a, V);
-  const int pieces = pieces_of(a, V, BWD_TT);
+  const int pieces = pieces_of(a, V, true);
   if (pieces > 1) {
     k.piece = ceil_div(ceil_div(a.T, pieces), BWD_TT) * BWD_TT;
     k.pieces = ceil_div(a.T, k.piece);
@@ -633,10 +682,12 @@ int run_backward(const haste_b200_gated_scan& a, cudaStream_t s) {
     gated_bwd<T, V, Decay, false, true><<<(int)(blocks * k.pieces), THREADS, 0, s>>>(k);
     HB_LAUNCH_OK();
     count_launch(1);
+    HB_TRY(launch_behind(gated_bwd<T, V, Decay, In, false>, blocks * k.pieces, k, s));
+  } else {
+    gated_bwd<T, V, Decay, In, false><<<(int)blocks, THREADS, 0, s>>>(k);
+    HB_LAUNCH_OK();
+    count_launch(1);
   }
-  gated_bwd<T, V, Decay, In, false><<<(int)(blocks * k.pieces), THREADS, 0, s>>>(k);
-  HB_LAUNCH_OK();
-  count_launch(1);
   if (Decay) {
     SumJobs jobs;
     jobs.add(a.ddecay, 0, 1, a.D, HASTE_B200_F32);
