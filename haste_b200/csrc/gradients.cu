@@ -60,26 +60,26 @@ __device__ __forceinline__ const Entry& entry_of(const Table<N>& t, int chunk) {
 }
 
 // A thread's whole words of a chunk, and the first and the last word of a tensor, which may be its neighbours' too.
-template <typename T>
+template <typename T, int B = 16>  // of B bytes
 struct Words {
-  static constexpr int V = 16 / sizeof(T);
-  Raw<T, V> w[LOADS];
+  static constexpr int V = B / sizeof(T), N = LOADS * 16 / B;
+  Raw<T, V> w[N];
   long long first, end;  // element, counted from the start of the tensor's first word, of the thread's first word; the tensor's end
   int pad;
   __device__ __forceinline__ Words(const Entry& e, int chunk)
-      : first(((long long)(chunk - e.first) * WORDS + threadIdx.x) * V), end(e.pad + e.numel), pad(e.pad) {
+      : first(((long long)(chunk - e.first) * (THREADS * N) + threadIdx.x) * V), end(e.pad + e.numel), pad(e.pad) {
     const T* base = static_cast<const T*>(e.data) - pad;
 #pragma unroll
-    for (int k = 0; k < LOADS; ++k) w[k] = load_if<T, V>(whole(k), base + at(k));
+    for (int k = 0; k < N; ++k) w[k] = load_if<T, V>(whole(k), base + at(k));
   }
   __device__ __forceinline__ long long at(int k) const { return first + (long long)k * THREADS * V; }
   __device__ __forceinline__ bool whole(int k) const { return at(k) >= pad && at(k) + V <= end; }
   // f(element) for those in words that are not whole
   template <typename F>
   __device__ __forceinline__ void edges(const F& f) const {
-    if (whole(0) && whole(LOADS - 1)) return;
+    if (whole(0) && whole(N - 1)) return;
 #pragma unroll 1
-    for (int k = 0; k < LOADS; ++k)
+    for (int k = 0; k < N; ++k)
       if (!whole(k))
         for (long long i = max(at(k), (long long)pad); i < min(at(k) + V, end); ++i) f(i);
   }
@@ -130,6 +130,7 @@ __device__ __forceinline__ double squares(const Entry& e, int chunk) {
 template <int N>
 __global__ void __launch_bounds__(THREADS, PER_SM) norm_kernel(const __grid_constant__ Table<N> t, double* parts) {
   __shared__ double shared[THREADS / 32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double sum = 0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const Entry& e = entry_of(t, c);
@@ -149,17 +150,21 @@ __device__ __forceinline__ double norm_of(const Finish& f, double* shared) {
 }
 __global__ void __launch_bounds__(THREADS) finish_kernel(const Finish f) {
   __shared__ double shared[THREADS / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const double norm = norm_of(f, shared);
   if (threadIdx.x == 0) *f.norm = (float)norm;
 }
 
 template <typename T, typename O>
 __device__ __forceinline__ void scale(const Entry& e, int chunk, float factor) {
-  const Words<T> words(e, chunk);
-  constexpr int V = Words<T>::V, S = 16 / sizeof(O) < V ? 16 / sizeof(O) : V;  // S: elements of a store
+  // (Words that make 16 bytes at most on either side, so that a warp's stores leave no gaps: bf16 into float32, 402 MB, two
+  // stores of 16 bytes a word 250 us.)
+  constexpr int B = sizeof(O) > sizeof(T) ? 8 : 16;
+  const Words<T, B> words(e, chunk);
+  constexpr int V = Words<T, B>::V;
   O* base = static_cast<O*>(e.out) - e.pad;
 #pragma unroll
-  for (int k = 0; k < LOADS; ++k) {
+  for (int k = 0; k < Words<T, B>::N; ++k) {
     if (!words.whole(k)) continue;
     O* to = base + words.at(k);
     float v[V];
@@ -167,13 +172,7 @@ __device__ __forceinline__ void scale(const Entry& e, int chunk, float factor) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] *= factor;
     if (e.wide) {
-#pragma unroll
-      for (int j = 0; j < V; j += S) {
-        float part[S];
-#pragma unroll
-        for (int q = 0; q < S; ++q) part[q] = v[j + q];
-        store<O, S>(to + j, part);
-      }
+      store<O, V>(to, v);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) st(to + j, v[j]);
@@ -191,8 +190,9 @@ __device__ __forceinline__ void scale_to(const Entry& e, int chunk, float factor
 // The last chunks first: those are what the norm's launch has left in L2.  Gradients that stay as they are and where
 // they are cost no more than the sum of the partials.
 template <int N>
-__global__ void __launch_bounds__(THREADS, PER_SM) clip_kernel(const __grid_constant__ Table<N> t, const Finish f) {
+__global__ void __launch_bounds__(THREADS, 3) clip_kernel(const __grid_constant__ Table<N> t, const Finish f) {
   __shared__ double shared[THREADS / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (this launch may have overtaken the norm's)
   const double norm = norm_of(f, shared);
   if (blockIdx.x == 0 && threadIdx.x == 0 && t.from == 0) *f.norm = (float)norm;
   const double ratio = f.max_norm / (norm + 1e-6);
@@ -211,7 +211,7 @@ Entry entry(const haste_b200_gradient& g) {
   const int e = size_of(g.dtype), o = size_of(g.out_dtype);
   Entry r{g.data, g.out, g.numel, 0, (signed char)g.dtype, (signed char)g.out_dtype, 0, 0};
   r.pad = (signed char)(reinterpret_cast<uintptr_t>(g.data) % 16 / e);
-  const int V = 16 / e, bytes = std::min(16, V * o);
+  const int V = (o > e ? 8 : 16) / e, bytes = V * o;
   r.wide = (reinterpret_cast<uintptr_t>(g.out) - (uintptr_t)(r.pad * o)) % bytes == 0;
   return r;
 }
@@ -219,6 +219,23 @@ long long chunks_of(const haste_b200_gradient& g) {
   const int V = 16 / size_of(g.dtype);
   const long long n = reinterpret_cast<uintptr_t>(g.data) % 16 / size_of(g.dtype) + g.numel;
   return (n + (long long)V * WORDS - 1) / ((long long)V * WORDS);
+}
+
+// A launch that may begin while the one in front of it ends; it waits for that itself.
+template <typename K, typename... A>
+int launch_behind(K kernel, int blocks, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  HB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  count_launch(1);
+  return HASTE_B200_OK;
 }
 
 constexpr int FEW = 60, MANY = 960;  // entries of a launch's table: 2 KB of arguments, or 31 KB
@@ -237,6 +254,9 @@ int launch_table(const haste_b200_gradient* g, int n, int from, int chunks, doub
     t.chunks += (int)chunks_of(g[i]);
     t.e[t.count++] = e;
   }
+  // (Of several tables only the first comes close behind: what a launch waits for is the one in front of it, and all norms'
+  // have ended when that one's does, since none of them begins early.)
+  if (f && from == 0) return launch_behind(clip_kernel<N>, blocks_of(chunks), s, t, *f);
   if (f) clip_kernel<N><<<blocks_of(chunks), THREADS, 0, s>>>(t, *f);
   else norm_kernel<N><<<blocks_of(chunks), THREADS, 0, s>>>(t, parts);
   HB_LAUNCH_OK();
@@ -301,10 +321,7 @@ int run(const haste_b200_gradient* g, int count, const float* max_norm, float* n
   }));
   const Finish f{parts, from, norm, max_norm ? *max_norm : 0.f};
   if (!max_norm || from == 0) {
-    finish_kernel<<<1, THREADS, 0, s>>>(f);
-    HB_LAUNCH_OK();
-    count_launch(1);
-    return HASTE_B200_OK;
+    return launch_behind(finish_kernel, 1, s, f);
   }
   from = 0;
   return each_launch(g, count, [&](const haste_b200_gradient* some, int n, int used, int chunks) {

@@ -17,6 +17,9 @@ from . import _C
 __all__ = ["grad_norm", "clip_gradients", "clip_grad_norm_"]
 
 
+_native = _C.native
+
+
 def _tensors(gradients):
     return [gradients] if torch.is_tensor(gradients) else [g for g in gradients if g is not None]
 
@@ -24,21 +27,20 @@ def _tensors(gradients):
 def grad_norm(gradients):
     """The norm of a tensor or of several (those that are None count as zero)."""
     some = _tensors(gradients)
-    return _C.native().clip_gradients(some, None, None) if some else torch.zeros(())
+    return _native().clip_gradients(some, None, None) if some else torch.zeros(())
 
 
 def clip_gradients(gradients, max_norm, out=None):
     """Scales the gradients so that their norm is at most `max_norm` (a factor of 1 where that is infinite), in place or,
     where given, into `out`: tensors of the same shapes and strides, of any of the three types.  No two may overlap in
-    memory.  Returns the norm before.
+    memory; in place, a tensor that is listed twice counts once.  Returns the norm before.
 
     A norm that is not finite scales as the formula says: an infinite one to zero (infinite values to NaN), NaN to NaN."""
-    with torch.no_grad():
-        if out is not None:
-            gradients, out = ([t] if torch.is_tensor(t) else list(t) for t in (gradients, out))
-            return _C.native().clip_gradients(gradients, float(max_norm), out) if gradients else torch.zeros(())
-        some = _tensors(gradients)
-        return _C.native().clip_gradients(some, float(max_norm), None) if some else torch.zeros(())
+    if out is not None:
+        gradients, out = ([t] if torch.is_tensor(t) else list(t) for t in (gradients, out))
+        return _native().clip_gradients(gradients, max_norm, out) if gradients or out else torch.zeros(())
+    some = _tensors(gradients)
+    return _native().clip_gradients(some, max_norm, None) if some else torch.zeros(())
 
 
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
@@ -46,9 +48,10 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     With `error_if_nonfinite` a norm that is not finite raises and leaves the gradients as they are."""
     if torch.is_tensor(parameters):
         parameters = [parameters]
-    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
+    grads = [p.grad for p in parameters]
+    grads = [g for g in grads if g is not None]
     if error_if_nonfinite and grads:
         norm = grad_norm(grads)
         if not torch.isfinite(norm):
             raise RuntimeError(f"haste_b200: the norm of the gradients is {norm.item()}; they are not clipped")
-    return clip_gradients(grads, max_norm)
+    return _native().clip_gradients(grads, max_norm, None) if grads else torch.zeros(())

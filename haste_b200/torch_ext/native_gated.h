@@ -349,7 +349,8 @@ void refuse_overlaps(const std::vector<haste_b200_gradient>& g) {
   }
 }
 
-// The norm of all gradients (a float32 scalar).  With max_norm they are scaled into `out`, or where they are.
+// The norm of all gradients (a float32 scalar).  With max_norm they are scaled into `out`, or where they are; then a tensor
+// that is listed twice counts once.
 Tensor clip_gradients(const std::vector<Tensor>& gradients, const c10::optional<double>& max_norm,
                       const c10::optional<std::vector<Tensor>>& out) {
   if (gradients.empty()) refuse("there must be a gradient");
@@ -373,18 +374,31 @@ Tensor clip_gradients(const std::vector<Tensor>& gradients, const c10::optional<
   devices(gradients[0], gradients);
   if (out) devices(gradients[0], *out);
   if (max_norm) {
-    refuse_overlaps(g);
-    for (const Tensor& t : out ? *out : gradients) {
-      TORCH_CHECK(!(t.is_leaf() && t.requires_grad() && at::GradMode::is_enabled()),
-                  "haste_b200: a leaf that requires grad cannot be scaled in place");
-      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    if (!out) {
+      std::vector<void*> seen;
+      for (const Tensor& t : gradients) seen.push_back(t.unsafeGetTensorImpl());
+      std::sort(seen.begin(), seen.end());
+      if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) {
+        seen.clear();
+        size_t n = 0;
+        for (size_t i = 0; i < gradients.size(); ++i) {
+          if (std::find(seen.begin(), seen.end(), gradients[i].unsafeGetTensorImpl()) != seen.end()) continue;
+          seen.push_back(gradients[i].unsafeGetTensorImpl());
+          g[n++] = g[i];
+        }
+        g.resize(n);
+      }
     }
+    refuse_overlaps(g);
+    for (const Tensor& t : out ? *out : gradients)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   const c10::cuda::CUDAGuard guard(gradients[0].device());
-  Tensor norm = at::empty({}, gradients[0].options().dtype(at::kFloat).requires_grad(false));
-  Tensor scratch = at::empty({std::max<int64_t>(1, lib.grad_norm_scratch(g.data(), (int)g.size()))}, norm.options());
-  if (max_norm) CALL(clip_gradients, g.data(), (int)g.size(), (float)*max_norm, static_cast<float*>(norm.data_ptr()), static_cast<float*>(scratch.data_ptr()), stream());
-  else CALL(grad_norm, g.data(), (int)g.size(), static_cast<float*>(norm.data_ptr()), static_cast<float*>(scratch.data_ptr()), stream());
+  const at::TensorOptions o = gradients[0].options().dtype(at::kFloat).requires_grad(false);
+  Tensor norm = at::empty({}, o), scratch = at::empty({std::max<int64_t>(1, lib.grad_norm_scratch(g.data(), (int)g.size()))}, o);
+  float *to = static_cast<float*>(norm.data_ptr()), *with = static_cast<float*>(scratch.data_ptr());
+  if (max_norm) CALL(clip_gradients, g.data(), (int)g.size(), (float)*max_norm, to, with, stream());
+  else CALL(grad_norm, g.data(), (int)g.size(), to, with, stream());
   return norm;
 }
 

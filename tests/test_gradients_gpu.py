@@ -136,7 +136,7 @@ def test_axes_in_any_order_and_refusals():
             (([base.double()], 1.0), TypeError, "float32, bfloat16 and float16"),
             (([base], -1.0), ValueError, "max_norm"),
             (([base], float("nan")), ValueError, "max_norm"),
-            (([base, base], 1.0), ValueError, "overlap"),
+            (([base, base.view(-1)], 1.0), ValueError, "overlap"),
             (([base, base[1:]], 1.0), ValueError, "overlap"),
             (([base], 1.0, [base[0]]), ValueError, "shapes"),
             (([t], 1.0, [torch.empty(t.shape, device="cuda")]), ValueError, "lie in memory"),
@@ -146,7 +146,11 @@ def test_axes_in_any_order_and_refusals():
             (([base, base.cpu()], 1.0), RuntimeError, "CUDA")):
         with pytest.raises(error, match=says):
             gradients.clip_gradients(*args)
-    gradients.grad_norm([base, base])  # reading twice is fine
+    twice = base.clone()
+    check(gradients.grad_norm([base, base]), [base, base])
+    both = [base, out.clone()]
+    check(gradients.clip_gradients([twice, out, twice], 1.0), both)  # the same tensor, in place: once
+    check_scaled(twice, base, norm_of(both), 1.0)
     shared = torch.nn.Parameter(torch.zeros(6, 5, 4, device="cuda"))
     shared.grad = base.clone()
     check(clip_grad_norm_([shared, shared, torch.nn.Parameter(torch.zeros(3, device="cuda"))], 1.0), [base])
