@@ -66,6 +66,7 @@ struct Params {
 // A contraction that stores its sums as they are, or one that is a projection's, with operands of type T.
 struct Plain {
   static constexpr bool projection = false, tiles = false;
+  typedef float T, TO;
 };
 template <typename T_, typename TO_>
 struct Projection {
@@ -232,72 +233,121 @@ __device__ __forceinline__ void store_projection(const Params& p, const Epilogue
 // Sixteen-bit operands: a warp's 32 rows of the tile, in steps of 128 bytes of y.  Lane r holds row r of the sums, so bias and
 // activation happen in the registers that tensor memory is read into; y (and p, what the backward pass reads) goes as
 // 16-byte words into a tile of shared memory that a bulk store takes out, and the residual comes in by the same tile: rows
-// by eight lanes from memory, words of its own row to each lane.  buf: 4 KB for y, 4 KB for p.
-// (With the sums themselves through shared memory, and loads and stores of four elements behind it, the epilogue bounded
-// the product: bf16 64000 x 2048, K = 1024 with SiLU 401 us, with p 428.)
+// by eight lanes from memory, words of its own row to each lane.  buf: two tiles of 4 KB, y's by turns, or p's and y's; a
+// tile is written again once the store of the step before has read it.  Bias and residual are asked for a step ahead, the
+// first of a tile before its sums are there.
+// (bf16 64000 x 2048, K = 1024 with SiLU / and p: the sums themselves through shared memory, and loads and stores of four
+// elements behind it 401 / 428 us; one tile each for y and p, bias and residual asked for when they are needed 259 / 292.)
 template <typename EP>
-__device__ __forceinline__ void project_tile(const Params& p, const EP& ep, uint32_t taddr, int m0, int n0, uint8_t* buf) {
+struct Early {
   typedef typename EP::T T;
   typedef typename EP::TO TO;
-  constexpr int CW = 128 / sizeof(TO), V = 16 / sizeof(TO);  // columns of a step, of a 16-byte word of y
-  const Epilogue& e = ep.e;
-  const int lane = threadIdx.x & 31;
-  uint4* tile = reinterpret_cast<uint4*>(buf);
-  uint4* kept = tile + 256;
-  uint4 res[8];
-  auto fetch = [&](int n) {  // rows i * 4 + lane / 8, word lane % 8
+  static constexpr int CW = 128 / sizeof(TO), V = 16 / sizeof(TO);  // columns of a step, of a 16-byte word of y
+  uint4 bias[8], res[8];
+  // 32 columns from n on (N is a multiple of eight)
+  __device__ __forceinline__ void ask_bias(const Params& p, const Epilogue& e, int n) {
+    if (!e.bias) return;
+    if (e.bias_f32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j * 4 < p.N) bias[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(e.bias) + n + j * 4));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j * 8 < p.N) bias[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.bias) + n + j * 8));
+    }
+  }
+  // rows i * 4 + lane / 8, word lane % 8
+  __device__ __forceinline__ void ask_residual(const Params& p, const Epilogue& e, int m0, int n) {
+    if (!e.residual) return;
+    const int lane = threadIdx.x & 31, c = n + (lane & 7) * V;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3), c = n + (lane & 7) * V;
-      res[i] = make_uint4(0, 0, 0, 0);
+      const int r = i * 4 + (lane >> 3);
       if (m0 + r < p.M && c < p.N)
         res[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const TO*>(e.residual) + (long long)(m0 + r) * e.ld_res + c));
     }
+  }
+  __device__ __forceinline__ void ask(const Params& p, const EP& ep, int m0, int n0) {
+    ask_bias(p, ep.e, n0);
+    ask_residual(p, ep.e, m0, n0);
+  }
+};
+struct Nothing {
+  template <typename EP>
+  __device__ __forceinline__ void ask(const Params&, const EP&, int, int) {}
+};
+template <typename EP>
+__device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Early<EP>& early, uint32_t taddr, int m0, int n0, uint8_t* buf,
+                                             int& turn) {
+  typedef typename EP::T T;
+  typedef typename EP::TO TO;
+  constexpr int CW = Early<EP>::CW, V = Early<EP>::V;
+  const Epilogue& e = ep.e;
+  const int lane = threadIdx.x & 31;
+  const bool keeps = sizeof(TO) == 2 && e.pre;
+  uint4* const kept = reinterpret_cast<uint4*>(buf);
+  uint4* tile = kept + 256;
+  auto free_tile = [&]() {  // of two stores under way the older one has read its tile
+    if (lane == 0) tma_stores_read<1>();
+    __syncwarp();
   };
-  if (e.residual) fetch(n0);
+  auto send = [&](const CUtensorMap* map, uint4* from, int n) {
+    fence_async();
+    __syncwarp();
+    if (lane == 0) tma_store_3d(map, smem_u32(from), n, m0, 0);
+  };
 #pragma unroll 1
   for (int n = n0; n < min(n0 + BN, p.N); n += CW) {
-    if (lane == 0) tma_stores_read();
-    __syncwarp();  // the tiles before have been read
+    if (!keeps) {  // (from tile to tile too)
+      tile = kept + turn * 256;
+      turn ^= 1;
+    }
     if (e.residual) {
+      if (keeps) {  // (y's store is the newer one)
+        if (lane == 0) tma_stores_read<0>();
+        __syncwarp();
+      } else {
+        free_tile();
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = i * 4 + (lane >> 3);
-        tile[r * 8 + ((lane & 7) ^ (r & 7))] = res[i];
+        tile[r * 8 + ((lane & 7) ^ (r & 7))] = early.res[i];
       }
-      __syncwarp();
-      if (n + CW < n0 + BN) fetch(n + CW);
+      if (n + CW < n0 + BN) early.ask_residual(p, e, m0, n + CW);
     }
+    uint32_t packed[CW == 64 ? 32 : 1];  // y, until its tile is free
 #pragma unroll
     for (int h = 0; h < CW / 32; ++h) {
       uint32_t r[32];
       float v[32];
       tc_ld32(taddr + (n - n0) + h * 32, r);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = 0.f;
       if (e.bias) {
+        if (e.bias_f32) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {  // (N is a multiple of eight)
-          float b[8] = {};
-          const int c = n + h * 32 + j;
-          if (c < p.N) {
-            if (e.bias_f32) ss::load<float, 8>(static_cast<const float*>(e.bias) + c, b);
-            else ss::load<T, 8>(static_cast<const T*>(e.bias) + c, b);
+          for (int j = 0; j < 8; ++j) {
+            v[4 * j] = __uint_as_float(early.bias[j].x); v[4 * j + 1] = __uint_as_float(early.bias[j].y);
+            v[4 * j + 2] = __uint_as_float(early.bias[j].z); v[4 * j + 3] = __uint_as_float(early.bias[j].w);
           }
+        } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[j + k] = b[k];
+          for (int j = 0; j < 4; ++j) ss::load<T, 8>(reinterpret_cast<const T*>(&early.bias[j]), reinterpret_cast<float(&)[8]>(v[8 * j]));
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+        if (n + h * 32 + 32 < n0 + BN) early.ask_bias(p, e, n + h * 32 + 32);
       }
       tc_wait_ld();
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
       if (e.pre) {
+        if (keeps && h == 0) free_tile();
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint4 word;
           ss::store<T, 8>(reinterpret_cast<T*>(&word), reinterpret_cast<const float(&)[8]>(v[w * 8]));
-          if (sizeof(TO) == 2) kept[lane * 8 + ((h * 4 + w) ^ (lane & 7))] = word;
+          if (keeps) kept[lane * 8 + ((h * 4 + w) ^ (lane & 7))] = word;
           else if (m0 + lane < p.M && n + w * 8 < p.N)  // (half a line a row)
             *reinterpret_cast<uint4*>(static_cast<T*>(e.pre) + (long long)(m0 + lane) * e.ld_pre + n + w * 8) = word;
         }
@@ -306,25 +356,36 @@ __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, uint
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = epi::activate<false, decltype(act)::value>(v[j]);
       });
+      if (e.residual) {
+        if (h == 0) __syncwarp();
 #pragma unroll
-      for (int w = 0; w < 32 / V; ++w) {
-        uint4* word = &tile[lane * 8 + ((h * 4 + w) ^ (lane & 7))];
-        float(&y)[V] = reinterpret_cast<float(&)[V]>(v[w * V]);
-        if (e.residual) {
+        for (int w = 0; w < 32 / V; ++w) {
           float q[V];
-          ss::load<TO, V>(reinterpret_cast<const TO*>(word), q);
+          ss::load<TO, V>(reinterpret_cast<const TO*>(&tile[lane * 8 + ((h * 4 + w) ^ (lane & 7))]), q);
 #pragma unroll
-          for (int k = 0; k < V; ++k) y[k] += q[k];
+          for (int k = 0; k < V; ++k) v[w * V + k] += q[k];
         }
-        ss::store<TO, V>(reinterpret_cast<TO*>(word), y);
+      }
+      if constexpr (sizeof(TO) == 2) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          ss::store<TO, 8>(reinterpret_cast<TO*>(&packed[h * 16 + w * 4]), reinterpret_cast<const float(&)[8]>(v[w * 8]));
+      } else {
+        if (!e.residual) free_tile();
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          tile[lane * 8 + (w ^ (lane & 7))] = make_uint4(__float_as_uint(v[4 * w]), __float_as_uint(v[4 * w + 1]),
+                                                         __float_as_uint(v[4 * w + 2]), __float_as_uint(v[4 * w + 3]));
       }
     }
-    fence_async();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_3d(&ep.y, smem_u32(tile), n, m0, 0);
-      if (sizeof(TO) == 2 && e.pre) tma_store_3d(&ep.pre, smem_u32(kept), n, m0, 0);
+    if (keeps) send(&ep.pre, kept, n);
+    if constexpr (sizeof(TO) == 2) {
+      if (!e.residual) free_tile();
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+        tile[lane * 8 + (w ^ (lane & 7))] = make_uint4(packed[4 * w], packed[4 * w + 1], packed[4 * w + 2], packed[4 * w + 3]);
     }
+    send(&ep.y, tile, n);
   }
 }
 
@@ -527,6 +588,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
     uint8_t* tile = aligned + R::STAGES * C::STAGE_BYTES + (warp - 2) * R::TILE;
     uint32_t acc_phase = 0;  // one parity bit per accumulator
     int cidx = 0;
+    [[maybe_unused]] int turn = 0;  // which of its two tiles a warp stores next
     bool ok = true;
     for (int item = blockIdx.x; item < total_items; item += gridDim.x) {
       const int tn = item % p.tiles_n;
@@ -544,6 +606,9 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
       for (int c = 0; c < nchunks; ++c) {
         const int acc = cidx % NACC;
         ++cidx;
+        typename std::conditional<EP::tiles, Early<EP>, Nothing>::type early;
+        if constexpr (EP::tiles)
+          if (ep.whole && !p.partial) early.ask(p, ep, m0, n0);
         if (ok) ok = mbar_wait(accf_bar(acc), (acc_phase >> acc) & 1u, abort_flag, p.err, 4);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -563,7 +628,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
           bool stored = false;
           if constexpr (EP::tiles)
             if (ep.whole && !p.partial) {
-              if (m0 < p.M) project_tile(p, ep, taddr, m0, n0, tile);
+              if (m0 < p.M) project_tile(p, ep, early, taddr, m0, n0, tile, turn);
               stored = true;
             }
 #pragma unroll 1
@@ -631,6 +696,7 @@ template <int NPROD, typename T, typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
 projection_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the sums of a K split)
   gemm_tile<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 // fp16 planes, or the bf16 planes that have taken their place.
@@ -814,6 +880,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
     const int half = (warp - 2) >> 2;  // which 128 columns of the accumulator
     uint32_t acc_phase = 0;  // one parity bit per accumulator
     int cidx = 0;
+    [[maybe_unused]] int turn = 0;  // which of its two tiles a warp stores next
     bool ok = true;
     for (int item = pair; item < total_items; item += npairs) {
       const int tn = item % p.tiles_n;
@@ -830,6 +897,9 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
       for (int c = 0; c < nchunks; ++c) {
         const int acc = cidx % PAIR_NACC;
         ++cidx;
+        typename std::conditional<EP::tiles, Early<EP>, Nothing>::type early;
+        if constexpr (EP::tiles)
+          if (ep.whole && !p.partial) early.ask(p, ep, m0, n0);
         if (ok) ok = mbar_wait(accf_bar(acc), (acc_phase >> acc) & 1u, abort_flag, p.err, 14);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -849,7 +919,7 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
           bool stored = false;
           if constexpr (EP::tiles)
             if (ep.whole && !p.partial) {
-              if (m0 < p.M) project_tile(p, ep, taddr, m0, n0, tile);
+              if (m0 < p.M) project_tile(p, ep, early, taddr, m0, n0, tile, turn);
               stored = true;
             }
 #pragma unroll 1
@@ -909,6 +979,7 @@ template <int NPROD, typename T, typename TO>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 projection_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                        const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   gemm_pair<NPROD, PLAIN>(map_a, map_b, p, ep);
 }
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
@@ -1261,18 +1332,35 @@ void launch_reduce(const float* part, int splits, int M, int N, int ld_part, voi
     splitk_reduce_kernel<TC, false><<<blocks, 256, 0, stream>>>(part, splits, stride, M, N, ld_part, (TC*)c, ldc, accumulate);
 }
 
-// The same for a projection, element by element.
+// The same for a projection, four columns a thread, whose bias, activation and residual come behind the sums.  It may be
+// launched while the product is under way, and waits for it.
 template <typename T, typename TO>
 __global__ void __launch_bounds__(256) projection_reduce_kernel(const float* __restrict__ part, int splits, int M, int N, int ld_part,
-                                                                TO* __restrict__ c, long long ldc, const Epilogue e) {
-  const long long total = (long long)M * N, stride = (long long)M * ld_part;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int m = (int)(i / N), n = (int)(i - (long long)m * N);
-    const float* src = part + (long long)m * ld_part + n;
-    float s = 0.f;
+                                                                int wide, TO* __restrict__ c, long long ldc, const Epilogue e) {
+  const unsigned quads = ld_part / 4, total = (unsigned)M * quads;
+  const long long stride = (long long)M * ld_part;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const int m = i / quads, n = (i - m * quads) * 4;
+    if (n >= N) continue;
+    const float4* src = reinterpret_cast<const float4*>(part + (long long)m * ld_part + n);
+    float v[4] = {};
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += src[k * stride];
-    epi::finish<T, TO>(e, s, m, n, c + m * ldc + n);
+    for (int k = 0; k < splits; ++k) {
+      const float4 f = src[k * (stride / 4)];
+      v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+    }
+    TO* to = c + m * ldc + n;
+    if (wide) {
+      float bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bias[j] = e.bias ? epi::bias_at<T>(e, n + j) : 0.f;
+      epi::finish4<T, TO>(e, v, bias, m, n, to);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < N) epi::finish<T, TO>(e, v[j], m, n + j, to + j);
+    }
   }
 }
 
@@ -1515,9 +1603,17 @@ int launch_projection(const GemmDesc& g, const Cut& c, const CUtensorMap& m_a, c
   }
   count_launch(1);
   if (!c.via_partial) return HASTE_B200_OK;
-  const int blocks = (int)min(((long long)c.M * c.N + 255) / 256, 8LL * c.sms);
-  projection_reduce_kernel<T, TO><<<blocks, 256, 0, stream>>>(p.partial, c.splits, c.M, c.N, c.part_ld, (TO*)g.c, g.ldc, e);
-  HB_LAUNCH_OK();
+  cfg = {};
+  cfg.stream = stream;
+  cfg.gridDim = dim3((int)min(((long long)c.M * (c.part_ld / 4) + 255) / 256, 8LL * c.sms));
+  cfg.blockDim = dim3(256);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int wide = p.wide && c.N % 4 == 0;
+  HB_CUDA_OK(cudaLaunchKernelEx(&cfg, projection_reduce_kernel<T, TO>, (const float*)p.partial, c.splits, c.M, c.N, c.part_ld, wide,
+                                (TO*)g.c, g.ldc, e));
   count_launch(1);
   return HASTE_B200_OK;
 }

@@ -171,9 +171,9 @@ int launch(const Args& a, int splits, cudaStream_t s) {
 template <typename T, typename TO>
 int run(Args a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  // shares of C until two blocks an SM have work, a step of every warp each at least
+  // shares of C until there is a block for every SM, each with all the loads that a warp has under way at once
   int splits = 1;
-  while (splits < 8 && (long long)splits * ceil_div(a.H, ROWS) < 2LL * sm_count() && a.C / (2 * splits) >= WARPS * 4 * V) splits *= 2;
+  while (splits < 8 && (long long)splits * ceil_div(a.H, ROWS) < sm_count() && a.C / (2 * splits) >= WARPS * 4 * V * 2) splits *= 2;
   a.per = ceil_div(ceil_div(a.C, splits), V) * V;
   const bool wide = a.C % V == 0 && a.x_ld % V == 0 && aligned(a.x, 16) && aligned(a.w, 16);
 #define HB_FEW(MT) return wide ? launch<T, MT, true, TO>(a, splits, s) : launch<T, MT, false, TO>(a, splits, s)
