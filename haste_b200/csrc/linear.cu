@@ -119,8 +119,8 @@ GemmDesc dw_product(const haste_b200_linear& a, const void* dp, long long ld, vo
   return product(a, a.H, a.C, a.M, dp, 1, ld, a.x, a.x_ld, 1, a.dweight, a.C, a.dtype, scratch);
 }
 
-// Few rows: 64 of 16 bits, 8 of fp32, which has no matrix instruction of its own.
-bool few_rows(const haste_b200_linear& a) { return a.M <= (a.dtype == HASTE_B200_F32 ? 8 : 64); }
+// Few rows: 32 of 16 bits, 8 of fp32, which has no matrix instruction of its own.
+bool few_rows(const haste_b200_linear& a) { return a.M <= (a.dtype == HASTE_B200_F32 ? 8 : 32); }
 
 struct Layout {
   size_t dp, part, gemm, bytes;

@@ -1,4 +1,4 @@
-// Projections of few rows (tokens): y[M,H] = act(x[M,C] W[H,C]^T + bias) + residual, M up to 64.
+// Projections of few rows (tokens): y[M,H] = act(x[M,C] W[H,C]^T + bias) + residual, M up to 32.
 //
 // The weight is read once and nothing else counts: HBM bounds it.  So the weights go from memory straight into the
 // registers that the matrix instruction takes them from, many loads ahead; tcgen05, whose operands go through shared
@@ -13,7 +13,7 @@ namespace few {
 
 using namespace ss;
 
-constexpr int WARPS = 8, ROWS = 16;  // of W: the rows of a matrix instruction
+constexpr int WARPS = 8;
 
 struct Args {
   const void *x, *w;
@@ -51,31 +51,40 @@ __device__ __forceinline__ Raw<T, 16 / (int)sizeof(T)> load16(bool ok, const T* 
   return r;
 }
 
-// A block takes 16 rows of W and a cluster's share of C; its warps share that out in turn.  Thread (g, t) of a warp has
-// rows g and g + 8 and 16 bytes of each, 32 (fp32: 16) values of C to the four t's.  The order of C in a product is free, so
-// those bytes are used as the registers of two matrix instructions (k = 2t, 2t + 1, 2t + 8, 2t + 9) as they lie, with x
+// A block takes RT times 16 rows of W and a cluster's share of C; its warps share that out in turn.  Thread (g, t) of a warp has
+// rows g and g + 8 of each 16 and 16 bytes of each, 32 (fp32: 16) values of C to the four t's.  The order of C in a product is free,
+// so those bytes are used as the registers of two matrix instructions (k = 2t, 2t + 1, 2t + 8, 2t + 9) as they lie, with x
 // the same way.  MT tiles of eight tokens.  fp32 multiplies on the FMA units.
+// x comes from L2 once for every RT 16 rows: from 17 tokens on two.  bf16, us: 1 x 1024, H = 4096 6.3 (8.4 MB: 1.3 at the copy
+// bandwidth, and about 2.5 for a launch and its first loads), 32 tokens 8.4; 1 x 4096, H = 4096 11.3 (33.6 MB: 5.1), 32 18.1.
+// 64 tokens in this way 29 and 53, where the tensor cores with K split take 12 and 18.
 // The warps' sums meet in shared memory, the blocks' of a cluster in the shared memory of each, rows shared out.
 template <typename T, int MT, bool Wide, typename TO>
+struct Shape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int V = 16 / sizeof(T), STEP = 4 * V, TOK = MT * 8, RT = MT >= 4 ? 2 : 1, ROWS = RT * 16;
+  static constexpr int AHEAD = MT >= 4 ? 2 : 4;  // steps whose loads are under way together
+};
+template <typename T, int MT, bool Wide, typename TO>
 __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
-  constexpr bool F32 = sizeof(T) == 4;
-  constexpr int V = 16 / sizeof(T), STEP = 4 * V, TOK = MT * 8, AHEAD = MT >= 4 ? 2 : 4;
+  typedef Shape<T, MT, Wide, TO> S;
+  constexpr bool F32 = S::F32;
+  constexpr int V = S::V, STEP = S::STEP, TOK = S::TOK, RT = S::RT, ROWS = S::ROWS, AHEAD = S::AHEAD;
   __shared__ float sums[WARPS][TOK][ROWS + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int splits = gridDim.x, split = blockIdx.x, h0 = blockIdx.y * ROWS;  // (a cluster is a row of blocks)
   const int c0 = split * a.per, c1 = min(a.C, c0 + a.per);
-  const T *w0 = static_cast<const T*>(a.w) + (long long)(h0 + g) * a.C, *w1 = w0 + 8LL * a.C;
-  const bool ok0 = h0 + g < a.H, ok1 = h0 + g + 8 < a.H;
+  const T* w = static_cast<const T*>(a.w) + (long long)(h0 + g) * a.C;
   const T* x = static_cast<const T*>(a.x);
-  float d[MT][4] = {};               // [tile]: (g, token 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
+  float d[RT][MT][4] = {};                   // [tile]: (g, token 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
   float f[F32 ? 2 : 1][F32 ? TOK : 1] = {};  // fp32: the thread's part of (row, token)
   for (int c = c0 + warp * STEP * AHEAD; c < c1; c += WARPS * STEP * AHEAD) {
-    Raw<T, V> wa[AHEAD], wb[AHEAD], xs[AHEAD][F32 ? 1 : MT];
+    Raw<T, V> ws[AHEAD][RT][2], xs[AHEAD][F32 ? 1 : MT];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int at = c + i * STEP + t * V;
-      wa[i] = load16<T, Wide>(ok0, w0, at, c1);
-      wb[i] = load16<T, Wide>(ok1, w1, at, c1);
+#pragma unroll
+      for (int r = 0; r < 2 * RT; ++r) ws[i][r / 2][r % 2] = load16<T, Wide>(h0 + g + 8 * r < a.H, w + 8LL * r * a.C, at, c1);
       if constexpr (!F32)
 #pragma unroll
         for (int m = 0; m < MT; ++m) xs[i][m] = load16<T, Wide>(m * 8 + g < a.M, x + (m * 8 + g) * a.x_ld, at, c1);
@@ -85,8 +94,8 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
       for (int i = 0; i < AHEAD; ++i) {
         const int at = c + i * STEP + t * V;
         float p[V], q[V];
-        unpack<T, V>(wa[i], p);
-        unpack<T, V>(wb[i], q);
+        unpack<T, V>(ws[i][0][0], p);
+        unpack<T, V>(ws[i][0][1], q);
 #pragma unroll
         for (int m = 0; m < TOK; ++m) {
           float v[V];
@@ -102,11 +111,13 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t w[4] = {wa[i].w[2 * half], wb[i].w[2 * half], wa[i].w[2 * half + 1], wb[i].w[2 * half + 1]};
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) mma<T>(d[m], w, xs[i][m].w[2 * half], xs[i][m].w[2 * half + 1]);
-        }
+          for (int r = 0; r < RT; ++r) {
+            const uint32_t k[4] = {ws[i][r][0].w[2 * half], ws[i][r][1].w[2 * half], ws[i][r][0].w[2 * half + 1], ws[i][r][1].w[2 * half + 1]};
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma<T>(d[r][m], k, xs[i][m].w[2 * half], xs[i][m].w[2 * half + 1]);
+          }
     }
   }
   if constexpr (F32) {
@@ -121,16 +132,18 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
       }
   } else {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sums[warp][m * 8 + 2 * t + i % 2][g + i / 2 * 8] = d[m][i];
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[warp][m * 8 + 2 * t + i % 2][r * 16 + g + i / 2 * 8] = d[r][m][i];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < TOK * ROWS; i += WARPS * 32) {
     const int m = i / ROWS, r = i % ROWS;
     float s = sums[0][m][r];
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) s += sums[w][m][r];
+    for (int v = 1; v < WARPS; ++v) s += sums[v][m][r];
     if (splits > 1) sums[0][m][r] = s;
     else if (m < a.M && h0 + r < a.H) epi::finish<T, TO>(a.e, s, m, h0 + r, static_cast<TO*>(a.y) + m * a.y_ld + h0 + r);
   }
@@ -151,9 +164,15 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
 }
 
 template <typename T, int MT, bool Wide, typename TO>
-int launch(const Args& a, int splits, cudaStream_t s) {
+int launch(Args a, cudaStream_t s) {
+  typedef Shape<T, MT, Wide, TO> S;
+  // Shares of C until there are two blocks an SM, each with the loads that its warps have under way together.
+  const int tiles = ceil_div(a.H, S::ROWS);
+  int splits = 1;
+  while (splits < 8 && splits * tiles < 2 * sm_count() && a.C / (2 * splits) >= WARPS * S::STEP * S::AHEAD) splits *= 2;
+  a.per = ceil_div(ceil_div(a.C, splits), S::V) * S::V;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits, ceil_div(a.H, ROWS));
+  cfg.gridDim = dim3(splits, tiles);
   cfg.blockDim = dim3(WARPS * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -169,21 +188,16 @@ int launch(const Args& a, int splits, cudaStream_t s) {
 }
 
 template <typename T, typename TO>
-int run(Args a, cudaStream_t s) {
+int run(const Args& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  // shares of C until there is a block for every SM, each with all the loads that a warp has under way at once
-  int splits = 1;
-  while (splits < 8 && (long long)splits * ceil_div(a.H, ROWS) < sm_count() && a.C / (2 * splits) >= WARPS * 4 * V * 2) splits *= 2;
-  a.per = ceil_div(ceil_div(a.C, splits), V) * V;
   const bool wide = a.C % V == 0 && a.x_ld % V == 0 && aligned(a.x, 16) && aligned(a.w, 16);
-#define HB_FEW(MT) return wide ? launch<T, MT, true, TO>(a, splits, s) : launch<T, MT, false, TO>(a, splits, s)
+#define HB_FEW(MT) return wide ? launch<T, MT, true, TO>(a, s) : launch<T, MT, false, TO>(a, s)
   if constexpr (sizeof(T) == 4) {
     HB_FEW(1);
   } else {
     if (a.M <= 8) HB_FEW(1);
     if (a.M <= 16) HB_FEW(2);
-    if (a.M <= 32) HB_FEW(4);
-    HB_FEW(8);
+    HB_FEW(4);
   }
 #undef HB_FEW
 }
