@@ -73,9 +73,9 @@ struct Projection {
   static constexpr bool projection = true, tiles = sizeof(T_) == 2;
   typedef T_ T;
   typedef TO_ TO;
-  CUtensorMap y, pre;  // for whole-tile stores
+  CUtensorMap y, pre;  // for bulk stores of tiles
   Epilogue e;
-  int whole;  // y, what is kept and the residual take them
+  int whole;  // y, what is kept, bias and residual take accesses of 16 bytes
 };
 
 template <int NPROD>
@@ -256,13 +256,15 @@ __device__ __forceinline__ void store_projection(const Params& p, const Epilogue
   }
 }
 // Sixteen-bit operands: a warp's 32 rows of the tile, in steps of 128 bytes of y.  Lane r holds row r of the sums, so bias and
-// activation happen in the registers that tensor memory is read into; y (and p, what the backward pass reads) goes as
-// 16-byte words into a tile of shared memory that a bulk store takes out, and the residual comes in by the same tile: rows
-// by eight lanes from memory, words of its own row to each lane.  buf: two tiles of 4 KB, y's by turns, or p's and y's; a
-// tile is written again once the store of the step before has read it.  Bias and residual are asked for a step ahead, those of
-// the next tile (next_m, next_n; beyond the matrix where there is none) with the last step.
-// (bf16 64000 x 2048, K = 1024 with SiLU / and p: the sums themselves through shared memory, and loads and stores of four
-// elements behind it 401 / 428 us; one tile each for y and p, bias and residual asked for when they are needed 259 / 292.)
+// activation happen in the registers that tensor memory is read into.  y (and p, what the backward pass reads) goes by
+// 16-byte words through a tile of shared memory, and the residual comes in the other way by the same tile, eight lanes a row.
+// Without a residual the tile leaves by a bulk store, and is written again once the store of the step before has read it:
+// p's and y's tiles, or y's by turns.  Such a store queues behind the operands' loads, which a residual, in whose way it is
+// from the step's beginning, cannot wait for: with one, lanes store what lanes have loaded.
+// Bias and residual are asked for a step ahead, those of the next tile (next_m, next_n; beyond the matrix where there is none)
+// with the last step.  buf: two tiles of 4 KB.
+// (bf16 64000 x 2048, K = 1024, SiLU / with p / residual alone: 215 / 240 / 268 us; bulk stores for all 213 / 245 / 316, lanes
+// for all 228 / 271 / 248; the sums themselves through shared memory, and accesses of four elements behind it, 401 / 428.)
 template <typename EP>
 struct Early {
   typedef typename EP::T T;
@@ -302,17 +304,31 @@ struct Nothing {
   template <typename EP>
   __device__ __forceinline__ void ask(const Params&, const EP&, int, int) {}
 };
-template <typename EP>
+// Rows of WORDS 16-byte words of a tile, from the warp's shared memory to memory; c: this lane's first column, of `cols`.
+template <int WORDS, typename TX>
+__device__ __forceinline__ void write_rows(const uint4* tile, TX* to, long long ld, int rows, int cols) {
+  constexpr int V = 16 / sizeof(TX), PER = 32 / WORDS;  // rows of an instruction
+  const int lane = threadIdx.x & 31, u = lane % WORDS;
+  if (u * V >= cols) return;
+#pragma unroll
+  for (int i = 0; i < 32 / PER; ++i) {
+    const int r = i * PER + lane / WORDS;
+    if (r < rows) *reinterpret_cast<uint4*>(to + r * ld + u * V) = tile[r * 8 + (u ^ (r & 7))];
+  }
+}
+// With RESIDUAL, or without.
+template <bool RESIDUAL, typename EP>
 __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Early<EP>& early, uint32_t taddr, int m0, int n0,
                                              int next_m, int next_n, uint8_t* buf, int& turn) {
   typedef typename EP::T T;
   typedef typename EP::TO TO;
   constexpr int CW = Early<EP>::CW, V = Early<EP>::V;
   const Epilogue& e = ep.e;
-  const int lane = threadIdx.x & 31;
-  const bool keeps = sizeof(TO) == 2 && e.pre;
+  const int lane = threadIdx.x & 31, rows = min(32, p.M - m0);
   uint4* const kept = reinterpret_cast<uint4*>(buf);
   uint4* tile = kept + 256;
+  const bool keeps = e.pre && sizeof(TO) == 2;  // by a tile of its own
+  auto word_of = [&](uint4* t, int w) { return t + lane * 8 + (w ^ (lane & 7)); };  // of this lane's row
   auto free_tile = [&]() {  // of two stores under way the older one has read its tile
     if (lane == 0) tma_stores_read<1>();
     __syncwarp();
@@ -324,17 +340,8 @@ __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Earl
   };
 #pragma unroll 1
   for (int n = n0; n < min(n0 + BN, p.N); n += CW) {
-    if (!keeps) {  // (from tile to tile too)
-      tile = kept + turn * 256;
-      turn ^= 1;
-    }
-    if (e.residual) {
-      if (keeps) {  // (y's store is the newer one)
-        if (lane == 0) tma_stores_read<0>();
-        __syncwarp();
-      } else {
-        free_tile();
-      }
+    if constexpr (RESIDUAL) {
+      __syncwarp();  // the tiles before have been read
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = i * 4 + (lane >> 3);
@@ -342,8 +349,12 @@ __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Earl
       }
       if (n + CW < min(n0 + BN, p.N)) early.ask_residual(p, e, m0, n + CW);
       else early.ask_residual(p, e, next_m, next_n);
+      __syncwarp();
+    } else if (!keeps) {  // (by turns from tile to tile too)
+      tile = kept + turn * 256;
+      turn ^= 1;
     }
-    uint32_t packed[CW == 64 ? 32 : 1];  // y, until its tile is free
+    uint32_t packed[!RESIDUAL && CW == 64 ? 32 : 1];  // y, until its tile is free
 #pragma unroll
     for (int h = 0; h < CW / 32; ++h) {
       uint32_t r[32];
@@ -369,12 +380,12 @@ __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Earl
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
       if (e.pre) {
-        if (keeps && h == 0) free_tile();
+        if (!RESIDUAL && keeps && h == 0) free_tile();
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint4 word;
           ss::store<T, 8>(reinterpret_cast<T*>(&word), reinterpret_cast<const float(&)[8]>(v[w * 8]));
-          if (keeps) kept[lane * 8 + ((h * 4 + w) ^ (lane & 7))] = word;
+          if (keeps) *word_of(kept, h * 4 + w) = word;
           else if (m0 + lane < p.M && n + w * 8 < p.N)  // (half a line a row)
             *reinterpret_cast<uint4*>(static_cast<T*>(e.pre) + (long long)(m0 + lane) * e.ld_pre + n + w * 8) = word;
         }
@@ -383,36 +394,40 @@ __device__ __forceinline__ void project_tile(const Params& p, const EP& ep, Earl
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = epi::activate<false, decltype(act)::value>(v[j]);
       });
-      if (e.residual) {
-        if (h == 0) __syncwarp();
+      if constexpr (RESIDUAL) {
 #pragma unroll
         for (int w = 0; w < 32 / V; ++w) {
+          TO* word = reinterpret_cast<TO*>(word_of(tile, h * (32 / V) + w));
+          float(&y)[V] = reinterpret_cast<float(&)[V]>(v[w * V]);
           float q[V];
-          ss::load<TO, V>(reinterpret_cast<const TO*>(&tile[lane * 8 + ((h * 4 + w) ^ (lane & 7))]), q);
+          ss::load<TO, V>(word, q);
 #pragma unroll
-          for (int k = 0; k < V; ++k) v[w * V + k] += q[k];
+          for (int k = 0; k < V; ++k) y[k] += q[k];
+          ss::store<TO, V>(word, y);
         }
-      }
-      if constexpr (sizeof(TO) == 2) {
+      } else if constexpr (sizeof(TO) == 2) {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
           ss::store<TO, 8>(reinterpret_cast<TO*>(&packed[h * 16 + w * 4]), reinterpret_cast<const float(&)[8]>(v[w * 8]));
       } else {
-        if (!e.residual) free_tile();
+        free_tile();
 #pragma unroll
-        for (int w = 0; w < 8; ++w)
-          tile[lane * 8 + (w ^ (lane & 7))] = make_uint4(__float_as_uint(v[4 * w]), __float_as_uint(v[4 * w + 1]),
-                                                         __float_as_uint(v[4 * w + 2]), __float_as_uint(v[4 * w + 3]));
+        for (int w = 0; w < 8; ++w) ss::store<TO, 4>(reinterpret_cast<TO*>(word_of(tile, w)), reinterpret_cast<const float(&)[4]>(v[w * 4]));
       }
     }
-    if (keeps) send(&ep.pre, kept, n);
-    if constexpr (sizeof(TO) == 2) {
-      if (!e.residual) free_tile();
+    if constexpr (RESIDUAL) {
+      __syncwarp();
+      if (keeps) write_rows<8, T>(kept, static_cast<T*>(e.pre) + (long long)m0 * e.ld_pre + n, e.ld_pre, rows, p.N - n);
+      write_rows<8, TO>(tile, static_cast<TO*>(p.c) + (long long)m0 * p.ldc + n, p.ldc, rows, p.N - n);
+    } else {
+      if (keeps) send(&ep.pre, kept, n);
+      if constexpr (sizeof(TO) == 2) {
+        free_tile();
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
-        tile[lane * 8 + (w ^ (lane & 7))] = make_uint4(packed[4 * w], packed[4 * w + 1], packed[4 * w + 2], packed[4 * w + 3]);
+        for (int w = 0; w < 8; ++w) *word_of(tile, w) = make_uint4(packed[4 * w], packed[4 * w + 1], packed[4 * w + 2], packed[4 * w + 3]);
+      }
+      send(&ep.y, tile, n);
     }
-    send(&ep.y, tile, n);
   }
 }
 
@@ -457,7 +472,7 @@ __device__ __forceinline__ void store_chunk(const Params& p, const EP& ep, int s
 template <int NPROD, int MODE>
 constexpr int chunk_of() { return MODE == PLAIN ? Cfg<NPROD>::CHUNK : (MODE == F16_PLANES ? 2 : 1); }
 
-// Shared memory: the ring, a tile per epilogue warp (two where whole tiles are stored, which on pairs takes a stage), barriers.
+// Shared memory: the ring, a tile per epilogue warp (a projection's of 16 bits two, which on pairs takes a stage), barriers.
 template <int NPROD, typename EP, bool PAIR>
 struct Room {
   static constexpr int STAGES = PAIR && EP::tiles ? Cfg<NPROD>::STAGES - 1 : Cfg<NPROD>::STAGES;
@@ -659,7 +674,8 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
               const int later = item + gridDim.x;
               const bool last = later >= total_items;
               const int next_m = last ? p.M : later / p.tiles_n % p.tiles_m * BM + quad * 32, next_n = last ? p.N : later % p.tiles_n * BN;
-              if (m0 < p.M) project_tile(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn);
+              if (m0 < p.M) ep.e.residual ? project_tile<true>(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn)
+                                                   : project_tile<false>(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn);
               else early.ask(p, ep, next_m, next_n);
               stored = true;
             }
@@ -956,7 +972,8 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
               const bool last = later >= total_items;
               const int next_m = last ? p.M : later / p.tiles_n % p.tiles_m * PBM + (int)rank * BM + quad * 32;
               const int next_n = last ? p.N : later % p.tiles_n * PBN + half * BN;
-              if (m0 < p.M && n0 < p.N) project_tile(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn);
+              if (m0 < p.M && n0 < p.N) ep.e.residual ? project_tile<true>(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn)
+                                                   : project_tile<false>(p, ep, early, taddr, m0, n0, next_m, next_n, tile, turn);
               else early.ask(p, ep, next_m, next_n);
               stored = true;
             }
