@@ -103,8 +103,11 @@ __device__ __forceinline__ float exp2_int(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Planes: bf16; two of fp16; three of bf16 in the place of those, handed over as often per product.
-enum { PLAIN, F16_PLANES, UNEVEN };
+// Planes: bf16; two of fp16; three of bf16 in the place of those, handed over as often per product; three of bf16 for a
+// projection, handed over every k-block with the least significant products first, so that of its 24 accumulations four meet
+// a sum of full size (relative error against fp64, 2331 x 250 x 1000 and its gradients: 0.9e-6 .. 1.4e-6 as elsewhere,
+// 0.9e-7 .. 1.1e-7 so; 16000 x 1024 x 2048 1.1e-7 .. 1.4e-7, 335 us).
+enum { PLAIN, F16_PLANES, UNEVEN, CAREFUL };
 
 // The powers of two that fp16 planes leave in a tile: of this lane's row, and of the four columns that the lane
 // stores of the chunk from n0 on.  (Loaded when they are used: the sums fill the registers till then.)
@@ -605,8 +608,9 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
             for (int pr = 0; pr < NPROD; ++pr) {
               // plane pairs, most significant first:
               //   (0,0) (0,1) (1,0) | (1,1) (0,2) (2,0)      0 = hi, 1 = mid/lo, 2 = lo
-              const int ia = pr == 2 ? 1 : (pr == 3 ? 1 : (pr == 5 ? 2 : 0));
-              const int ib = pr == 1 ? 1 : (pr == 3 ? 1 : (pr == 4 ? 2 : 0));
+              const int q = MODE == CAREFUL ? NPROD - 1 - pr : pr;
+              const int ia = q == 2 ? 1 : (q == 3 ? 1 : (q == 5 ? 2 : 0));
+              const int ib = q == 1 ? 1 : (q == 3 ? 1 : (q == 4 ? 2 : 0));
               const uint32_t pa = sa + ia * TILE_BYTES;
               const uint32_t pb = sb + ib * TILE_BYTES;
 #pragma unroll
@@ -700,7 +704,7 @@ __device__ __forceinline__ void gemm_tile(const CUtensorMap& map_a, const CUtens
         // Partial tiles of few rows leave from the lanes: one tile per CTA, and the four trips through shared memory, one
         // after the other, take 2 us longer than their stores (64 x 2048, K = 512 20.7 / 18.7 us, 32 x 4096, K = 1024
         // 24.9 / 22.8).
-        if (MODE == PLAIN && p.partial && p.M <= 64) {
+        if ((MODE == PLAIN || MODE == CAREFUL) && p.partial && p.M <= 64) {
           const int m = m0 + lane;
           float* dst = p.partial + ((long long)sp * p.M + m) * p.partial_ld + n0;
 #pragma unroll
@@ -745,7 +749,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 projection_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the sums of a K split)
-  gemm_tile<NPROD, PLAIN>(map_a, map_b, p, ep);
+  gemm_tile<NPROD, NPROD == 6 ? CAREFUL : PLAIN>(map_a, map_b, p, ep);
 }
 // fp16 planes, or the bf16 planes that have taken their place.
 __global__ void __launch_bounds__(THREADS, 1)
@@ -902,8 +906,9 @@ __device__ __forceinline__ void gemm_pair(const CUtensorMap& map_a, const CUtens
             const uint32_t sb = sa + C::PLANES * TILE_BYTES;
 #pragma unroll
             for (int pr = 0; pr < NPROD; ++pr) {
-              const int ia = pr == 2 ? 1 : (pr == 3 ? 1 : (pr == 5 ? 2 : 0));
-              const int ib = pr == 1 ? 1 : (pr == 3 ? 1 : (pr == 4 ? 2 : 0));
+              const int q = MODE == CAREFUL ? NPROD - 1 - pr : pr;
+              const int ia = q == 2 ? 1 : (q == 3 ? 1 : (q == 5 ? 2 : 0));
+              const int ib = q == 1 ? 1 : (q == 3 ? 1 : (q == 4 ? 2 : 0));
               const uint32_t pa = sa + ia * TILE_BYTES;
               const uint32_t pb = sb + ib * TILE_BYTES;
 #pragma unroll
@@ -1035,7 +1040,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 projection_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                        const __grid_constant__ Params p, const __grid_constant__ Projection<T, TO> ep) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  gemm_pair<NPROD, PLAIN>(map_a, map_b, p, ep);
+  gemm_pair<NPROD, NPROD == 6 ? CAREFUL : PLAIN>(map_a, map_b, p, ep);
 }
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_tcgen05_pair_f16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -1532,7 +1537,7 @@ const char* refusal(const GemmDesc& g) {
 // 365 / 330, 16384 x 512 x 1024 298 / 278, 8000 x 1024 x 1024 193 / 179; M x K x N.  Below 8 G multiply-adds, or 256 of
 // K, nothing is left).
 bool f16_planes(const GemmDesc& g) {
-  return g.precise && g.dtype == HASTE_B200_F32 && g.dtype_c == HASTE_B200_F32 && !g.accumulate && g.a_cs == 1 &&
+  return g.precise && !g.projection && g.dtype == HASTE_B200_F32 && g.dtype_c == HASTE_B200_F32 && !g.accumulate && g.a_cs == 1 &&
          g.b_cs == 1 && g.b_rs != 1 && g.K >= 256 && (double)g.M * g.N * g.K >= 8e9;
 }
 // How a contraction is carried out: kernel, K split, and the scratch for planes of fp32 operands and partial tiles.

@@ -107,6 +107,8 @@ GemmDesc product(const haste_b200_linear& a, int M, int N, int K, const void* x,
   g.precise = 1;
   g.projection = true;
   g.scratch = scratch;
+  static const Epilogue nothing{};
+  if (a.dtype == HASTE_B200_F32) g.epilogue = &nothing;  // (by the projections' own, more exact product)
   return g;
 }
 GemmDesc forward_product(const haste_b200_linear& a, void* scratch) {
