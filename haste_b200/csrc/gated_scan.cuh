@@ -13,6 +13,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 #include "state_space.cuh"
 
@@ -408,8 +409,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
   const long long rows = (long long)a.N * a.D, row = (long long)at.n * a.D + d;
   const float2 decay = decay_of<Decay, V>(a.decay, d);
   const bool far = goes_far(decay);
-  // (dlog_a / ddecay is r; in units of log(2) it is r too, and dlog_a has no units of its own)
-  const float2 natural = __fmul2_rn(decay, both(0.6931471805599453f));
+  const float2 natural = __fmul2_rn(decay, both(0.6931471805599453f));  // decay as it was given
   // (a channel whose decay is zero adds nothing to its state: w, whose slope has no value there, counts as constant)
   const float2 moves = make_float2(decay.x != 0.f ? 1.f : 0.f, decay.y != 0.f ? 1.f : 0.f);
   float2 start = !Ends && a.dfinal ? load_floats<V>(a.dfinal + row) : both(0.f), total = both(1.f), sum = both(0.f);
@@ -585,15 +585,17 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
 
 // ------------------------------------------------------------------ host side
 // Pieces of the sequence: none while the channels make blocks enough (two an SM; backward, which keeps four on an SM where
-// the forward pass keeps seven, one and a half), else as many as make seven an SM, of a tile at least (four an SM: bf16
-// 1000 x 8 x 1024 47 us, backward 62).  us, whole / in
-// pieces, both gates, bf16 1000 x N x 1024: N = 8 forward 70 / 39, backward 86 / 51; 16 78 / 66, 96 / 100; 32 92 / 111, 128 / 172.
-// fp32 2000 x 1 x 1024 162 / 20, 221 / 29; bf16 100 x 8 x 1024 14 / 12, 18 / 17.
+// the forward pass keeps seven, one and a half), else as many as make seven an SM (four: bf16 1000 x 8 x 1024 47 us,
+// backward 62), of a tile at least and three times the root of the steps at most, beyond which folding them takes longer than
+// walking them (bf16 16000 x 1 x 64, backward: without that bound 40 / 38 us, with it 21 / 24).  us, whole / in pieces, both
+// gates, bf16 1000 x N x 1024: N = 8 forward 70 / 39, backward 86 / 51; 16 78 / 66, 96 / 100; 32 92 / 111, 128 / 172; fp32
+// 2000 x 1 x 1024 162 / 17, 221 / 26; bf16 100 x 8 x 1024 14 / 12, 18 / 17.
 inline int pieces_of(const haste_b200_gated_scan& a, int V, bool backward) {
   const long long blocks = (long long)a.N * ceil_div(a.D, 32 * V), sms = sm_count();
   const int tile = backward ? BWD_TT : FWD_TT;
   if (blocks * 2 >= sms * (backward ? 3 : 4) || a.T < 4 * tile) return 1;
-  return (int)std::min((long long)(a.T / tile), (7 * sms + blocks - 1) / blocks);
+  const long long most = std::min(a.T / tile, (int)(3 * std::sqrt((double)a.T)));
+  return (int)std::min(most, (7 * sms + blocks - 1) / blocks);
 }
 // (Scratch is asked for before the pointers are there, which decide on one channel a lane or two: the most of both.)
 inline int most_pieces(const haste_b200_gated_scan& a, bool backward) {
