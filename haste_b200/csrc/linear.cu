@@ -161,7 +161,7 @@ int check(const haste_b200_linear& a, bool backward) {
 
 template <typename T, typename TO>
 int few_forward(const haste_b200_linear& a, const Epilogue& e, cudaStream_t s) {
-  return few::run<T, TO>(few::Args{a.x, a.weight, a.x_ld, a.y, a.y_ld, a.M, a.C, a.H, 0, e}, s);
+  return few::run<T, TO>(few::Args{a.x, a.weight, a.x_ld, a.y, a.y_ld, a.M, a.C, a.H, 1, 0, e}, s);
 }
 
 }  // namespace

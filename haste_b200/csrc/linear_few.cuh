@@ -20,7 +20,7 @@ struct Args {
   long long x_ld;
   void* y;
   long long y_ld;
-  int M, C, H, per;  // per: values of C that a block takes
+  int M, C, H, splits, per;  // splits: blocks that share C out, `per` values each
   Epilogue e;
 };
 
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const Args a) {
   constexpr int V = S::V, STEP = S::STEP, TOK = S::TOK, RT = S::RT, ROWS = S::ROWS, AHEAD = S::AHEAD;
   __shared__ float sums[WARPS][TOK][ROWS + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int splits = gridDim.x, split = blockIdx.x, h0 = blockIdx.y * ROWS;  // (a cluster is a row of blocks)
+  const int splits = a.splits, split = blockIdx.x % splits, h0 = blockIdx.x / splits * ROWS;  // (those blocks are a cluster)
   const int c0 = split * a.per, c1 = min(a.C, c0 + a.per);
   const T* w = static_cast<const T*>(a.w) + (long long)(h0 + g) * a.C;
   const T* x = static_cast<const T*>(a.x);
@@ -170,9 +170,10 @@ int launch(Args a, cudaStream_t s) {
   const int tiles = ceil_div(a.H, S::ROWS);
   int splits = 1;
   while (splits < 8 && splits * tiles < 2 * sm_count() && a.C / (2 * splits) >= WARPS * S::STEP * S::AHEAD) splits *= 2;
+  a.splits = splits;
   a.per = ceil_div(ceil_div(a.C, splits), S::V) * S::V;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits, tiles);
+  cfg.gridDim = dim3(splits * tiles);
   cfg.blockDim = dim3(WARPS * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

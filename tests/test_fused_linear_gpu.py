@@ -252,6 +252,18 @@ def test_graphs_and_streams_share_nothing(M, C, H):
         assert all(torch.equal(p, q) for p, q in zip(a, o))
 
 
+@pytest.mark.parametrize("M", [2, 40])
+@pytest.mark.parametrize("C,H", [(8, (1 << 20) - 1), ((1 << 20) - 1, 8)])
+def test_the_most_inputs_and_outputs(C, H, M):
+    """Ones, whose sums are exact: at most 2^20."""
+    from haste_b200 import ssm
+    x, w = torch.ones(M, C, device="cuda", dtype=BF16), torch.ones(H, C, device="cuda", dtype=BF16)
+    w[-1] = 2
+    residual = torch.zeros(M, H, device="cuda")
+    y = ssm.fused_linear(x, w, residual=residual)
+    assert (y[:, :-1] == C).all() and (y[:, -1] == 2 * C).all()
+
+
 def test_more_elements_than_32_bits_count():
     from haste_b200 import ssm
     M, C, H = 1050000, 8, 2056

@@ -83,6 +83,7 @@ def test_gated_scan_step_refuses():
     (dict(weight=z(6)), ValueError, "2 dimensions"),
     (dict(weight=z(6, 5)), ValueError, "weight must be"),
     (dict(weight=z(0, 4)), ValueError, "weight must have"),
+    (dict(weight=z(1 << 20, 4)), ValueError, "weight must have"),
     (dict(x=z(5, 2, 0), weight=z(6, 0)), ValueError, "weight must have"),
     (dict(weight=z(6, 4, dtype=torch.bfloat16)), TypeError, "weight must be"),
     (dict(bias=z(4)), ValueError, "bias must be"),
