@@ -435,8 +435,8 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
  *   x [M,C], residual, y [M,H]: rows x_ld, residual_ld, y_ld elements apart, elements of a row next to each other
  *   weight [H,C] dense, dtype; C and H are 1 to 2^20 - 1, M is at most 2^30   bias [H] param_dtype (F32 or dtype; may be NULL)
  *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y.
- *   pre [M,H] dense, dtype: the sums with bias, written for the backward pass; NULL if there will be none, or if
- *   activation is HASTE_B200_IDENTITY.
+ *   pre [M,H] dense, dtype: the sums with bias, written for the backward pass (where one is infinite, or beyond dtype's
+ *   range, slopes are their limits, 0 or 1); NULL if there will be none, or if activation is HASTE_B200_IDENTITY.
  * backward: dy [M,H] out_dtype, rows dy_ld apart; writes dx [M,C] (rows dx_ld apart; may be NULL), dweight [H,C] (may be
  * NULL) in dtype and dbias [H] in param_dtype (may be NULL).  The residual's gradient is dy.
  * scratch: haste_b200_linear_scratch() bytes, aligned to 256, asked for with all other members set (backward: dx,
