@@ -287,7 +287,8 @@ struct Early {
         if (n + j * 8 < p.N) bias[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(e.bias) + n + j * 8));
     }
   }
-  // rows i * 4 + lane / 8, word lane % 8
+  // rows i * 4 + lane / 8, word lane % 8.  (Plain loads: the residual may be y's own buffer, each word of which the lane that
+  // stores it has read before.)
   __device__ __forceinline__ void ask_residual(const Params& p, const Epilogue& e, int m0, int n) {
     if (!e.residual) return;
     const int lane = threadIdx.x & 31, c = n + (lane & 7) * V;
@@ -295,7 +296,7 @@ struct Early {
     for (int i = 0; i < 8; ++i) {
       const int r = i * 4 + (lane >> 3);
       if (m0 + r < p.M && c < p.N)
-        res[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const TO*>(e.residual) + (long long)(m0 + r) * e.ld_res + c));
+        res[i] = *reinterpret_cast<const uint4*>(static_cast<const TO*>(e.residual) + (long long)(m0 + r) * e.ld_res + c);
     }
   }
   __device__ __forceinline__ void ask(const Params& p, const EP& ep, int m0, int n0) {
@@ -1396,7 +1397,7 @@ void launch_reduce(const float* part, int splits, int M, int N, int ld_part, voi
 // launched while the product is under way, and waits for it.
 template <typename T, typename TO>
 __global__ void __launch_bounds__(256) projection_reduce_kernel(const float* __restrict__ part, int splits, int M, int N, int ld_part,
-                                                                int wide, TO* __restrict__ c, long long ldc, const Epilogue e) {
+                                                                int wide, TO* c, long long ldc, const Epilogue e) {
   const unsigned quads = ld_part / 4, total = (unsigned)M * quads;
   const long long stride = (long long)M * ld_part;
   asm volatile("griddepcontrol.wait;" ::: "memory");

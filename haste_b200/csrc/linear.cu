@@ -157,6 +157,7 @@ int check(const haste_b200_linear& a, bool backward) {
       HB_REQUIRE(!a.dx || a.dx_ld >= a.C, "dx_ld");
     } else {
       HB_REQUIRE(a.y && a.y_ld >= a.H && (!a.residual || a.residual_ld >= a.H), "null pointer");
+      HB_REQUIRE(a.residual != a.y || a.residual_ld == a.y_ld || a.M == 1, "a residual in y's place has its rows");
     }
   }
   return HASTE_B200_OK;

@@ -434,7 +434,7 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
  * accurate to fp32 rounding).  No counterpart in the reference, whose layers project inside.
  *   x [M,C], residual, y [M,H]: rows x_ld, residual_ld, y_ld elements apart, elements of a row next to each other
  *   weight [H,C] dense, dtype; C and H are 1 to 2^20 - 1, M is at most 2^30   bias [H] param_dtype (F32 or dtype; may be NULL)
- *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y.
+ *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y, with the same rows.
  *   pre [M,H] dense, dtype: the sums with bias, written for the backward pass (where one is infinite, or beyond dtype's
  *   range, slopes are their limits, 0 or 1); NULL if there will be none, or if activation is HASTE_B200_IDENTITY.
  * backward: dy [M,H] out_dtype, rows dy_ld apart; writes dx [M,C] (rows dx_ld apart; may be NULL), dweight [H,C] (may be
