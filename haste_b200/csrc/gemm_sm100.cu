@@ -1064,6 +1064,10 @@ struct SplitJob {
   long long ld_dst = 0, plane_stride = 0;
   int vec_ok = 0;
 };
+__device__ __forceinline__ float within_bf16(float v) {  // (a NaN stays)
+  asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(v) : "f"(-0x1.fep127f), "f"(0x1.fep127f));
+  return v;
+}
 template <int PLANES, typename TS>
 __device__ __forceinline__ void split_planes(const SplitJob& job0, const SplitJob& job1) {
   const SplitJob& job = blockIdx.y ? job1 : job0;
@@ -1099,8 +1103,13 @@ __device__ __forceinline__ void split_planes(const SplitJob& job0, const SplitJo
     __nv_bfloat16* dp = dst + r * ld_dst + c;
 #pragma unroll
     for (int pl = 0; pl < PLANES; ++pl) {
-      __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]);
-      __nv_bfloat162 b = __floats2bfloat162_rn(x[2], x[3]);
+      float y[4] = {x[0], x[1], x[2], x[3]};
+      // (Three planes hold all of a finite value: the first as bf16's largest where it would round to an infinity.)
+      if (PLANES == 3 && pl == 0)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = within_bf16(x[j]);
+      __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]);
+      __nv_bfloat162 b = __floats2bfloat162_rn(y[2], y[3]);
       uint2 w;
       w.x = *reinterpret_cast<uint32_t*>(&a);
       w.y = *reinterpret_cast<uint32_t*>(&b);

@@ -247,8 +247,10 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
 
     x [...,C], weight [H,C] (as torch.nn.Linear has it) in x's type, bias [H] in that type or float32, residual [...,H]
     in that type or float32, which is then the result's.  `activation` is None, "relu", "silu", "gelu" (x times the
-    normal distribution), "tanh" or "sigmoid".  Sums are float32; float32 inputs are multiplied to float32's rounding (an
-    infinite one makes NaN of its row's or column's sums).  Rows may lie at any distance, and time-major views of batch-first tensors are read as they lie."""
+    normal distribution), "tanh" or "sigmoid".  Sums are float32.  float32 inputs are multiplied to float32's
+    rounding, those below 2^-102 to within 2^-126; an infinite one makes NaN of its row's or column's sums from nine rows on
+    and in gradients, what the formula has in up to eight.  Rows may lie at any distance, and time-major views of batch-first
+    tensors are read as they lie."""
     if activation not in ops.ACTIVATIONS:
         raise ValueError(f"haste_b200: activation must be one of {list(ops.ACTIVATIONS)}, got {activation!r}")
     if _shown():

@@ -431,7 +431,9 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
 
 /* ---- Projections ---------------------------------------------------------- */
 /* y[m,h] = act(sum_c x[m,c] weight[h,c] + bias[h]) + residual[m,h], on the tensor cores, sums in fp32 (fp32 operands:
- * accurate to fp32 rounding).  No counterpart in the reference, whose layers project inside.
+ * accurate to fp32 rounding, those below 2^-102 to within 2^-126; an infinite one makes NaN of its row's or column's sums
+ * from nine rows on and in gradients, what the formula has in up to eight).  No counterpart in the reference, whose
+ * layers project inside.
  *   x [M,C], residual, y [M,H]: rows x_ld, residual_ld, y_ld elements apart, elements of a row next to each other
  *   weight [H,C] dense, dtype; C and H are 1 to 2^20 - 1, M is at most 2^30   bias [H] param_dtype (F32 or dtype; may be NULL)
  *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y, with the same rows.
