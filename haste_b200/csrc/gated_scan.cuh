@@ -84,6 +84,15 @@ __device__ __forceinline__ float at_most(float v, float most) {  // (a NaN stays
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
   return r;
 }
+// A decay is an exponential and never zero: where it, or a product of them, rounds to zero, float's smallest number stands
+// for it.  So an infinite state stays infinite however the sequence is cut, where zero times it would be a NaN, and a finite one
+// is off by 2^-149 of itself at most, as its product's rounding is.
+__device__ __forceinline__ float not_zero(float v) {  // (a NaN stays)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0x1p-149f));
+  return r;
+}
+__device__ __forceinline__ float2 not_zero(float2 v) { return make_float2(not_zero(v.x), not_zero(v.y)); }
 template <int V, typename F>
 __device__ __forceinline__ float2 each(float2 v, const F& f) {
   return make_float2(f(v.x), V == 2 ? f(v.y) : 0.f);
@@ -153,7 +162,7 @@ __device__ __forceinline__ void decays(float2 l, bool far, float2& a, float2& n)
   }
   a = make_float2(n.x + 1.f, n.y + 1.f);
   if (far) {
-    const float2 e = each<V>(l, [](float x) { return exp2_fast(x); });
+    const float2 e = each<V>(l, [](float x) { return not_zero(exp2_fast(x)); });
     const bool x = l.x < -0.505f, y = l.y < -0.505f;
     a = make_float2(x ? e.x : a.x, y ? e.y : a.y);
     n = make_float2(x ? e.x - 1.f : n.x, y ? e.y - 1.f : n.y);
@@ -225,7 +234,7 @@ __device__ __forceinline__ float2 fold_pieces(const float2* first, int count, lo
   for (int i = warp * each; i < min(count, (warp + 1) * each); ++i) {
     const float2 *q = first + i * step, x = q[0], y = V == 2 ? q[V - 1] : both(0.f);
     e = __ffma2_rn(make_float2(x.x, y.x), e, make_float2(x.y, y.y));
-    p = __fmul2_rn(p, make_float2(x.x, y.x));
+    p = not_zero(__fmul2_rn(p, make_float2(x.x, y.x)));
   }
   shared[warp][lane] = make_float4(p.x, p.y, e.x, e.y);
   __syncthreads();
@@ -314,6 +323,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
       e = __ffma2_rn(s[j], e, b[j]);
       p = __fmul2_rn(p, s[j]);
     }
+    p = not_zero(p);
     pairs[k & 1][seg][lane] = make_float4(p.x, p.y, e.x, e.y);
     __syncthreads();
     if constexpr (Ends) {
@@ -322,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) gated_fwd(Args<T> a) {
         for (int q = 0; q < SEG; ++q) {
           const float4 w = pairs[k & 1][q][lane];
           h = __ffma2_rn(make_float2(w.x, w.y), h, make_float2(w.z, w.w));
-          total = __fmul2_rn(total, make_float2(w.x, w.y));
+          total = not_zero(__fmul2_rn(total, make_float2(w.x, w.y)));
         }
     } else {
       h = k ? behind[(k - 1) & 1][lane] : start;
@@ -502,6 +512,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
       if (!Ends) e = __ffma2_rn(s[j], e, b[j]);
       p = __fmul2_rn(p, s[j]);
     }
+    p = not_zero(p);
 #pragma unroll
     for (int j = L - 1; j >= 0; --j) m = __fmul2_rn(s[j], __fadd2_rn(dy[j], m));
     pairs[k & 1][seg][lane] = make_float4(p.x, p.y, e.x, e.y);
@@ -513,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
         for (int q = SEG - 1; q >= 0; --q) {
           const float4 w = pairs[k & 1][q][lane];
           mu = __ffma2_rn(make_float2(w.x, w.y), mu, backs[k & 1][q][lane]);
-          total = __fmul2_rn(total, make_float2(w.x, w.y));
+          total = not_zero(__fmul2_rn(total, make_float2(w.x, w.y)));
         }
     } else {
       for (int q = 0; q < seg; ++q) {
