@@ -32,8 +32,8 @@ def grad_norm(gradients):
 
 def clip_gradients(gradients, max_norm, out=None):
     """Scales the gradients so that their norm is at most `max_norm` (a factor of 1 where that is infinite), in place or,
-    where given, into `out`: tensors of the same shapes and strides, of any of the three types.  No two may overlap in
-    memory; in place, a tensor that is listed twice counts once.  Returns the norm before.
+    where given, into `out`: tensors of the same shapes that lie in memory alike, of any of the three types.  No two may
+    overlap in memory; in place, a tensor that is listed twice counts once.  Returns the norm before.
 
     A norm that is not finite scales as the formula says: an infinite one to zero (infinite values to NaN), NaN to NaN."""
     if out is not None:

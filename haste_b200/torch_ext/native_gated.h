@@ -321,6 +321,12 @@ haste_b200_gradient range_of(const Tensor& t, const char* name) {
     refuse(std::string(name) + " must fill one range of memory each, got strides over " + shape_of(t));
   return {ptr(t), ptr(t), (long long)t.numel(), dtype, dtype};
 }
+// Whether the elements of two tensors of one shape lie in the same order (an axis of one element has any stride).
+bool lies_like(const Tensor& a, const Tensor& b) {
+  for (int64_t i = 0; a.numel() > 1 && i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
 struct Span {
   const char *from, *to;
   int gradient;  // number, or -1 - number of an output
@@ -367,7 +373,7 @@ Tensor clip_gradients(const std::vector<Tensor>& gradients, const c10::optional<
     const Tensor& o = (*out)[i];
     if (o.sizes() != gradients[i].sizes()) refuse("out must have the gradients' shapes, got " + shape_of(o) + " for " + shape_of(gradients[i]));
     const haste_b200_gradient to = range_of(o, "out");
-    if (o.numel() > 1 && o.strides() != gradients[i].strides()) refuse("out must lie in memory like the gradients");
+    if (!lies_like(o, gradients[i])) refuse("out must lie in memory like the gradients");
     g.back().out = const_cast<void*>(to.data);
     g.back().out_dtype = to.dtype;
   }

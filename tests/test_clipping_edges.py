@@ -1,0 +1,28 @@
+"""Gradient clipping: what a call takes and refuses, without a GPU, and the same on one."""
+import pytest
+import torch
+
+
+LAYOUTS = [lambda: (torch.ones(4, 1), torch.empty(1, 4).t()), lambda: (torch.ones(1, 5, 3), torch.empty(5, 1, 3).transpose(0, 1)),
+           lambda: (torch.ones(3, 1, 2).transpose(0, 1), torch.empty(1, 3, 2)), lambda: (torch.ones(6, 2).t()[None], torch.empty(6, 2).t()[None])]
+
+
+@pytest.mark.parametrize("make", LAYOUTS)
+def test_axes_of_one_element_have_any_stride(make):
+    """(The check behind the one of strides is what refuses tensors that are not on a GPU.)"""
+    from haste_b200 import gradients
+    g, out = make()
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        gradients.clip_gradients([g], 1.0, out=[out])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", LAYOUTS)
+def test_axes_of_one_element_on_a_gpu(make):
+    from haste_b200 import gradients
+    g, out = make()
+    dev = [torch.empty_strided(t.shape, t.stride(), device="cuda").copy_(t) for t in (g, out)]
+    norm = gradients.clip_gradients([dev[0]], 0.5, out=[dev[1]])
+    want = dev[0] * (0.5 / (norm + 1e-6))
+    # six roundings: the norm, its sum, the division and the product here, the factor and the product there
+    assert torch.allclose(dev[1], want, rtol=6 * 2.0 ** -24, atol=0)
