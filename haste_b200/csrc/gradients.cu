@@ -303,6 +303,7 @@ int check(const haste_b200_gradient* g, int count, bool writes, const float* nor
     HB_REQUIRE(storage_dtype(g[i].out_dtype), "out_dtype");
     HB_REQUIRE(g[i].out || g[i].numel == 0, "null pointer");
     HB_REQUIRE(aligned(g[i].out, size_of(g[i].out_dtype)), "misaligned output");
+    HB_REQUIRE(g[i].out != g[i].data || g[i].out_dtype == g[i].dtype || g[i].numel == 0, "in place a gradient keeps its own type");
   }
   return HASTE_B200_OK;
 }

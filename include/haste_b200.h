@@ -472,8 +472,8 @@ long long haste_b200_linear_scratch(const haste_b200_linear* args, int backward)
 /* norm = sqrt(sum over all gradients of their squares);  out = data * min(1, max_norm / (norm + 1e-6)), with a factor
  * of 1 where max_norm is infinite.  No counterpart in the reference.
  * `gradients` is host memory, read before the call returns; data, out and norm (one float) are on the device.  A
- * gradient is `numel` elements that lie next to each other; out (of out_dtype) may be data itself, and must otherwise
- * overlap no gradient and no other out.  A norm that is not finite scales as the formula says: infinite ones to zero
+ * gradient is `numel` elements that lie next to each other; out (of out_dtype) may be data itself, of its own type, and
+ * must otherwise overlap no gradient and no other out.  A norm that is not finite scales as the formula says: infinite ones to zero
  * (and infinite values to NaN), a NaN to NaN.  scratch: haste_b200_grad_norm_scratch() floats, aligned to 8 bytes.
  * The calls allocate nothing, keep nothing and may be captured. */
 typedef struct {

@@ -1,6 +1,12 @@
 """Gradient clipping: what a call takes and refuses, without a GPU, and the same on one."""
+import ctypes
+
 import pytest
 import torch
+
+
+class Gradient(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_longlong), ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
 
 
 LAYOUTS = [lambda: (torch.ones(4, 1), torch.empty(1, 4).t()), lambda: (torch.ones(1, 5, 3), torch.empty(5, 1, 3).transpose(0, 1)),
@@ -26,3 +32,15 @@ def test_axes_of_one_element_on_a_gpu(make):
     want = dev[0] * (0.5 / (norm + 1e-6))
     # six roundings: the norm, its sum, the division and the product here, the factor and the product there
     assert torch.allclose(dev[1], want, rtol=6 * 2.0 ** -24, atol=0)
+
+
+def test_another_type_in_place_is_refused():
+    """Through the C ABI: elements of another type do not lie where the gradient's do."""
+    from haste_b200 import _C
+    L = _C.lib()
+    memory = (ctypes.c_char * 64)()
+    at = ctypes.addressof(memory) + -ctypes.addressof(memory) % 16
+    for dtype, out_dtype in ((0, 1), (1, 0), (1, 2), (2, 1)):
+        g = Gradient(at, at, 4, dtype, out_dtype)
+        assert L.haste_b200_clip_gradients(ctypes.byref(g), 1, 1.0, at, at, None) == 1
+        assert b"own type" in L.haste_b200_last_error()
