@@ -51,7 +51,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     grads = [p.grad for p in parameters]
     grads = [g for g in grads if g is not None]
     if error_if_nonfinite and grads:
-        norm = grad_norm(grads)
+        norm = grad_norm(list({id(g): g for g in grads}.values()))
         if not torch.isfinite(norm):
             raise RuntimeError(f"haste_b200: the norm of the gradients is {norm.item()}; they are not clipped")
     return _native().clip_gradients(grads, max_norm, None) if grads else torch.zeros(())

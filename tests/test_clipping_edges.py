@@ -44,3 +44,13 @@ def test_another_type_in_place_is_refused():
         g = Gradient(at, at, 4, dtype, out_dtype)
         assert L.haste_b200_clip_gradients(ctypes.byref(g), 1, 1.0, at, at, None) == 1
         assert b"own type" in L.haste_b200_last_error()
+
+
+@pytest.mark.gpu
+def test_a_parameter_listed_twice_counts_once_for_its_norm_too():
+    """3e38 is finite; twice its square has a root beyond float32."""
+    import haste_b200
+    p = torch.nn.Parameter(torch.zeros(1, device="cuda"))
+    p.grad = torch.full((1,), 3e38, device="cuda")
+    norm = haste_b200.clip_grad_norm_([p, p], 1.0, error_if_nonfinite=True)
+    assert norm.item() == p.grad.new_tensor(3e38).item() and abs(p.grad.item() - 1) < 1e-6
