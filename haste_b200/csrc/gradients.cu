@@ -104,22 +104,26 @@ __device__ __noinline__ double wide_squares(const T* base, long long first, long
 }
 
 // A thread's squares are added in float32, and once more in 64 bits where that over- or underflows.  Sums of threads
-// are 64 bits, in a fixed order.
+// are 64 bits, in a fixed order.  (Words of zeros have no squares that underflow.)
 template <typename T>
 __device__ __forceinline__ double squares(const Entry& e, int chunk) {
   const Words<T> words(e, chunk);
   constexpr int V = Words<T>::V;
   float s[4] = {};
+  uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < LOADS; ++k) {
     float v[V];
+#pragma unroll
+    for (uint32_t w : words.w[k].w) bits |= w;
     unpack<T, V>(words.w[k], v);
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j % 4] = fmaf(v[j], v[j], s[j % 4]);
   }
   double sum = (s[0] + s[1]) + (s[2] + s[3]);
   const T* base = static_cast<const T*>(e.data) - e.pad;
-  if (!(sum > 1e-20 && sum < 1e30)) sum = wide_squares<T>(base, words.first, e.pad, words.end);
+  constexpr uint32_t SIGNS = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+  if (!(sum > 1e-20 && sum < 1e30) && (bits & ~SIGNS)) sum = wide_squares<T>(base, words.first, e.pad, words.end);
   words.edges([&](long long i) {
     const double v = ld(base + i);
     sum = fma(v, v, sum);

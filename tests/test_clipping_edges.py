@@ -54,3 +54,17 @@ def test_a_parameter_listed_twice_counts_once_for_its_norm_too():
     p.grad = torch.full((1,), 3e38, device="cuda")
     norm = haste_b200.clip_grad_norm_([p, p], 1.0, error_if_nonfinite=True)
     assert norm.item() == p.grad.new_tensor(3e38).item() and abs(p.grad.item() - 1) < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_zeros_of_either_sign_beside_values_whose_squares_vanish(dtype):
+    from haste_b200 import gradients
+    zeros = torch.zeros(70001, device="cuda", dtype=dtype)
+    zeros[::2] *= -1
+    assert gradients.grad_norm([zeros, zeros[:3]]).item() == 0
+    small = torch.finfo(dtype).smallest_normal
+    some = zeros.clone()
+    some[4321], some[70000], some[1] = small, -small, small
+    want = small * 3 ** 0.5
+    assert abs(gradients.grad_norm([zeros, some, zeros]).item() - want) <= 2.0 ** -24 * want + 2.0 ** -149
