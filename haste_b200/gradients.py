@@ -4,10 +4,11 @@
     norm = gradients.clip_gradients(grads, 1.0, out=masters)     # scales into other tensors, of other types
     norm = gradients.grad_norm(grads)
 
-norm = sqrt(sum of squares over all tensors), a float32 scalar on their device, summed in 64 bits in a fixed order, so
-that neither large nor small gradients leave float32's range on the way; gradients are multiplied by
-min(1, max_norm / (norm + 1e-6)).  Tensors are float32, bfloat16 or float16, in any mixture, on one GPU, and fill one
-range of memory each, in any order of axes.  The calls run on the current stream, never wait for the device (unless
+norm = sqrt(sum of squares over all tensors), a float32 scalar on their device.  Up to 64 squares at a time are added in float32,
+again in 64 bits where their sum leaves 1e-20 to 1e30, so that neither large nor small gradients leave float32's range on the
+way; those sums are added in 64 bits, in a fixed order.  The norm is within 10.5 roundings of float32 (2^-24 each).  Gradients
+are multiplied by min(1, max_norm / (norm + 1e-6)).  Tensors are float32, bfloat16 or float16, in any mixture, on one GPU, and
+fill one range of memory each, in any order of axes.  The calls run on the current stream, never wait for the device (unless
 `error_if_nonfinite` asks for it), and may be captured in graphs.  The reference has no counterpart of them.
 """
 import torch
