@@ -33,7 +33,10 @@ int check(const haste_b200_gated_scan& a, bool backward) {
 
 int dispatch(const haste_b200_gated_scan& a, bool backward, cudaStream_t s) {
   HB_TRY(check(a, backward));
-  if (a.N == 0 || a.D == 0) return HASTE_B200_OK;
+  if (a.N == 0 || a.D == 0) {  // (of no rows the decay's gradient is zero)
+    if (backward && a.decay && a.ddecay && a.D > 0) HB_CUDA_OK(cudaMemsetAsync(a.ddecay, 0, (size_t)a.D * 4, s));
+    return HASTE_B200_OK;
+  }
   ProfScope p(backward ? PH_REC_BWD : PH_REC_FWD, s);
   if (a.dtype == HASTE_B200_F32) return run<float>(a, backward, s);
   if (a.dtype == HASTE_B200_BF16) return run<__nv_bfloat16>(a, backward, s);

@@ -89,7 +89,6 @@ std::vector<OptTensor> gated_scan_backward(const Tensor& x, const Tensor& gate, 
   if (c.inner.defined()) dinner = output(c.inner);
   if (c.decay.defined()) ddecay = at::empty_like(c.decay);
   if (c.state.defined()) ds = at::empty_like(c.state);
-  if ((!c.a.N || !c.a.D) && ddecay.defined()) ddecay.zero_();
   c.a.dy = view(dy); c.a.dx = view(dx); c.a.dgate = view(dgate); c.a.dinput_gate = view(dinner);
   c.a.checkpoints = data<float>(saved);
   c.a.dfinal_state = data<float>(dfinal);
