@@ -252,7 +252,7 @@ __device__ __forceinline__ float2 fold_pieces(const float2* first, int count, lo
 // zero), the warps' pairs meet in shared memory, each warp folds those in front of its own into the tile's starting state,
 // and walks its steps again from registers.  One barrier a tile: pairs and the state behind the tile have two buffers.
 // The next tile's words are under way from when the present ones have been used.
-// bf16 1000 x 64 x 1024 with both gates: 129 us, 4.1 TB/s; with the sigmoids, series and root left out 99 us, which is what
+// bf16 1000 x 64 x 1024 with both gates: 129 us, 4.1 TB/s (fp32 161, 6.5 TB/s, at the copy bandwidth); with the sigmoids, series and root left out 99 us, which is what
 // the accesses and barriers take.  Eight steps a warp and blocks of 256 threads 135 us (fewer instructions, but 3.5 blocks
 // an SM to share out); words copied to shared memory tiles ahead 142; one reciprocal for both gates 129.
 //
@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(256) gated_step(Args<T> a) {
 // the one that the forward pass left in front of it; a segment is a pair for the states, and for the adjoint
 // mu = a lam, which runs the other way, the same product and a third number.
 // Ends: pieces but the first leave (product, mu that they give to one of zero behind them).
-// bf16 1000 x 64 x 1024 with both gates: 233 us, 3.9 TB/s, bound by what 16 warps an SM issue next to each other (0.6 of the
-// slots): a step's numbers fill 128 registers a thread.  Five blocks an SM spill (629 us), blocks of 256 threads 242.
+// bf16 1000 x 64 x 1024 with both gates: 227 us, 4.0 TB/s (by itself, from a cold L2, 234), bound by what 16 warps an SM issue
+// next to each other (0.6 of the slots): a step's numbers fill 128 registers a thread; fp32 350 us, 5.2 TB/s.  Five blocks an SM spill (629 us), blocks of 256 threads 242.
 template <typename T, int V, bool Decay, bool In, bool Ends>
 __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
   constexpr int L = BWD_L, TT = BWD_TT;
@@ -598,8 +598,10 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) gated_bwd(Args<T> a) {
 // Pieces of the sequence: none while the channels make blocks enough (two an SM; backward, which keeps four on an SM where
 // the forward pass keeps seven, one and a half), else as many as make seven an SM (four: bf16 1000 x 8 x 1024 47 us,
 // backward 62), of a tile at least and three times the root of the steps at most, beyond which folding them takes longer than
-// walking them (bf16 16000 x 1 x 64, backward: without that bound 40 / 38 us, with it 21 / 24).  us, whole / in pieces, both
-// gates, bf16 1000 x N x 1024: N = 8 forward 70 / 39, backward 86 / 51; 16 78 / 66, 96 / 100; 32 92 / 111, 128 / 172; fp32
+// walking them.  Forward / backward in us with once, twice, three times, 4.5 times the root and without a bound: bf16 4000 x 1 x 256
+// 12.8 / 15.5, 11.2 / 12.9, 11.2 / 12.9, 13.7 / 17.8, the same; 16000 x 1 x 64 20.6 / 22.5, 15.9 / 17.7, 15.5 / 17.4, 17.3 / 18.4,
+// 31.4 / 30.8; fp32 23.9 / 27.6, 19.4 / 20.8, 19.3 / 20.1, 23.0 / 20.9, 39.4 / 31.5; bf16 64000 x 1 x 64 40.0 / 42.0, 31.8 / 34.0,
+// 35.8 / 39.3, 42.1 / 45.6, the same.  us, whole / in pieces, both gates, bf16 1000 x N x 1024: N = 8 forward 70 / 39, backward 86 / 51; 16 78 / 66, 96 / 100; 32 92 / 111, 128 / 172; fp32
 // 2000 x 1 x 1024 162 / 17, 221 / 26; bf16 100 x 8 x 1024 14 / 12, 18 / 17.
 inline int pieces_of(const haste_b200_gated_scan& a, int V, bool backward) {
   const long long blocks = (long long)a.N * ceil_div(a.D, 32 * V), sms = sm_count();

@@ -267,7 +267,8 @@ __device__ __forceinline__ void store_projection(const Params& p, const Epilogue
 // Bias and residual are asked for a step ahead, those of the next tile (next_m, next_n; beyond the matrix where there is none)
 // with the last step.  buf: two tiles of 4 KB.
 // (bf16 64000 x 2048, K = 1024, SiLU / with p / residual alone: 215 / 240 / 268 us; bulk stores for all 213 / 245 / 316, lanes
-// for all 228 / 271 / 248; the sums themselves through shared memory, and accesses of four elements behind it, 401 / 428.)
+// for all 228 / 271 / 248.  Outputs that are no multiple of eight go through shared memory as sums, in accesses of four elements
+// behind it, or of one (store_projection): 2044 of them 288 / 332, 2047 928 / 1014.)
 template <typename EP>
 struct Early {
   typedef typename EP::T T;

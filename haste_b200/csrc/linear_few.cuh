@@ -55,9 +55,11 @@ __device__ __forceinline__ Raw<T, 16 / (int)sizeof(T)> load16(bool ok, const T* 
 // rows g and g + 8 of each 16 and 16 bytes of each, 32 (fp32: 16) values of C to the four t's.  The order of C in a product is free,
 // so those bytes are used as the registers of two matrix instructions (k = 2t, 2t + 1, 2t + 8, 2t + 9) as they lie, with x
 // the same way.  MT tiles of eight tokens.  fp32 multiplies on the FMA units.
-// x comes from L2 once for every RT 16 rows: from 17 tokens on two.  bf16, us: 1 x 1024, H = 4096 6.3 (8.4 MB: 1.3 at the copy
-// bandwidth, and about 2.5 for a launch and its first loads), 32 tokens 8.4; 1 x 4096, H = 4096 11.3 (33.6 MB: 5.1), 32 18.1.
-// 64 tokens in this way 29 and 53, where the tensor cores with K split take 12 and 18.
+// x comes from L2 once for every RT 16 rows: from 17 tokens on two.  bf16, us by itself: 1 x 1024, H = 4096 6.3 (8.4 MB: 1.3 at
+// the copy bandwidth, and about 2.5 for a launch and its first loads), 32 tokens 8.4; 1 x 4096, H = 4096 11.3 (33.6 MB: 5.1), 32
+// 18.1.  64 tokens in this way 29 and 53, where the tensor cores with K split take 12 and 18.  What 32 tokens wait for: a step's
+// loads are issued together, and the next step's only when they have been multiplied.  fp32 in a graph, 1 / 8 tokens x 4096, H =
+// 4096: 22.2 / 32.4 (67 MB: 10.2); nine, through the tensor cores with the weight split into planes, 58.8.
 // The warps' sums meet in shared memory, the blocks' of a cluster in the shared memory of each, rows shared out.
 template <typename T, int MT, bool Wide, typename TO>
 struct Shape {

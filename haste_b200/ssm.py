@@ -204,7 +204,8 @@ def gated_scan(x, gate, decay=None, input_gate=None, initial_state=None, lengths
     h_t = a_t h_{t-1} + w_t x_t sigmoid(input_gate_t).  Returns (h of every step, final_state).
 
     x, gate, input_gate [T,N,D] have one type; decay [D] has any and is taken as float32, values above zero count as
-    zero; `initial_state` [N,D] float32 (zeros without it)."""
+    zero; `initial_state` [N,D] float32 (zeros without it).  In gradients 1 / w is taken as 1 / sqrt(w^2 + 1e-30), and a
+    decay of zero leaves w constant."""
     if lengths is not None:
         lengths = _lengths(lengths, x)
     decay = _float(decay)
@@ -247,10 +248,10 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
 
     x [...,C], weight [H,C] (as torch.nn.Linear has it) in x's type, bias [H] in that type or float32, residual [...,H]
     in that type or float32, which is then the result's.  `activation` is None, "relu", "silu", "gelu" (x times the
-    normal distribution), "tanh" or "sigmoid".  Sums are float32.  float32 inputs are multiplied to float32's
-    rounding, those below 2^-102 to within 2^-126; an infinite one makes NaN of its row's or column's sums from nine rows on
-    and in gradients, what the formula has in up to eight.  Rows may lie at any distance, and time-major views of batch-first
-    tensors are read as they lie."""
+    normal distribution), "tanh" or "sigmoid".  Sums are float32; their gradient is rounded to x's type.
+    float32 inputs are multiplied to float32's rounding, those below 2^-110 to within 2^-134; an infinite one makes NaN of
+    its row's or column's sums from nine rows on and in gradients, what the formula has in up to eight.  Rows may lie at any
+    distance, and time-major views of batch-first tensors are read as they lie."""
     if activation not in ops.ACTIVATIONS:
         raise ValueError(f"haste_b200: activation must be one of {list(ops.ACTIVATIONS)}, got {activation!r}")
     if _shown():

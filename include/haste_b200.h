@@ -409,7 +409,7 @@ long long haste_b200_fused_norm_scratch(const haste_b200_fused_norm* args);
  * checkpoints: what the backward pass starts its pieces from, haste_b200_gated_scan_checkpoints() floats; NULL if
  * there will be none.
  * backward: reads checkpoints, dy and dfinal_state; writes dx, dgate, dinput_gate (if input_gate), ddecay (if decay)
- * and dstate (may be NULL).  scratch: haste_b200_gated_scan_scratch() floats, aligned to 8 bytes. */
+ * and dstate (may be NULL); 1 / w is taken as 1 / sqrt(w^2 + 1e-30), and a decay of zero leaves w constant.  scratch: haste_b200_gated_scan_scratch() floats, aligned to 8 bytes. */
 typedef struct {
   int dtype, T, N, D;
   haste_b200_sequence x, gate, input_gate, y;
@@ -431,7 +431,7 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
 
 /* ---- Projections ---------------------------------------------------------- */
 /* y[m,h] = act(sum_c x[m,c] weight[h,c] + bias[h]) + residual[m,h], on the tensor cores, sums in fp32 (fp32 operands:
- * accurate to fp32 rounding, those below 2^-102 to within 2^-126; an infinite one makes NaN of its row's or column's sums
+ * accurate to fp32 rounding, those below 2^-110 to within 2^-134; an infinite one makes NaN of its row's or column's sums
  * from nine rows on and in gradients, what the formula has in up to eight).  No counterpart in the reference, whose
  * layers project inside.
  *   x [M,C], residual, y [M,H]: rows x_ld, residual_ld, y_ld elements apart, elements of a row next to each other
@@ -439,8 +439,9 @@ long long haste_b200_gated_scan_scratch(const haste_b200_gated_scan* args, int b
  *   residual (may be NULL) and y have out_dtype: F32 or dtype.  residual may be the same buffer as y, with the same rows.
  *   pre [M,H] dense, dtype: the sums with bias, written for the backward pass (where one is infinite, or beyond dtype's
  *   range, slopes are their limits, 0 or 1); NULL if there will be none, or if activation is HASTE_B200_IDENTITY.
- * backward: dy [M,H] out_dtype, rows dy_ld apart; writes dx [M,C] (rows dx_ld apart; may be NULL), dweight [H,C] (may be
- * NULL) in dtype and dbias [H] in param_dtype (may be NULL).  The residual's gradient is dy.
+ * backward: dy [M,H] out_dtype, rows dy_ld apart; its product with the slopes is rounded to dtype.  Writes dx [M,C] (rows
+ * dx_ld apart; may be NULL), dweight [H,C] (may be NULL) in dtype and dbias [H] in param_dtype (may be NULL).  The
+ * residual's gradient is dy.
  * scratch: haste_b200_linear_scratch() bytes, aligned to 256, asked for with all other members set (backward: dx,
  * dweight, dbias not NULL if they will be written).  The calls keep nothing and may be captured. */
 #define HASTE_B200_IDENTITY 0
